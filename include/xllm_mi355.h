@@ -550,6 +550,116 @@ int xllm_mi355_decode_metadata_update(const int32_t* src_tokens, const int32_t* 
                                       int64_t actual_batch_size, int64_t actual_indices_size, void* stream);
 
 /*
+ * The tables of a step, built on the GPU from the requests' lengths: block table, positions, slots, lengths.  What the
+ * reference's batch builder derives on the host, request by request, and copies to the device every step
+ * (xllm/core/framework/batch/batch_input_builder.cpp).  No counterpart on the device there.
+ * batch requests hold kv_lens[b] tokens in the cache and bring new_lens[b] more (1 for a decode, a chunk for a prefill, 0
+ * for an idle row; negative lengths count as 0); the step has room for max_new_tokens new tokens.  Requests are served in
+ * order: those behind the budget get fewer tokens or none.  A request keeps the first ceil(kv_lens[b] / block_size)
+ * entries of its row of block_table_in and takes the pages its new tokens need from free_pages, from entry free_head[0] on
+ * (null: 0), request after request.
+ *   block_table_out [batch, out_stride]: kept entries, pages taken, -1 up to table_width.  May be block_table_in itself
+ *                    (same stride): then only the entries behind the kept ones are written
+ *   seq_lens        [batch]: tokens after the step           cu_new_lens [batch + 1]: offsets of the requests' new tokens
+ *   positions       [max_new_tokens] int64, slots [max_new_tokens] int32, packed request after request: position and slot
+ *                   of every new token; 0 and -1 behind the last one
+ *   new_page_indptr [batch + 1]: offsets of the pages taken, relative to free_head
+ *   counters        [3]: tokens of the step; free_head for the next step; tokens that found no page (the free list or the
+ *                   table's width ran out): their slots are -1, and their requests must not attend before they are stored
+ * A slot that would not fit 31 bits, or whose kept entry is negative, is -1 as well.  Outputs must not overlap kv_lens,
+ * new_lens, free_pages or free_head.  max_new_tokens, n_free, table_width and block_size below 2^30, batch up to 2^20.
+ * One launch for up to 1024 requests, two beyond; integer arithmetic only, the same result every time.
+ */
+int xllm_mi355_build_step_tables(const int32_t* kv_lens, const int32_t* new_lens,
+                                 const int32_t* block_table_in, int64_t in_stride,
+                                 int32_t* block_table_out, int64_t out_stride, int64_t table_width,
+                                 const int32_t* free_pages, int64_t n_free, const int32_t* free_head,
+                                 int32_t* seq_lens, int32_t* cu_new_lens, int64_t* positions, int32_t* slots,
+                                 int32_t* new_page_indptr, int32_t* counters,
+                                 int64_t batch, int64_t block_size, int64_t max_new_tokens, void* stream);
+
+/*
+ * cos | sin rows for the rotary entry points of this library, out[r, i] = factor * cos(angle), out[r, half + i] = factor *
+ * sin(angle), angle = position(r) * inv_freq[i], with the angle and its reduction in 64 bits (a 32-bit angle at position
+ * 10^5 is off by 4e-3) and one rounding to out_dtype.  position(r) = positions[r], or first_position + r where positions is
+ * null.  Frequencies scaled for long contexts (the reference's rotary_embedding files in
+ * xllm/core/layers/common/) are the caller's inv_freq and factor; ops.rope_frequencies makes them.
+ * inv_freq: [half] fp64; out: [n_rows, 2 * half] contiguous, of out_dtype (fp32, bf16, fp16).  half up to 4096.
+ */
+int xllm_mi355_rope_cos_sin(const double* inv_freq, const int64_t* positions, int64_t first_position,
+                            int64_t n_rows, int64_t half, double factor, void* out, int out_dtype, void* stream);
+
+/*
+ * Rotary embedding of q and k in tensors of their own (the reference's rotary layers, xllm/core/layers/common/; the fused
+ * qkv form is xllm_mi355_rope_and_cache): dims [rotary_offset, rotary_offset + rotary_dim) of every head are rotated by the
+ * cos | sin row of the token's position, in fp32 with one rounding, the others kept.
+ *   q [n_tokens, n_heads_q, head_dim_q], k [n_tokens, n_heads_k, head_dim_k] (n_heads_k 0: no k), contiguous in the last
+ *   dim; strides = {token, head} in elements (host pointers); q_out / k_out likewise, or q / k themselves with the same
+ *   strides (in place; then only the rotated dims are touched).  Outputs must not overlap inputs otherwise.
+ *   cos_sin [n_positions, rotary_dim] contiguous, cos then sin.  A position outside [0, n_positions) is not rotated.
+ *   interleave  nonzero: pairs (2i, 2i + 1); zero: pairs (i, i + rotary_dim / 2)
+ *   inverse     nonzero: the transposed map (sin negated): undoes a rotation, and is its gradient
+ * dtype: bf16, fp16 or fp32; any even rotary_dim, any alignment (16-byte aligned operands take the fast path).
+ */
+int xllm_mi355_rotary_embedding(const int64_t* positions, const void* cos_sin, int64_t n_positions,
+                                const void* q, void* q_out, const void* k, void* k_out,
+                                int64_t n_tokens, int64_t n_heads_q, int64_t n_heads_k,
+                                int64_t head_dim_q, int64_t head_dim_k,
+                                int64_t rotary_offset_q, int64_t rotary_offset_k, int64_t rotary_dim,
+                                const int64_t* q_strides, const int64_t* q_out_strides,
+                                const int64_t* k_strides, const int64_t* k_out_strides,
+                                int interleave, int inverse, int dtype, int cos_sin_dtype, void* stream);
+
+/*
+ * The MLA layer's prologue in one launch, the counterpart of xllm_mi355_rope_and_cache: the latent norm, the rotation of
+ * the rope key and of the rope part of the queries, and the latent store of the reference's MLA layer
+ * (xllm/core/layers/dcu/deepseek_v2_attention.cpp:221-229 and what precedes it there):
+ *     latent = kv[t, :512] / sqrt(mean(kv[t, :512]^2) + eps) * kv_weight;   pe = rotate(kv[t, 512:576])
+ *     kv_out[t] = cache[slots[t]] = latent | pe;   q_pe_out[t, h] = rotate(q_pe[t, h])
+ * q_pe, q_pe_out [n_tokens, n_heads, 64] with token and head strides (q_pe a slice of the queries; q_pe_out contiguous is
+ * what xllm_mi355_paged_decode_mla reads; it may be q_pe itself), kv, kv_out rows of 576 with a row stride (kv_out null or
+ * kv itself or apart), cache [num_blocks, block_size, 1, 576] or null (one of kv_out and cache is needed).  Slots outside
+ * the cache are skipped; a position outside [0, n_positions) is not rotated.  Arithmetic in fp32, rounded once to dtype
+ * (bf16, fp16).  Pointers and strides multiples of 16 bytes.
+ */
+int xllm_mi355_mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const void* kv, void* kv_out,
+                                       const void* kv_weight, float eps,
+                                       const void* cos_sin, int64_t n_positions, const int64_t* positions,
+                                       void* k_cache, const int32_t* slot_mapping,
+                                       int64_t n_tokens, int64_t n_heads, int64_t d_latent, int64_t d_rope,
+                                       int64_t q_token_stride, int64_t q_head_stride,
+                                       int64_t q_out_token_stride, int64_t q_out_head_stride,
+                                       int64_t kv_row_stride, int64_t kv_out_row_stride,
+                                       int64_t block_size, int64_t num_blocks, int interleave,
+                                       int dtype, int cos_sin_dtype, void* stream);
+
+/*
+ * Paged decode, differential attention: the difference of two softmax maps over the same pages, optionally with the
+ * per-head RMS norm that follows it.  No counterpart in the reference, which has ordinary attention only.
+ *     o = (softmax(sm_scale q[b, 2h] . K[:, 2j]^T) - lambda[b, h] softmax(sm_scale q[b, 2h + 1] . K[:, 2j + 1]^T)) . V[:, j]
+ *     out[b, h] = out_scale * norm_weight * o / sqrt(mean(o^2) + eps)          (norm_weight null: out_scale * o)
+ * with j = h / (n_heads / n_kv_pairs).  q [batch, 2 n_heads, head_dim]; out [batch, n_heads, 2 head_dim]; token strides in
+ * elements.  k_cache [P, bs, 2 n_kv_pairs, head_dim]; v_cache [P, bs, n_kv_pairs, 2 head_dim]: both are the layout of
+ * xllm_mi355_reshape_and_cache (the value cache of 2 n_kv_pairs heads of head_dim holds the same bytes).
+ * lambda: fp32 with strides in elements (0 where a sequence or a head shares it).  norm_weight [2 head_dim] of `dtype`.
+ * block_table [batch, table_stride], of which table_width entries are valid: longer contexts are cut there.  window_left
+ * as in xllm_mi355_paged_decode_gqa.  A sequence with seq_lens[b] <= 0 gets out = 0.  Page ids are clamped into the cache.
+ * dtype (queries, caches, output): bf16 or fp16.  head_dim 64 or 128; any block size.
+ * The workspace needs no initialisation; two calls that overlap in time need one each.
+ */
+size_t xllm_mi355_paged_decode_diff_workspace_bytes(int64_t n_heads, int64_t n_kv_pairs, int64_t head_dim);
+int xllm_mi355_paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, void* out,
+                                 const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                                 const int32_t* seq_lens,
+                                 const float* lambda, int64_t lambda_batch_stride, int64_t lambda_head_stride,
+                                 const void* norm_weight, float eps, float out_scale,
+                                 int64_t batch, int64_t n_heads, int64_t n_kv_pairs, int64_t head_dim,
+                                 int64_t block_size, int64_t num_blocks,
+                                 int64_t q_token_stride, int64_t out_token_stride,
+                                 int64_t window_left, float sm_scale,
+                                 void* workspace, size_t workspace_bytes, int dtype, void* stream);
+
+/*
  * Opt-in timing of the dominant decode kernel.  No counterpart in the reference, which
  * relies on external profilers (xllm/core/platform/cuda_profiler.cpp,
  * xllm/core/platform/torch_profiler.cpp).  After xllm_mi355_profile_enable(n) the next n

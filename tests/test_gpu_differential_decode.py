@@ -1,0 +1,349 @@
+"""Differential paged decode against its definition in 64 bits, and the operators of a step run together."""
+import pytest
+import torch
+
+from xllm_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def problem(lens, H, pairs, D, bs, dtype, seed=0, spread=1.0, garbage=None):
+    """Caches whose used rows are random and whose other rows are `garbage`, with shuffled pages."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    B = len(lens)
+    pages = [-(-L // bs) for L in lens]
+    pool = sum(pages) + 3
+    order = torch.randperm(pool, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+    W = max(max(pages), 1) + 2
+    table, at = torch.full((B, W), 2 ** 30, dtype=torch.int32), 0   # (padding that must never be followed)
+    k = torch.randn(pool, bs, 2 * pairs, D, generator=gen, device=DEV).to(dtype)
+    v = torch.randn(pool, bs, pairs, 2 * D, generator=gen, device=DEV).to(dtype)
+    used = torch.zeros(pool * bs, dtype=torch.bool)
+    for b, n in enumerate(pages):
+        table[b, :n] = order[at:at + n]
+        at += n
+        t = torch.arange(lens[b])
+        used[table[b, t // bs].long() * bs + t % bs] = True
+    if garbage is not None:
+        for c in (k, v):
+            c.view(pool * bs, -1)[~used.to(DEV)] = garbage
+    q = (torch.randn(B, 2 * H, D, generator=gen, device=DEV) * spread).to(dtype)
+    return dict(q=q, k=k, v=v, table=table.to(DEV), lens=torch.tensor(lens, dtype=torch.int32, device=DEV))
+
+
+def reference(p, H, pairs, D, bs, lam, scale, weight, eps, out_scale, window=-1):
+    """(result, bound on the kernel's error) in 64 bits."""
+    B, g = p["q"].shape[0], H // pairs
+    out = torch.zeros(B, H, 2 * D, dtype=torch.float64, device=DEV)
+    bound = torch.zeros_like(out)
+    half = torch.finfo(p["q"].dtype).eps / 2
+    lam = lam.double().expand(B, H) if lam.numel() > 1 or lam.dim() else lam.double().expand(B, H)
+    for b, L in enumerate(p["lens"].tolist()):
+        L = min(L, p["table"].shape[1] * bs)
+        if L <= 0:
+            continue
+        t = torch.arange(0 if window < 0 else max(0, L - 1 - window), L, device=DEV)
+        slot = p["table"][b, t // bs].long() * bs + t % bs
+        k = p["k"].view(-1, pairs, 2, D)[slot].double().repeat_interleave(g, 1)         # [t, H, 2, D]
+        v = p["v"].view(-1, pairs, 2 * D)[slot].double().repeat_interleave(g, 1)        # [t, H, 2 D]
+        q = p["q"][b].double().view(H, 2, D)
+        s = torch.einsum("hmd,thmd->hmt", q, k) * scale
+        a = torch.softmax(s, -1)
+        o1, o2 = (torch.einsum("ht,thd->hd", a[:, m], v) for m in range(2))
+        m1, m2 = (torch.einsum("ht,thd->hd", a[:, m], v.abs()) for m in range(2))
+        l = lam[b][:, None]
+        o = o1 - l * o2
+        # Relative error of a probability: its score is a sum of D exact products in fp32, off by at most
+        # D 2^-24 times the sum of their magnitudes (in log2 units: times 1.4427), then exp2 and the two sums (2^-20
+        # together); p itself is kept as two 16-bit parts (half a step of half a step), or below fp16's normal range to
+        # 2^-25 of the largest.
+        mag = (q.abs()[None] * k.abs()).sum(-1).amax(0) * scale                          # [H, 2]
+        rel = (D * 2.0 ** -24 * mag + 2.0 ** -20 + half * half + 2.0 ** -24 * t.numel() ** 0.5)
+        err = rel[:, :1] * m1 + l.abs() * rel[:, 1:] * m2
+        f = torch.full((H, 1), out_scale, dtype=torch.float64, device=DEV)
+        if weight is not None:
+            rms = (o.square().mean(-1, keepdim=True) + eps).sqrt()
+            shift = err.square().mean(-1, keepdim=True).sqrt() / rms                     # the norm moves with its input
+            f = f * weight.double() / rms
+            err = err + o.abs() * (shift + 2.0 ** -21)
+        out[b] = o * f
+        bound[b] = err * f.abs() * 1.01 + half * (out[b].abs() + err * f.abs())
+    tiny = torch.finfo(p["q"].dtype).smallest_normal * torch.finfo(p["q"].dtype).eps / 2
+    return out, bound + tiny
+
+
+def run(p, H, D, lam, scale=None, weight=None, eps=1e-5, out_scale=1.0, window=-1, out=None):
+    B = p["q"].shape[0]
+    out = torch.full((B, H, 2 * D), 7.0, dtype=p["q"].dtype, device=DEV) if out is None else out
+    ops.batch_decode_diff(p["q"], p["k"], p["v"], out, p["table"], p["lens"], lam, scale=scale, norm_weight=weight, eps=eps,
+                          out_scale=out_scale, window_left=window)
+    return out
+
+
+def check(p, H, pairs, D, bs, lam, scale=None, weight=None, eps=1e-5, out_scale=1.0, window=-1):
+    got = run(p, H, D, lam, scale, weight, eps, out_scale, window)
+    want, bound = reference(p, H, pairs, D, bs, lam, scale or D ** -0.5, weight, eps, out_scale, window)
+    err = (got.double() - want).abs()
+    worst = (err / bound).max().item()
+    assert worst <= 1.0, f"error is {worst:.2f} of its bound (largest {err.max().item():.3e})"
+    return got
+
+
+def lam_of(H, seed=0):
+    return torch.rand(H, generator=torch.Generator().manual_seed(seed)).to(DEV) * 0.6 + 0.2
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,pairs,bs", [
+    ([1], 1, 1, 16), ([17], 2, 1, 16), ([0, 5, 0], 4, 2, 16), ([64, 63, 65, 1], 8, 2, 16), ([300, 7], 9, 1, 64),
+    ([40, 1000], 16, 1, 128), ([100, 333], 10, 5, 24), ([31, 32, 33], 17, 1, 8), ([50, 20], 40, 1, 1), ([2000], 4, 4, 16),
+    ([129, 0, 700, 16, 15], 32, 4, 16), ([5000, 3], 3, 1, 32)])
+def test_shapes(dtype, D, lens, H, pairs, bs):
+    p = problem(lens, H, pairs, D, bs, dtype, seed=sum(lens) + H, garbage=float("nan"))
+    w = (1 + 0.1 * torch.randn(2 * D, generator=torch.Generator().manual_seed(3))).to(dtype).to(DEV)
+    got = check(p, H, pairs, D, bs, lam_of(H), weight=w, out_scale=0.2)
+    for b, L in enumerate(lens):
+        if L == 0:
+            assert (got[b] == 0).all()
+    check(p, H, pairs, D, bs, lam_of(H, 1))
+
+
+def test_many_sequences_in_slices():
+    """More sequences than one launch takes, most of them short or empty."""
+    gen = torch.Generator().manual_seed(5)
+    lens = (torch.randint(0, 40, (2100,), generator=gen) * (torch.rand(2100, generator=gen) < 0.8)).tolist()
+    lens[2047], lens[2048], lens[2099] = 900, 1, 333
+    p = problem(lens, 2, 1, 64, 16, BF16, seed=5, garbage=float("inf"))
+    check(p, 2, 1, 64, 16, lam_of(2))
+
+
+@pytest.mark.parametrize("window", [0, 1, 15, 16, 100, 511, 5000])
+def test_sliding_window(window):
+    lens = [1, 16, 17, 130, 600, 0, 2500]
+    p = problem(lens, 4, 2, 128, 16, BF16, seed=window)
+    check(p, 4, 2, 128, 16, lam_of(4), window=window)
+
+
+def test_sharp_and_cancelling_maps():
+    """Scores spread over hundreds of units; two equal maps with lambda 1, where nothing but rounding is left; lambda 0."""
+    lens = [200, 1500]
+    p = problem(lens, 4, 2, 128, 16, BF16, seed=9, spread=30.0)
+    w = torch.ones(256, dtype=BF16, device=DEV)
+    check(p, 4, 2, 128, 16, lam_of(4), weight=w, out_scale=0.5)
+    same = dict(p)
+    same["q"] = p["q"].view(2, 4, 2, 128)[:, :, :1].expand(2, 4, 2, 128).reshape(2, 8, 128).contiguous()
+    same["k"] = p["k"].view(-1, 16, 2, 2, 128)[:, :, :, :1].expand(-1, 16, 2, 2, 128).reshape(p["k"].shape).contiguous()
+    got = run(same, 4, 128, torch.ones(1, device=DEV))
+    assert (got == 0).all()
+    check(p, 4, 2, 128, 16, torch.zeros(1, device=DEV))
+    close = dict(same)   # maps that differ in a few keys only: most of o cancels, and the norm scales up what is left
+    close["k"] = same["k"].clone()
+    close["k"][:, 3, 1::2] = p["k"][:, 3, 1::2]
+    check(close, 4, 2, 128, 16, torch.full((1,), 0.9, device=DEV), weight=w)
+
+
+def test_lambda_shapes_and_strides():
+    lens, H = [90, 700, 33], 6
+    p = problem(lens, H, 2, 64, 16, BF16, seed=4)
+    per = torch.rand(3, H, device=DEV)
+    a = check(p, H, 2, 64, 16, per)
+    assert torch.equal(a, run(p, H, 64, torch.stack([per, per], 2)[:, :, 0]))
+    assert torch.equal(run(p, H, 64, torch.full((H,), 0.4, device=DEV)), run(p, H, 64, torch.tensor(0.4, device=DEV)))
+    wide = torch.randn(3, 2 * H + 4, 64, device=DEV).to(BF16)
+    wide[:, :2 * H] = p["q"]
+    out = torch.full((3, H + 1, 128), 3.0, dtype=BF16, device=DEV)
+    q = dict(p, q=wide[:, :2 * H])
+    run(q, H, 64, per, out=out[:, :H])
+    assert torch.equal(out[:, :H], a) and (out[:, H] == 3).all()
+
+
+def test_bad_pages_and_long_lengths_stay_in_the_cache():
+    """Page ids outside the cache are clamped into it, and a length beyond the table is cut at the table."""
+    p = problem([64, 40], 2, 1, 64, 16, BF16, seed=8)
+    p["table"][0, 1], p["table"][1, 2] = -5, 2 ** 30
+    fixed = dict(p, table=p["table"].clone())
+    fixed["table"][0, 1], fixed["table"][1, 2] = 0, p["k"].shape[0] - 1
+    assert torch.equal(run(p, 2, 64, lam_of(2)), run(fixed, 2, 64, lam_of(2)))
+    full = problem([96, 96], 2, 1, 64, 16, BF16, seed=8)
+    full["table"] = full["table"][:, :6].contiguous()
+    cut = dict(full, lens=torch.tensor([10 ** 9, 2 ** 31 - 1], dtype=torch.int32, device=DEV))
+    assert torch.equal(run(cut, 2, 64, lam_of(2)), run(full, 2, 64, lam_of(2)))
+    none = dict(full, lens=torch.tensor([-3, 0], dtype=torch.int32, device=DEV))
+    assert (run(none, 2, 64, lam_of(2)) == 0).all()
+
+
+def test_a_cache_whose_offsets_pass_32_bits():
+    """Pages beyond 4 GiB of the cache."""
+    P, bs, pairs, D = 2200, 128, 16, 128   # 2200 * 128 * 8 KB = 2.3 GB a cache of keys; slots up to 281600
+    P = 4400
+    k = torch.zeros(P, bs, 2 * pairs, D, dtype=BF16, device=DEV)
+    v = torch.zeros(P, bs, pairs, 2 * D, dtype=BF16, device=DEV)
+    assert k.numel() * 2 > 2 ** 32
+    small = problem([250], pairs, pairs, D, bs, BF16, seed=2)
+    pages = [P - 1, P - 2]
+    for i, pg in enumerate(pages):
+        k[pg], v[pg] = small["k"][small["table"][0, i]], small["v"][small["table"][0, i]]
+    big = dict(small, k=k, v=v, table=torch.tensor([pages], dtype=torch.int32, device=DEV))
+    assert torch.equal(run(big, pairs, D, lam_of(pairs)), run(small, pairs, D, lam_of(pairs)))
+
+
+def test_same_bits_every_time_streams_and_graph():
+    lens = [700, 0, 45, 3000, 129, 16]
+    p = problem(lens, 8, 2, 128, 16, BF16, seed=1)
+    lam = lam_of(8)
+    w = torch.ones(256, dtype=BF16, device=DEV)
+    first = run(p, 8, 128, lam, weight=w)
+    outs = [torch.empty_like(first) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):   # two calls that overlap in time
+        for s, o in zip(streams, outs):
+            with torch.cuda.stream(s):
+                run(p, 8, 128, lam, weight=w, out=o)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], first) and torch.equal(outs[1], first)
+    graphs = []
+    for o in outs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run(p, 8, 128, lam, weight=w, out=o)
+        graphs.append(graph)
+    for i in range(3):
+        new = torch.randint(0, 3000, (6,), generator=torch.Generator().manual_seed(i)).clamp(max=torch.tensor(lens)).to(torch.int32)
+        p["lens"].copy_(new)
+        for o, graph in zip(outs, graphs):
+            o.fill_(5)
+            graph.replay()
+        eager = run(p, 8, 128, lam, weight=w)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager)
+
+
+def test_refusals():
+    p = problem([20, 30], 4, 2, 64, 16, BF16)
+    lam = lam_of(4)
+    out = torch.empty(2, 4, 128, dtype=BF16, device=DEV)
+    base = dict(query=p["q"], k_cache=p["k"], v_cache=p["v"], output=out, block_table=p["table"], seq_lens=p["lens"], lambda_=lam)
+    assert ops.batch_decode_diff(**base) is out
+    for change in (dict(query=p["q"][:, :7]), dict(query=p["q"].float()), dict(query=p["q"].transpose(0, 1)),
+                   dict(output=out[:, :3]), dict(output=out.float()), dict(k_cache=p["k"][:, :, :3]), dict(k_cache=p["k"].half()),
+                   dict(v_cache=p["v"][:, :, :1]), dict(v_cache=p["k"]), dict(block_table=p["table"].long()),
+                   dict(block_table=p["table"].t()), dict(block_table=p["table"][:1]), dict(seq_lens=p["lens"].long()),
+                   dict(seq_lens=p["lens"][:1]), dict(lambda_=lam.double()), dict(lambda_=lam[:3]), dict(lambda_=lam.view(2, 2)),
+                   dict(norm_weight=torch.ones(64, dtype=BF16, device=DEV)), dict(norm_weight=torch.ones(128, device=DEV)),
+                   dict(output=out[:1].expand(2, 4, 128)), dict(seq_lens=p["lens"].cpu()),
+                   dict(output=p["v"].view(-1)[:1024].view(2, 4, 128))):
+        with pytest.raises((ValueError, TypeError)):
+            ops.batch_decode_diff(**dict(base, **change))
+    with pytest.raises(Exception, match="invalid argument"):
+        ops.batch_decode_diff(**base, scale=-1.0)
+    wide = torch.zeros(2, 8, 32, dtype=BF16, device=DEV)
+    with pytest.raises(Exception, match="not implemented"):
+        ops.batch_decode_diff(**dict(base, query=wide, k_cache=torch.zeros(4, 16, 4, 32, dtype=BF16, device=DEV),
+                                     v_cache=torch.zeros(4, 16, 2, 64, dtype=BF16, device=DEV),
+                                     output=torch.zeros(2, 4, 64, dtype=BF16, device=DEV)))
+    none = torch.empty(0, 4, 128, dtype=BF16, device=DEV)
+    assert ops.batch_decode_diff(p["q"][:0], p["k"], p["v"], none, p["table"][:0], p["lens"][:0], lam) is none
+
+
+# ------------------------------------------------------------------------------------------
+# the operators of a step, together
+
+def rotate_rows64(x, pos, inv, interleave=False):
+    angle = pos.double()[:, None] * inv
+    c, s = angle.cos()[:, None], angle.sin()[:, None]
+    y = x.double().clone()
+    h = x.shape[-1] // 2
+    a, b = x.double()[..., :h], x.double()[..., h:]
+    y[..., :h], y[..., h:] = a * c - b * s, b * c + a * s
+    return y
+
+
+def test_prefill_and_decode_steps_of_differential_attention():
+    """Chunks and decode steps of a few requests: tables -> cos|sin rows -> rotation -> store -> attend, every step's
+    attention compared with one over the whole history kept on the side."""
+    B, H, pairs, D, bs, T, steps = 3, 4, 2, 64, 16, 40, 5
+    W, pool = 12, 30
+    i32 = dict(dtype=torch.int32, device=DEV)
+    inv, factor = ops.rope_frequencies(D, scaling=ops.RopeScaling("llama3", factor=8.0, original_max_position=64), device=DEV)
+    k_cache = torch.full((pool, bs, 2 * pairs, D), float("nan"), dtype=BF16, device=DEV)
+    v_cache = torch.full((pool, bs, pairs, 2 * D), float("nan"), dtype=BF16, device=DEV)
+    free, head = torch.randperm(pool, generator=torch.Generator().manual_seed(0)).to(**i32), torch.zeros(1, **i32)
+    kv, table = torch.zeros(B, **i32), torch.full((B, W), -1, **i32)
+    lam = lam_of(H)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    hist_k, hist_v = [[] for _ in range(B)], [[] for _ in range(B)]
+    for step in range(steps):
+        new = torch.tensor([[17, 5, 0], [1, 30, 2], [1, 1, 1], [1, 1, 33], [1, 1, 1]][step], **i32)
+        t = ops.build_step_tables(kv, new, table, free, bs, T, head)
+        n = int(new.sum())
+        assert t.counters.tolist()[0] == n and t.counters.tolist()[2] == 0
+        q = torch.randn(T, 2 * H, D, generator=gen, device=DEV).to(BF16)
+        k = torch.randn(T, 2 * pairs, D, generator=gen, device=DEV).to(BF16)
+        v = torch.randn(T, pairs, 2 * D, generator=gen, device=DEV).to(BF16)
+        rows = ops.build_cos_sin_cache(inv, position_ids=t.position_ids, attention_factor=factor)   # the step's own rows
+        q0, k0 = q.clone(), k.clone()
+        ops.rotary_embedding(torch.arange(T, device=DEV), q, k, rows)
+        for got, raw in ((q, q0), (k, k0)):
+            want = rotate_rows64(raw, t.position_ids, inv)
+            assert ((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -21 * raw.abs().max()).all()
+        ops.reshape_paged_cache(ops.ReshapePagedCacheParams(key=k, value=v.view(T, 2 * pairs, D), k_cache=k_cache,
+                                                            v_cache=v_cache.view(pool, bs, 2 * pairs, D),
+                                                            slot_mapping=t.slot_mapping))
+        cu = t.q_cu_seq_lens.tolist()
+        for b in range(B):
+            hist_k[b].append(k[cu[b]:cu[b + 1]])
+            hist_v[b].append(v[cu[b]:cu[b + 1]])
+        last = (t.q_cu_seq_lens[1:].long() - 1).clamp(min=0)   # the last token of every request
+        out = torch.empty(B, H, 2 * D, dtype=BF16, device=DEV)
+        ops.batch_decode_diff(q[last], k_cache, v_cache, out, t.block_table, t.seq_lens, lam)
+        flat = dict(q=q[last], lens=t.seq_lens, table=torch.arange(B * 256, **i32).view(B, 256),
+                    k=torch.zeros(B * 256, 1, 2 * pairs, D, dtype=BF16, device=DEV),
+                    v=torch.zeros(B * 256, 1, pairs, 2 * D, dtype=BF16, device=DEV))
+        for b in range(B):
+            hk, hv = torch.cat(hist_k[b]), torch.cat(hist_v[b])
+            assert hk.shape[0] == int(t.seq_lens[b])
+            flat["k"][b * 256:b * 256 + hk.shape[0], 0] = hk
+            flat["v"][b * 256:b * 256 + hk.shape[0], 0] = hv
+        want, bound = reference(flat, H, pairs, D, 1, lam, D ** -0.5, None, 0.0, 1.0)
+        assert ((out.double() - want).abs() <= bound).all()
+        kv, table, head = t.seq_lens, t.block_table, t.counters[1:2]
+
+
+def test_mla_step_from_lengths_to_attention():
+    """tables -> MLA prologue -> dense_decode, against the same rows attended in 64 bits."""
+    B, H, bs, pool, T = 4, 16, 64, 20, 4
+    i32 = dict(dtype=torch.int32, device=DEV)
+    kv_lens = torch.tensor([100, 63, 64, 0], **i32)
+    table = torch.full((B, 4), -1, **i32)
+    order = torch.randperm(pool, generator=torch.Generator().manual_seed(2)).to(**i32)
+    table[0, :2], table[1, :1], table[2, :1] = order[:2], order[2:3], order[3:4]
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    cache = (torch.randn(pool, bs, 1, 576, generator=gen, device=DEV) * 0.5).to(BF16)
+    t = ops.build_step_tables(kv_lens, torch.ones(B, **i32), table, order[4:].contiguous(), bs, T)
+    inv, factor = ops.rope_frequencies(64, scaling=ops.RopeScaling("yarn", factor=40.0, original_max_position=4096), device=DEV)
+    rows = ops.build_cos_sin_cache(inv, 256, attention_factor=factor)
+    q = torch.randn(T, H, 192, generator=gen, device=DEV).to(BF16)
+    kv = torch.randn(T, 576, generator=gen, device=DEV).to(BF16)
+    w = torch.ones(512, dtype=BF16, device=DEV)
+    q_nope = torch.randn(T, H, 512, generator=gen, device=DEV).to(BF16) * 0.3
+    before = cache.clone()
+    q_pe, _ = ops.mla_norm_rope_and_cache(q[..., 128:], kv, w, 1e-6, rows, True, t.position_ids, k_cache=cache,
+                                          slot_mapping=t.slot_mapping, out_q_pe=torch.empty(T, H, 64, dtype=BF16, device=DEV))
+    flat, old = cache.view(-1, 576), before.view(-1, 576)
+    untouched = torch.ones(pool * bs, dtype=torch.bool)
+    untouched[t.slot_mapping.tolist()] = False
+    assert torch.equal(flat.cpu()[untouched], old.cpu()[untouched])
+    scale = 192 ** -0.5
+    got = ops.dense_decode(ops.DenseDecodeParams(q_nope.view(B, 1, H, 512), q_pe.view(B, 1, H, 64), cache, t.seq_lens,
+                                                 t.block_table, 512, scale))
+    for b in range(B):
+        L = int(t.seq_lens[b])
+        tok = torch.arange(L, device=DEV)
+        c = flat[t.block_table[b, tok // bs].long() * bs + tok % bs].double()
+        s = torch.cat([q_nope[b], q_pe[b]], 1).double() @ c.t() * scale
+        want = torch.softmax(s, 1) @ c[:, :512]
+        assert (got[b, 0].double() - want).abs().max() <= 2e-2

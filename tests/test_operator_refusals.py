@@ -1,0 +1,127 @@
+"""What the step-table, rotary, MLA-prologue and differential entry points refuse before anything is launched: no GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from xllm_amd import capi, ops
+
+FAKE = 1 << 20   # an aligned non-null address: the calls below return before anything is launched
+BF16, FP16, FP32, FP8 = capi.BF16, capi.FP16, capi.FP32, capi.FP8_E4M3
+EINVAL, EDTYPE, ESHAPE, EWORKSPACE, EALIGN = -1, -2, -3, -4, -5
+
+
+def strides(a, b):
+    return (ctypes.c_int64 * 2)(a, b)
+
+
+def call(fn, base, **change):
+    args = dict(base)
+    assert set(change) <= set(args)
+    args.update(change)
+    return fn(*args.values())
+
+
+def test_step_tables():
+    fn = capi.lib().xllm_mi355_build_step_tables
+    base = dict(kv=FAKE, new=FAKE, tin=FAKE, in_stride=8, tout=FAKE, out_stride=8, width=8, free=FAKE, n_free=9, head=None,
+                seq=FAKE, cu=FAKE, pos=FAKE, slots=FAKE, indptr=FAKE, counters=FAKE, batch=4, bs=16, budget=8, stream=None)
+    assert call(fn, base, batch=0) == 0
+    for name in ("kv", "new", "tin", "tout", "free", "seq", "cu", "pos", "slots", "indptr", "counters"):
+        assert call(fn, base, **{name: None}) == EINVAL, name
+    for change in (dict(batch=-1), dict(bs=0), dict(width=0), dict(n_free=-1), dict(budget=-1), dict(in_stride=7),
+                   dict(out_stride=7), dict(out_stride=9)):   # (in place with another stride)
+        assert call(fn, base, **change) == EINVAL, change
+    for change in (dict(budget=1 << 30), dict(n_free=1 << 30), dict(bs=1 << 30), dict(batch=(1 << 20) + 1)):
+        assert call(fn, base, **change) == ESHAPE, change
+
+
+def test_cos_sin_rows():
+    fn = capi.lib().xllm_mi355_rope_cos_sin
+    base = dict(inv=FAKE, pos=None, first=0, rows=4, half=32, factor=1.0, out=FAKE, dtype=FP32, stream=None)
+    assert call(fn, base, rows=0) == 0
+    for change in (dict(inv=None), dict(out=None), dict(rows=-1), dict(half=0)):
+        assert call(fn, base, **change) == EINVAL, change
+    assert call(fn, base, half=4097) == ESHAPE
+    assert call(fn, base, dtype=FP8) == EDTYPE
+
+
+def test_rotation():
+    fn = capi.lib().xllm_mi355_rotary_embedding
+    st = strides(512, 128)
+    base = dict(pos=FAKE, table=FAKE, rows=10, q=FAKE, qo=FAKE, k=FAKE, ko=FAKE, T=4, hq=4, hk=4, dq=128, dk=128, oq=0, ok=0,
+                R=64, sq=st, sqo=st, sk=st, sko=st, interleave=0, inverse=0, dtype=BF16, ctype=FP32, stream=None)
+    assert call(fn, base, T=0) == 0
+    for change in (dict(pos=None), dict(table=None), dict(q=None), dict(qo=None), dict(k=None), dict(ko=None), dict(sq=None),
+                   dict(sqo=None), dict(sk=None), dict(sko=None), dict(T=-1), dict(rows=0), dict(hq=0), dict(hk=-1),
+                   dict(sq=strides(-512, 128)), dict(sqo=strides(640, 128))):   # (in place with other strides)
+        assert call(fn, base, **change) == EINVAL, change
+    for change in (dict(R=0), dict(R=63), dict(oq=65), dict(ok=-1), dict(ok=70), dict(R=256), dict(hq=65536)):
+        assert call(fn, base, **change) == ESHAPE, change
+    for change in (dict(dtype=FP8), dict(ctype=FP8)):
+        assert call(fn, base, **change) == EDTYPE, change
+
+
+def test_mla_prologue():
+    fn = capi.lib().xllm_mi355_mla_norm_rope_and_cache
+    base = dict(q=FAKE, qo=FAKE, kv=FAKE, kvo=None, w=FAKE, eps=1e-6, table=FAKE, rows=10, pos=FAKE, cache=FAKE, slots=FAKE,
+                T=4, H=8, dl=512, dr=64, qt=1536, qh=192, qot=512, qoh=64, kvs=576, kvos=0, bs=16, P=4, interleave=1,
+                dtype=BF16, ctype=FP32, stream=None)
+    assert call(fn, base, T=0) == 0
+    for change in (dict(q=None), dict(qo=None), dict(kv=None), dict(w=None), dict(table=None), dict(pos=None), dict(cache=None),
+                   dict(slots=None), dict(T=-1), dict(H=0), dict(rows=0), dict(bs=0), dict(P=0), dict(kvs=575),
+                   dict(kvo=FAKE, kvos=512), dict(eps=-1.0), dict(qt=-8)):
+        assert call(fn, base, **change) == EINVAL, change
+    for change in (dict(dl=256), dict(dr=32), dict(P=1 << 28)):
+        assert call(fn, base, **change) == ESHAPE, change
+    assert call(fn, base, dtype=FP32) == EDTYPE and call(fn, base, ctype=FP8) == EDTYPE
+    for change in (dict(q=FAKE + 2), dict(qo=FAKE + 8), dict(kv=FAKE + 4), dict(w=FAKE + 2), dict(table=FAKE + 4),
+                   dict(cache=FAKE + 8), dict(qt=1540), dict(qh=66), dict(kvs=577), dict(kvo=FAKE, kvos=580)):
+        assert call(fn, base, **change) == EALIGN, change
+
+
+def test_differential_decode():
+    lib = capi.lib()
+    size = lib.xllm_mi355_paged_decode_diff_workspace_bytes
+    assert size(16, 4, 128) > 0 and size(16, 4, 64) < size(16, 4, 128) < size(64, 4, 128)
+    assert size(0, 1, 128) == 0 and size(5, 2, 128) == 0 and size(4, 2, 96) == 0
+    fn = lib.xllm_mi355_paged_decode_diff
+    base = dict(q=FAKE, k=FAKE, v=FAKE, out=FAKE, table=FAKE, stride=8, width=8, lens=FAKE, lam=FAKE, lb=0, lh=1, w=None,
+                eps=1e-5, out_scale=1.0, batch=4, H=16, pairs=4, D=128, bs=16, P=100, qs=4096, os=4096, window=-1, scale=0.1,
+                ws=FAKE, ws_bytes=size(16, 4, 128), dtype=BF16, stream=None)
+    assert call(fn, base, batch=0) == 0
+    for name in ("q", "k", "v", "out", "table", "lens", "lam"):
+        assert call(fn, base, **{name: None}) == EINVAL, name
+    for change in (dict(batch=-1), dict(H=0), dict(pairs=3), dict(bs=0), dict(P=0), dict(width=0), dict(stride=7),
+                   dict(scale=0.0), dict(scale=float("nan")), dict(eps=-1.0), dict(lb=-1), dict(lh=-1), dict(qs=4095), dict(os=2048)):
+        assert call(fn, base, **change) == EINVAL, change
+    for change in (dict(D=96), dict(D=256), dict(P=1 << 28)):
+        assert call(fn, base, **change) == ESHAPE, change
+    for dtype in (FP32, FP8):
+        assert call(fn, base, dtype=dtype) == EDTYPE
+    for change in (dict(q=FAKE + 8), dict(k=FAKE + 2), dict(v=FAKE + 8), dict(out=FAKE + 4), dict(w=FAKE + 4), dict(qs=4100),
+                   dict(os=4097)):
+        assert call(fn, base, **change) == EALIGN, change
+    for change in (dict(ws=None), dict(ws=FAKE + 64), dict(ws_bytes=size(16, 4, 128) - 1)):
+        assert call(fn, base, **change) == EWORKSPACE, change
+
+
+def test_cpu_tensors_are_refused():
+    i32 = torch.int32
+    one = torch.zeros(1, dtype=i32)
+    q = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    rows = torch.zeros(4, 64)
+    pos = torch.zeros(1, dtype=torch.int64)
+    calls = [lambda: ops.build_step_tables(one, one, torch.zeros(1, 2, dtype=i32), one, 16, 1),
+             lambda: ops.build_cos_sin_cache(torch.ones(4, dtype=torch.float64), 3),
+             lambda: ops.rotary_embedding(pos, q, None, rows),
+             lambda: ops.mla_norm_rope_and_cache(q, torch.zeros(1, 576), torch.ones(512), 1e-6, rows, True, pos),
+             lambda: ops.batch_decode_diff(q, q, q, q, one, one, rows)]
+    for c in calls:
+        with pytest.raises(ValueError, match="GPU only"):
+            c()
+
+
+def test_frequencies_need_no_gpu():
+    inv, factor = ops.rope_frequencies(64, scaling=ops.RopeScaling("linear", factor=2.0), device="cpu")
+    assert inv.dtype == torch.float64 and inv[0] == 0.5 and factor == 1.0

@@ -68,6 +68,14 @@ SIGNATURES = {
     "xllm_mi355_mask_block_table_padding": (_i32, [_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "xllm_mi355_mla_absorbed_bmm": (_i32, [_p] * 3 + [_i64] * 8 + [_i32, _p]),
     "xllm_mi355_rope_and_cache": (_i32, [_p] * 10 + [_i64] * 7 + [_f32, _i32, _i64, _i64, _i32, _i32, _i32, _p]),
+    "xllm_mi355_build_step_tables": (_i32, [_p] * 3 + [_i64, _p, _i64, _i64, _p, _i64] + [_p] * 7 + [_i64] * 3 + [_p]),
+    "xllm_mi355_rope_cos_sin": (_i32, [_p, _p, _i64, _i64, _i64, ctypes.c_double, _p, _i32, _p]),
+    "xllm_mi355_rotary_embedding": (_i32, [_p, _p, _i64] + [_p] * 4 + [_i64] * 8 + [_p] * 4 + [_i32] * 4 + [_p]),
+    "xllm_mi355_mla_norm_rope_and_cache": (_i32, [_p] * 5 + [_f32, _p, _i64, _p, _p, _p] + [_i64] * 12 + [_i32] * 3
+                                           + [_p]),
+    "xllm_mi355_paged_decode_diff_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "xllm_mi355_paged_decode_diff": (_i32, [_p] * 5 + [_i64, _i64, _p, _p, _i64, _i64, _p, _f32, _f32] + [_i64] * 9
+                                     + [_f32, _p, _sz, _i32, _p]),
     "xllm_mi355_profile_enable": (_i32, [_i32]),
     "xllm_mi355_profile_collect": (_i32, [_p, _i32]),
     "xllm_mi355_stream_read": (_i32, [_p, _sz, _p, _p]),

@@ -465,4 +465,65 @@ int xllm_mi355_build_block_table(const int32_t* paged_kv_indptr, const int32_t* 
                            table_stride, seq_lens, batch, block_size, static_cast<hipStream_t>(stream));
 }
 
+int xllm_mi355_build_step_tables(const int32_t* kv_lens, const int32_t* new_lens, const int32_t* block_table_in,
+                                 int64_t in_stride, int32_t* block_table_out, int64_t out_stride, int64_t table_width,
+                                 const int32_t* free_pages, int64_t n_free, const int32_t* free_head,
+                                 int32_t* seq_lens, int32_t* cu_new_lens, int64_t* positions, int32_t* slots,
+                                 int32_t* new_page_indptr, int32_t* counters, int64_t batch, int64_t block_size,
+                                 int64_t max_new_tokens, void* stream) {
+  return build_step_tables(kv_lens, new_lens, block_table_in, in_stride, block_table_out, out_stride, table_width,
+                           free_pages, n_free, free_head, seq_lens, cu_new_lens, positions, slots, new_page_indptr,
+                           counters, batch, block_size, max_new_tokens, static_cast<hipStream_t>(stream));
+}
+
+int xllm_mi355_rope_cos_sin(const double* inv_freq, const int64_t* positions, int64_t first_position, int64_t n_rows,
+                            int64_t half, double factor, void* out, int out_dtype, void* stream) {
+  return rope_cos_sin(inv_freq, positions, first_position, n_rows, half, factor, out, out_dtype,
+                      static_cast<hipStream_t>(stream));
+}
+
+int xllm_mi355_rotary_embedding(const int64_t* positions, const void* cos_sin, int64_t n_positions, const void* q,
+                                void* q_out, const void* k, void* k_out, int64_t n_tokens, int64_t n_heads_q,
+                                int64_t n_heads_k, int64_t head_dim_q, int64_t head_dim_k, int64_t rotary_offset_q,
+                                int64_t rotary_offset_k, int64_t rotary_dim, const int64_t* q_strides,
+                                const int64_t* q_out_strides, const int64_t* k_strides, const int64_t* k_out_strides,
+                                int interleave, int inverse, int dtype, int cos_sin_dtype, void* stream) {
+  return rotary_embedding(positions, cos_sin, n_positions, q, q_out, k, k_out, n_tokens, n_heads_q, n_heads_k,
+                          head_dim_q, head_dim_k, rotary_offset_q, rotary_offset_k, rotary_dim, q_strides,
+                          q_out_strides, k_strides, k_out_strides, interleave, inverse, dtype, cos_sin_dtype,
+                          static_cast<hipStream_t>(stream));
+}
+
+int xllm_mi355_mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const void* kv, void* kv_out,
+                                       const void* kv_weight, float eps, const void* cos_sin, int64_t n_positions,
+                                       const int64_t* positions, void* k_cache, const int32_t* slot_mapping,
+                                       int64_t n_tokens, int64_t n_heads, int64_t d_latent, int64_t d_rope,
+                                       int64_t q_token_stride, int64_t q_head_stride, int64_t q_out_token_stride,
+                                       int64_t q_out_head_stride, int64_t kv_row_stride, int64_t kv_out_row_stride,
+                                       int64_t block_size, int64_t num_blocks, int interleave, int dtype,
+                                       int cos_sin_dtype, void* stream) {
+  return mla_norm_rope_and_cache(q_pe, q_pe_out, kv, kv_out, kv_weight, eps, cos_sin, n_positions, positions, k_cache,
+                                 slot_mapping, n_tokens, n_heads, d_latent, d_rope, q_token_stride, q_head_stride,
+                                 q_out_token_stride, q_out_head_stride, kv_row_stride, kv_out_row_stride, block_size,
+                                 num_blocks, interleave, dtype, cos_sin_dtype, static_cast<hipStream_t>(stream));
+}
+
+size_t xllm_mi355_paged_decode_diff_workspace_bytes(int64_t n_heads, int64_t n_kv_pairs, int64_t head_dim) {
+  return diff_workspace_bytes(n_heads, n_kv_pairs, head_dim);
+}
+
+int xllm_mi355_paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, void* out,
+                                 const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                                 const int32_t* seq_lens, const float* lambda, int64_t lambda_batch_stride,
+                                 int64_t lambda_head_stride, const void* norm_weight, float eps, float out_scale,
+                                 int64_t batch, int64_t n_heads, int64_t n_kv_pairs, int64_t head_dim,
+                                 int64_t block_size, int64_t num_blocks, int64_t q_token_stride,
+                                 int64_t out_token_stride, int64_t window_left, float sm_scale, void* workspace,
+                                 size_t workspace_bytes, int dtype, void* stream) {
+  return paged_decode_diff(q, k_cache, v_cache, out, block_table, table_stride, table_width, seq_lens, lambda,
+                           lambda_batch_stride, lambda_head_stride, norm_weight, eps, out_scale, batch, n_heads,
+                           n_kv_pairs, head_dim, block_size, num_blocks, q_token_stride, out_token_stride,
+                           window_left, sm_scale, workspace, workspace_bytes, dtype, static_cast<hipStream_t>(stream));
+}
+
 }  // extern "C"

@@ -181,6 +181,40 @@ int decode_metadata_update(const int32_t* src_tokens, const int32_t* src_positio
                            int64_t actual_num_tokens, int64_t padded_num_tokens, int64_t actual_batch_size,
                            int64_t actual_indices_size, hipStream_t stream);
 
+size_t diff_workspace_bytes(int64_t n_heads, int64_t n_pairs, int64_t head_dim);
+int paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, void* out, const int32_t* block_table,
+                      int64_t table_stride, int64_t table_width, const int32_t* seq_lens, const float* lambda,
+                      int64_t lambda_batch_stride, int64_t lambda_head_stride, const void* norm_weight, float eps,
+                      float out_scale, int64_t batch, int64_t n_heads, int64_t n_kv_pairs, int64_t head_dim,
+                      int64_t block_size, int64_t num_blocks, int64_t q_token_stride, int64_t out_token_stride,
+                      int64_t window_left, float sm_scale, void* workspace, size_t workspace_bytes, int dtype,
+                      hipStream_t stream);
+
+int build_step_tables(const int32_t* kv_lens, const int32_t* new_lens, const int32_t* block_table_in,
+                      int64_t in_stride, int32_t* block_table_out, int64_t out_stride, int64_t table_width,
+                      const int32_t* free_pages, int64_t n_free, const int32_t* free_head, int32_t* seq_lens,
+                      int32_t* cu_new, int64_t* positions, int32_t* slots, int32_t* new_page_indptr,
+                      int32_t* counters, int64_t batch, int64_t block_size, int64_t max_new_tokens,
+                      hipStream_t stream);
+
+int rope_cos_sin(const double* inv_freq, const int64_t* positions, int64_t first_position, int64_t n_rows, int64_t half,
+                 double factor, void* out, int out_dtype, hipStream_t stream);
+
+int rotary_embedding(const int64_t* positions, const void* cos_sin, int64_t n_positions, const void* q, void* q_out,
+                     const void* k, void* k_out, int64_t n_tokens, int64_t n_heads_q, int64_t n_heads_k,
+                     int64_t head_dim_q, int64_t head_dim_k, int64_t rotary_offset_q, int64_t rotary_offset_k,
+                     int64_t rotary_dim, const int64_t* q_strides, const int64_t* q_out_strides,
+                     const int64_t* k_strides, const int64_t* k_out_strides, int interleave, int inverse, int dtype,
+                     int cos_sin_dtype, hipStream_t stream);
+
+int mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const void* kv, void* kv_out, const void* kv_weight, float eps,
+                            const void* cos_sin, int64_t n_positions, const int64_t* positions, void* k_cache,
+                            const int32_t* slots, int64_t n_tokens, int64_t n_heads, int64_t d_latent, int64_t d_rope,
+                            int64_t q_token_stride, int64_t q_head_stride, int64_t q_out_token_stride,
+                            int64_t q_out_head_stride, int64_t kv_row_stride, int64_t kv_out_row_stride,
+                            int64_t block_size, int64_t num_blocks, int interleave, int dtype, int cos_sin_dtype,
+                            hipStream_t stream);
+
 // Kernel attributes (dynamic LDS size) are set per device.  Returns true the first time it is called with
 // `seen` on the current device (devices 0..63; beyond that always true: setting them again is harmless).
 inline bool first_use_on_current_device(std::atomic<uint64_t>& seen) {

@@ -1,0 +1,725 @@
+// Differential attention of one new token per sequence over paged keys and values, for gfx950.
+//
+//   S_m[t]  = scale * q[b, 2h + m] . K[t, 2j + m]          m = 0, 1 (the two maps of head h), j = h / group
+//   o       = (softmax(S_0) - lambda[b, h] * softmax(S_1)) . V[:, j]        V rows of 2 D values
+//   out     = out_scale * norm_w * o / sqrt(mean(o^2) + eps)                (norm_w null: out = out_scale * o)
+//
+// The KV heads of a token lie pair after pair, so the two key rows of a pair are one run of 2 D values, of the same
+// size and at the same place in the key cache as the value row in the value cache: one address per token serves both.
+// A decode step reads every key and value once for a few operations per byte, so the kernel is HBM bound and is built
+// to keep bytes in flight; both maps are taken in the one pass over the rows (two ordinary decodes would read V twice).
+//
+// Schedule.  The context of every (sequence, head block) is cut into stages of 16 tokens; the stages of the batch form
+// one list ordered (sequence, head block, stage).  A worker is one wavefront, four to a workgroup, one workgroup per CU;
+// every worker streams an equal range of the list, whatever the mix of lengths, and meets no other worker after the
+// common prefix sum of the lengths.  A range that holds a whole context writes the output row, a part of a context goes
+// to the workspace as (o, max, sum) in fp32 and diff_merge_kernel joins the parts.
+//
+// Data path.  Rows travel from global memory straight into a ring of the worker's own LDS (32 KB: two stages of 512-byte
+// rows, four of 256-byte rows), and the place of a stage's keys is filled again as soon as they are in registers, the
+// place of its values likewise.  Page-table entries take the same path two ring lengths ahead, so that no load of the
+// loop waits in a register (such a wait would also wait for every younger row in flight: the counter is in order).
+//   S^T[token, column] = K[token, dims] . Q^T        v_mfma_f32_16x16x32, K read from LDS, Q^T in registers
+//   O^T[dim, column]  += V^T[dim, token] . P^T       v_mfma_f32_16x16x16, V^T by the transposing LDS read, P^T straight
+//                                                    from the accumulators of S^T
+// The 16 columns hold both maps of up to eight heads (map 0 in columns 0-7, map 1 in 8-15: each map's query rows are
+// zero in the other's columns, so the two products add into one accumulator).  Groups of more than eight heads take two
+// blocks of 16 columns, one per map, so that rows are still read once for sixteen heads.
+// P is rounded to the 16-bit type in two parts, p = hi + lo, and both go through the matrix cores: the difference of the
+// maps can cancel most of o, which would leave the rounding of a single 16-bit P as the error of what remains (the norm
+// scales it up).  The second product costs 16 (8) more MFMAs per 16 KB (8 KB) of rows, which HBM leaves time for.
+// Softmax statistics, sums and the norm are in fp32.
+#include "common.cuh"
+#include "launch.h"
+
+namespace xllm_mi355 {
+
+namespace {
+
+constexpr int kDiffWaves = 4;
+constexpr int kDiffThreads = kDiffWaves * kWave;
+constexpr int kDiffTokens = 16;               // tokens of a stage
+constexpr int kDiffRing = 32768;              // ring bytes of a worker
+constexpr int kDiffMaxBatch = kWsMaxBatch;    // sequences per launch (their prefix and lengths lie in LDS)
+// A worker takes at least this many stages: with fewer, short batches would be cut into pieces whose partial rows cost
+// more than their keys and values.
+constexpr int kDiffMinStages = 4;
+constexpr float kDiffSlack = 8.0f;            // a maximum moves when a score exceeds it by this much (log2 units)
+
+typedef __attribute__((address_space(3))) s16x4 diff_lds_s16x4;
+
+struct DiffArgs {
+  const char* q;
+  const char* k_cache;
+  const char* v_cache;
+  char* out;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const float* lambda;
+  const char* norm_w;
+  int* ws_prefix;       // [batch + 1], written by workgroup 0 for the merge
+  float* ws_o;          // [2 * workers][columns][2 D]
+  float* ws_ml;         // [2 * workers][columns][2]: maximum (log2 units), sum
+  int64_t table_stride;
+  int64_t q_stride_bytes;
+  int64_t out_stride_bytes;
+  int64_t row_bytes;    // bytes of a token in either cache
+  int64_t lambda_batch_stride;
+  int64_t lambda_head_stride;
+  int batch;
+  int n_heads;          // differential heads
+  int n_pairs;          // KV pairs
+  int group;            // heads per pair
+  int hb_per_pair;      // head blocks per pair
+  int block_size;
+  int bs_shift;         // log2(block_size) or -1
+  int num_blocks;
+  int max_len;          // what the table can hold
+  int window_left;
+  int n_workers;
+  float scale_log2;
+  float eps;
+  float out_scale;
+};
+
+__device__ __forceinline__ int diff_len(const DiffArgs& a, int b) { return max(0, min(a.seq_lens[b], a.max_len)); }
+__device__ __forceinline__ int diff_first(const DiffArgs& a, int L) {
+  return a.window_left < 0 ? 0 : max(0, L - 1 - a.window_left);
+}
+__device__ __forceinline__ int diff_stages(const DiffArgs& a, int L) {
+  return L > 0 ? (L + kDiffTokens - 1) / kDiffTokens - diff_first(a, L) / kDiffTokens : 0;
+}
+// How many workers take part, and where the range of worker w begins.
+__device__ __forceinline__ int diff_used(const DiffArgs& a, int64_t total) {
+  const int64_t n = total / kDiffMinStages;
+  return static_cast<int>(n < 1 ? 1 : (n < a.n_workers ? n : a.n_workers));
+}
+__device__ __forceinline__ int64_t diff_start(int64_t w, int64_t total, int used) { return w * total / used; }
+
+__device__ __forceinline__ void diff_dma16(const char* p, u32 lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(p) : "memory");
+}
+__device__ __forceinline__ void diff_dma4(const int32_t* p, u32 lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void diff_wait_vm() {
+  static_assert(N >= 0 && N < 64, "range of the counter");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void diff_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ float diff_rows_max(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  auto t = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
+  x = fmaxf(as_f32(t[0]), as_f32(t[1]));
+  auto u = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);
+  return fmaxf(as_f32(u[0]), as_f32(u[1]));
+}
+__device__ __forceinline__ float diff_rows_sum(float x) {
+  auto t = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
+  x = as_f32(t[0]) + as_f32(t[1]);
+  auto u = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);
+  return as_f32(u[0]) + as_f32(u[1]);
+}
+
+// v0 - lambda v1 with both maps' results rounded alike: left to itself the compiler fuses the first one's normalisation
+// into the subtraction, and two equal maps with lambda = 1 leave its rounding behind instead of zero.
+__device__ __forceinline__ float diff_of(float v0, float lam, float v1) {
+#pragma clang fp contract(off)
+  const float t = lam * v1;
+  return v0 - t;
+}
+
+// A stage of the list.  Every field is the same in all lanes.
+struct DiffCursor {
+  int b, hb, st, n;    // sequence, head block, stage, stages of the context
+  int L, lo;           // context length, first attended token
+};
+
+template <int D, int NB>
+struct DiffShape {
+  static constexpr int kRow = 4 * D;                       // bytes of a pair's row
+  static constexpr int kChunks = kRow / 16;                // 16-byte chunks of a row
+  static constexpr int kRowsPerLoad = kWave / kChunks;
+  static constexpr int kLoads = kDiffTokens / kRowsPerLoad; // load instructions of a stage's keys, and of its values
+  static constexpr int kTile = kDiffTokens * kRow;         // bytes of a stage's keys
+  static constexpr int kStages = kDiffRing / (2 * kTile);  // ring length
+  static constexpr int kPageSlots = 2 * kStages;           // page-table entries are fetched two ring lengths ahead
+  static constexpr int kCols = 16 * NB;
+  static constexpr int kHeads = NB == 1 ? 8 : 16;          // heads of a head block
+  // LDS: rings | page entries [waves][kPageSlots][64] | scan scratch [8] | lengths [batch] | prefix [batch + 1]
+  static constexpr int kPageOff = kDiffWaves * kDiffRing;
+  static constexpr int kTmpOff = kPageOff + kDiffWaves * kPageSlots * kWave * 4;
+  static constexpr int kLensOff = kTmpOff + 32;
+  static size_t lds_bytes(int batch) { return kLensOff + static_cast<size_t>(2 * batch + 1) * 4; }
+};
+
+// One head's finished row: o0 and o1 are the normalised results of the two maps for the lane's dims
+// 16 mb + 4 (lane / 16) + r.  All four lanes of a head (l, l ^ 16, l ^ 32, l ^ 48) call it together.
+template <typename QT, int MB>
+__device__ __forceinline__ void diff_store_row(const DiffArgs& a, const f32x4 (&o)[MB], int b, int head, bool on, int g) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) ss += o[mb][r] * o[mb][r];
+  ss = diff_rows_sum(ss);
+  float f = a.out_scale;
+  if (a.norm_w != nullptr) f *= 1.0f / __builtin_sqrtf(ss / static_cast<float>(MB * 16) + a.eps);
+  if (!on) return;
+  char* row = a.out + b * a.out_stride_bytes + static_cast<int64_t>(head) * MB * 32;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    f32x4 w = {1.0f, 1.0f, 1.0f, 1.0f};
+    if (a.norm_w != nullptr) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(a.norm_w + (mb * 16 + 4 * g) * 2);
+      w = f32x4{QT::lo(x[0]), QT::hi(x[0]), QT::lo(x[1]), QT::hi(x[1])};
+    }
+    const u32x2 y = {QT::pack(o[mb][0] * f * w[0], o[mb][1] * f * w[1]), QT::pack(o[mb][2] * f * w[2], o[mb][3] * f * w[3])};
+    *reinterpret_cast<u32x2*>(row + (mb * 16 + 4 * g) * 2) = y;
+  }
+}
+
+template <typename QT, int D, int NB>
+__global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a) {
+  using S = DiffShape<D, NB>;
+  constexpr int KS = D / 32;       // k-steps of a map's scores
+  constexpr int MB = 2 * D / 16;   // dim blocks of the output
+  constexpr int NS = S::kStages;
+  constexpr int NL = S::kLoads;
+  constexpr int kStageOps = 1 + 2 * NL;   // vector memory operations of a stage: page entries, keys, values
+
+  extern __shared__ __align__(16) char smem[];
+  int* tmp = reinterpret_cast<int*>(smem + S::kTmpOff);
+  int* lens = reinterpret_cast<int*>(smem + S::kLensOff);
+  int* prefix = lens + a.batch;
+  const int tid = threadIdx.x;
+  const int lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, g = lane >> 4;
+  const int n_hb = a.n_pairs * a.hb_per_pair;
+
+  // ---- lengths and the exclusive prefix sum of the stages
+  {
+    const int per = (a.batch + kDiffThreads - 1) / kDiffThreads;
+    const int lo = min(a.batch, tid * per), hi = min(a.batch, lo + per);
+    int local = 0;
+    for (int b = lo; b < hi; ++b) {
+      const int L = diff_len(a, b);
+      lens[b] = L;
+      local += diff_stages(a, L);
+    }
+    int incl = local;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int t = __shfl_up(incl, d, kWave);
+      if (lane >= d) incl += t;
+    }
+    if (lane == kWave - 1) tmp[wave] = incl;
+    __syncthreads();
+    int excl = incl - local;
+    for (int w = 0; w < wave; ++w) excl += tmp[w];
+    for (int b = lo; b < hi; ++b) {
+      prefix[b] = excl;
+      excl += diff_stages(a, lens[b]);
+    }
+    if (tid == kDiffThreads - 1) prefix[a.batch] = excl;   // (an empty slice leaves the total as it came in)
+    __syncthreads();
+  }
+  if (blockIdx.x == 0)
+    for (int b = tid; b <= a.batch; b += kDiffThreads) a.ws_prefix[b] = prefix[b];
+
+  const int64_t total = static_cast<int64_t>(prefix[a.batch]) * n_hb;
+  const int used = diff_used(a, total);
+  // neighbours in the list sit on different CUs, so that a short list still spreads over the chip
+  const int worker = wave * gridDim.x + blockIdx.x;
+  if (total == 0 || worker >= used) return;
+  const int64_t begin = diff_start(worker, total, used);
+  const int N = static_cast<int>(diff_start(worker + 1, total, used) - begin);
+  if (N <= 0) return;
+
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  auto enter = [&](DiffCursor& c) {   // the context fields of sequence c.b
+    c.L = uniform(lens[c.b]);
+    c.lo = diff_first(a, c.L);
+    c.n = diff_stages(a, c.L);
+  };
+  auto advance = [&](DiffCursor& c) {
+    if (++c.st < c.n) return;
+    c.st = 0;
+    if (++c.hb < n_hb) return;
+    c.hb = 0;
+    do ++c.b; while (c.b < a.batch - 1 && uniform(prefix[c.b + 1]) == uniform(prefix[c.b]));
+    if (c.b < a.batch) enter(c);
+  };
+  DiffCursor cc;   // computing
+  {
+    int lo = 0, hi = a.batch - 1;   // the last sequence that begins at or before the range (its stages hold it)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (static_cast<int64_t>(prefix[mid]) * n_hb <= begin) lo = mid;
+      else hi = mid - 1;
+    }
+    cc.b = uniform(lo);
+    enter(cc);
+    const int rest = uniform(static_cast<int>(begin - static_cast<int64_t>(prefix[cc.b]) * n_hb));
+    cc.hb = rest / cc.n;
+    cc.st = rest - cc.hb * cc.n;
+  }
+  DiffCursor lc = cc, pc = cc;   // loading rows, loading page entries
+
+  const u32 lds0 = uniform(static_cast<u32>(reinterpret_cast<uintptr_t>(smem)));
+  const u32 ring_lds = lds0 + wave * kDiffRing;
+  const char* ring = smem + wave * kDiffRing;
+  const u32 page_lds = lds0 + S::kPageOff + wave * S::kPageSlots * kWave * 4;
+  const int* page_mem = reinterpret_cast<const int*>(smem + S::kPageOff) + wave * S::kPageSlots * kWave;
+
+  // token (lane & 15) of a stage; what lies outside the attended range repeats its first or last token, so that every
+  // row in LDS is one that the sequence owns (a probability of zero times a stale NaN would be NaN)
+  auto token_of = [&](const DiffCursor& c) {
+    const int t = (c.lo / kDiffTokens + c.st) * kDiffTokens + c16;
+    return max(c.lo, min(t, c.L - 1));
+  };
+  auto split = [&](int t, int& col, int& off) {
+    if (a.bs_shift >= 0) {
+      col = t >> a.bs_shift;
+      off = t & (a.block_size - 1);
+    } else {
+      col = static_cast<int>(static_cast<u32>(t) / static_cast<u32>(a.block_size));
+      off = t - col * a.block_size;
+    }
+  };
+  // Page entries of stage x (the cursor pc) into their slot.  Past the range the last stage's are fetched again: the
+  // waits below count operations, and every stage has the same number of them.
+  int px = 0;
+  auto fetch_pages = [&]() {
+    int col, off;
+    split(token_of(pc), col, off);
+    diff_dma4(a.block_table + pc.b * a.table_stride + col, page_lds + (px % S::kPageSlots) * (kWave * 4));
+    ++px;
+    if (px < N) advance(pc);
+  };
+  // Row offsets of the next stage to load (the cursor lc), then its keys and its values.
+  const int dc = lane % S::kChunks, dr = lane / S::kChunks;
+  int lx = 0;
+  int64_t row_off[NL];
+  auto load_keys = [&]() {
+    const int t = token_of(lc);
+    int col, off;
+    split(t, col, off);
+    const int page = max(0, min(page_mem[(lx % S::kPageSlots) * kWave + lane], a.num_blocks - 1));
+    const int slot = page * a.block_size + off;
+    const int pair = lc.hb / a.hb_per_pair;
+    const u32 base = ring_lds + (lx % NS) * (2 * S::kTile);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = i * S::kRowsPerLoad + dr;
+      const int s = __shfl(slot, row, kWave);
+      row_off[i] = s * a.row_bytes + pair * S::kRow;
+      diff_dma16(a.k_cache + row_off[i] + ((dc ^ row) & (S::kChunks - 1)) * 16, uniform(base + i * 1024));
+    }
+  };
+  auto load_values = [&]() {
+    const u32 base = ring_lds + (lx % NS) * (2 * S::kTile) + S::kTile;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = i * S::kRowsPerLoad + dr;
+      diff_dma16(a.v_cache + row_off[i] + (dc ^ ((row & 7) << 1)) * 16, uniform(base + i * 1024));
+    }
+    ++lx;
+    if (lx < N) advance(lc);
+  };
+
+  // ---- prologue: the first ring of stages in flight, the next ring's page entries with them
+#pragma unroll 1
+  for (int i = 0; i < NS; ++i) fetch_pages();
+  diff_wait_vm<0>();
+#pragma unroll 1
+  for (int i = 0; i < NS && i < N; ++i) {
+    fetch_pages();
+    load_keys();
+    load_values();
+  }
+
+  // ---- the range
+  u32x4 q[2 * KS];
+  f32x4 o[NB][MB];
+  float m[NB], l[NB];
+  bool fresh = true;         // a context begins: its query rows are still to be fetched
+  bool first_run = true;     // the first context of the range
+  bool from_start = false;   // the context's first stage was this worker's
+  const int k_read = c16 * S::kRow;
+  const int v_row = 4 * g + (c16 >> 2);
+  const int v_read = v_row * S::kRow + (c16 & 1) * 8;
+  const int v_chunk = ((c16 & 3) >> 1) ^ ((v_row & 7) << 1);
+
+#pragma unroll 1
+  for (int s = 0; s < N; ++s) {
+    const int pair = cc.hb / a.hb_per_pair;
+    const int head0 = pair * a.group + (cc.hb - pair * a.hb_per_pair) * S::kHeads;   // first head of the block
+    const int heads = min(S::kHeads, (pair + 1) * a.group - head0);
+    if (fresh) {
+      fresh = false;
+      from_start = cc.st == 0;
+      const int head = NB == 1 ? c16 & 7 : c16;
+      const char* row = a.q + cc.b * a.q_stride_bytes + static_cast<int64_t>(head0 + (head < heads ? head : 0)) * (4 * D) + g * 16;
+#pragma unroll
+      for (int mp = 0; mp < 2; ++mp) {
+        const bool on = head < heads && (NB == 2 || (c16 >> 3) == mp);
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+          const u32x4 x = ldg16(row + mp * (2 * D) + kk * 64);
+          q[mp * KS + kk] = on ? x : u32x4{0, 0, 0, 0};
+        }
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        m[nb] = kNegBig;
+        l[nb] = 0.0f;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) o[nb][mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+    }
+    const bool more = s + NS < N;
+    const char* st = ring + (s % NS) * (2 * S::kTile);
+
+    // ---- keys: wait for them, read them, and fill their place again
+    if (s + NS <= N) diff_wait_vm<NL + (NS - 1) * kStageOps>();
+    else diff_wait_vm<0>();
+    u32x4 kr[2 * KS];
+#pragma unroll
+    for (int i = 0; i < 2 * KS; ++i)
+      kr[i] = *reinterpret_cast<const u32x4*>(st + k_read + (((i * 4 + g) ^ c16) & (S::kChunks - 1)) * 16);
+    diff_wait_lds();
+    if (more) {
+      fetch_pages();
+      load_keys();
+    }
+
+    // ---- scores: lane (column c16, tokens 4 g .. 4 g + 3)
+    f32x4 sc[NB];
+    {
+      f32x4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        s0 = Mfma<QT>::k32(kr[kk], q[kk], s0);
+        s1 = Mfma<QT>::k32(kr[KS + kk], q[KS + kk], s1);
+      }
+      if constexpr (NB == 1) {
+        sc[0] = s0 + s1;   // (each is zero in the other's columns)
+      } else {
+        sc[0] = s0;
+        sc[NB - 1] = s1;
+      }
+    }
+    const int tok0 = (cc.lo / kDiffTokens + cc.st) * kDiffTokens + 4 * g;
+    u32x2 p_hi[NB], p_lo[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float sv[4];
+      bool over = false;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sv[r] = tok0 + r < cc.L && tok0 + r >= cc.lo ? sc[nb][r] * a.scale_log2 : -INFINITY;
+        over |= sv[r] > m[nb] + kDiffSlack;
+      }
+      if (__builtin_amdgcn_ballot_w64(over) != 0) {   // rare once the maxima have settled
+        const float mx = diff_rows_max(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])));
+        if (mx > m[nb] + kDiffSlack) {
+          const float alpha = fast_exp2(m[nb] - mx);
+          m[nb] = mx;
+          l[nb] *= alpha;
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) o[nb][mb] *= alpha;
+        }
+      }
+      float p[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[r] = fast_exp2(sv[r] - m[nb]);
+        l[nb] += p[r];
+      }
+      p_hi[nb] = u32x2{QT::pack(p[0], p[1]), QT::pack(p[2], p[3])};
+      p_lo[nb] = u32x2{QT::pack(p[0] - QT::lo(p_hi[nb][0]), p[1] - QT::hi(p_hi[nb][0])),
+                       QT::pack(p[2] - QT::lo(p_hi[nb][1]), p[3] - QT::hi(p_hi[nb][1]))};
+    }
+
+    // ---- values: the same, by the transposing read (lane c16 of 16 supplies 4 dims of token 4 g + c16 / 4 and receives
+    // the 4 tokens 4 g .. of dim 16 mb + c16)
+    if (more) diff_wait_vm<(NS - 1) * kStageOps + 1 + NL>();
+    else diff_wait_vm<0>();
+    s16x4 vt[MB];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+      vt[mb] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((diff_lds_s16x4*)(st + S::kTile + v_read + ((v_chunk ^ (2 * mb)) * 16)));
+    diff_wait_lds();
+    if (more) load_values();
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        o[nb][mb] = Mfma<QT>::k16(vt[mb], p_hi[nb], o[nb][mb]);
+        o[nb][mb] = Mfma<QT>::k16(vt[mb], p_lo[nb], o[nb][mb]);
+      }
+
+    // ---- the end of the context, or of the range
+    const bool last = cc.st == cc.n - 1;
+    if (last || s == N - 1) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) l[nb] = diff_rows_sum(l[nb]);
+      if (last && from_start) {
+        const int head = NB == 1 ? c16 & 7 : c16;
+        const bool on = head < heads && (NB == 2 || c16 < 8);
+        const float lam = a.lambda[cc.b * a.lambda_batch_stride + (head0 + (head < heads ? head : 0)) * a.lambda_head_stride];
+        f32x4 d[MB];
+        const float inv0 = 1.0f / l[0], inv1 = 1.0f / l[NB - 1];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float v0 = o[0][mb][r] * inv0;
+            // (one block: the same head's column of the other map is eight lanes on, row_ror:8)
+            const float v1 = NB == 1 ? dpp<0x128>(v0) : o[NB - 1][mb][r] * inv1;
+            d[mb][r] = diff_of(v0, lam, v1);
+          }
+        diff_store_row<QT, MB>(a, d, cc.b, head0 + (head < heads ? head : 0), on, g);
+      } else {
+        const int64_t slot = 2 * static_cast<int64_t>(worker) + (first_run ? 0 : 1);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int head = NB == 1 ? c16 & 7 : c16;
+          const int64_t col = slot * S::kCols + nb * 16 + c16;
+          if (head < heads) {
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) *reinterpret_cast<f32x4*>(a.ws_o + col * (2 * D) + mb * 16 + 4 * g) = o[nb][mb];
+            if (g == 0) *reinterpret_cast<f32x2*>(a.ws_ml + col * 2) = f32x2{m[nb], l[nb]};
+          }
+        }
+      }
+      first_run = false;
+      fresh = true;
+    }
+    if (s + 1 < N) advance(cc);
+  }
+}
+
+// Joins the parts of the contexts that several workers hold, and writes zeros for empty contexts.  One workgroup per
+// (head, sequence); the parts are dealt to its wavefronts, a lane holds 2 D / 64 dims of both maps.  The parts are read
+// and added in the order of the list, whatever order they were written in.
+template <typename QT, int D, int NB>
+__global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(DiffArgs a) {
+  using S = DiffShape<D, NB>;
+  constexpr int E = 2 * D / kWave;   // dims per lane
+  typedef __attribute__((ext_vector_type(E))) float fvec;
+  __shared__ float acc[kDiffWaves][2][2 * D];
+  __shared__ float sums[kDiffWaves][2][2];   // maximum, sum
+  const int head = blockIdx.x, b = blockIdx.y;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int pair = head / a.group;
+  const int in_pair = head - pair * a.group;
+  const int hb = pair * a.hb_per_pair + in_pair / S::kHeads;
+  const int h = in_pair % S::kHeads;
+  const int n_hb = a.n_pairs * a.hb_per_pair;
+  const int p0 = a.ws_prefix[b], n = a.ws_prefix[b + 1] - p0;
+  char* row = a.out + b * a.out_stride_bytes + static_cast<int64_t>(head) * (4 * D);
+  if (n == 0) {
+    if (wave == 0)
+      for (int i = 0; i < E / 2; ++i) reinterpret_cast<u32*>(row)[lane * (E / 2) + i] = 0;
+    return;
+  }
+  const int64_t total = static_cast<int64_t>(a.ws_prefix[a.batch]) * n_hb;
+  const int used = diff_used(a, total);
+  const int64_t s0 = static_cast<int64_t>(p0) * n_hb + static_cast<int64_t>(hb) * n, s1 = s0 + n - 1;
+  auto worker_of = [&](int64_t id) {
+    int w = static_cast<int>(id * used / total);
+    while (w + 1 < used && diff_start(w + 1, total, used) <= id) ++w;
+    return w;
+  };
+  const int wf = worker_of(s0), wl = worker_of(s1);
+  if (wf == wl) return;   // one worker held it whole and wrote the row
+  const int first_slot = diff_start(wf, total, used) < s0 ? 1 : 0;
+  auto column = [&](int w, int mp) {
+    const int64_t slot = 2 * static_cast<int64_t>(w) + (w == wf ? first_slot : 0);
+    return slot * S::kCols + (NB == 1 ? mp * 8 : mp * 16) + h;
+  };
+  fvec o[2];
+  float m[2], l[2];
+#pragma unroll
+  for (int mp = 0; mp < 2; ++mp) {
+    o[mp] = fvec(0.0f);
+    m[mp] = kNegBig;
+    l[mp] = 0.0f;
+  }
+#pragma unroll 4
+  for (int w = wf + wave; w <= wl; w += kDiffWaves) {
+#pragma unroll
+    for (int mp = 0; mp < 2; ++mp) {
+      const int64_t col = column(w, mp);
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(a.ws_ml + col * 2);
+      const fvec x = *reinterpret_cast<const fvec*>(a.ws_o + col * (2 * D) + lane * E);
+      const float mx = fmaxf(m[mp], ml[0]);
+      const float f0 = fast_exp2(m[mp] - mx), f1 = fast_exp2(ml[0] - mx);
+      o[mp] = o[mp] * f0 + x * f1;
+      l[mp] = l[mp] * f0 + ml[1] * f1;
+      m[mp] = mx;
+    }
+  }
+#pragma unroll
+  for (int mp = 0; mp < 2; ++mp) {
+    *reinterpret_cast<fvec*>(&acc[wave][mp][lane * E]) = o[mp];
+    if (lane == 0) {
+      sums[wave][mp][0] = m[mp];
+      sums[wave][mp][1] = l[mp];
+    }
+  }
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int mp = 0; mp < 2; ++mp) {
+    float mx = m[mp];
+#pragma unroll
+    for (int w = 1; w < kDiffWaves; ++w) mx = fmaxf(mx, sums[w][mp][0]);
+    fvec t = fvec(0.0f);
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kDiffWaves; ++w) {
+      const float f = fast_exp2(sums[w][mp][0] - mx);
+      t += *reinterpret_cast<const fvec*>(&acc[w][mp][lane * E]) * f;
+      sum += sums[w][mp][1] * f;
+    }
+    o[mp] = t * (1.0f / sum);
+  }
+  const float lam = a.lambda[b * a.lambda_batch_stride + head * a.lambda_head_stride];
+  fvec d;
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) d[i] = diff_of(o[0][i], lam, o[1][i]);
+#pragma unroll
+  for (int i = 0; i < E; ++i) ss += d[i] * d[i];
+  ss = group_sum<32>(ss);
+  ss += __shfl_xor(ss, 32, kWave);
+  float f = a.out_scale;
+  if (a.norm_w != nullptr) f *= 1.0f / __builtin_sqrtf(ss / static_cast<float>(2 * D) + a.eps);
+#pragma unroll
+  for (int i = 0; i < E; i += 2) {
+    float w0 = 1.0f, w1 = 1.0f;
+    if (a.norm_w != nullptr) {
+      const u32 x = reinterpret_cast<const u32*>(a.norm_w)[(lane * E + i) / 2];
+      w0 = QT::lo(x);
+      w1 = QT::hi(x);
+    }
+    reinterpret_cast<u32*>(row)[(lane * E + i) / 2] = QT::pack(d[i] * f * w0, d[i + 1] * f * w1);
+  }
+}
+
+template <typename QT, int D, int NB>
+int launch_diff(const DiffArgs& a, hipStream_t stream) {
+  using S = DiffShape<D, NB>;
+  static std::atomic<uint64_t> seen{0};
+  const void* kern = reinterpret_cast<const void*>(diff_decode_kernel<QT, D, NB>);
+  if (first_use_on_current_device(seen)) {
+    const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(S::lds_bytes(kDiffMaxBatch)));
+    if (e != hipSuccess) return static_cast<int>(e);
+  }
+  launch_timed(diff_decode_kernel<QT, D, NB>, dim3(static_cast<unsigned>(a.n_workers / kDiffWaves)), dim3(kDiffThreads),
+               S::lds_bytes(a.batch), stream, a);
+  int rc = static_cast<int>(hipGetLastError());
+  if (rc != 0) return rc;
+  launch_timed(diff_merge_kernel<QT, D, NB>, dim3(static_cast<unsigned>(a.n_heads), static_cast<unsigned>(a.batch)),
+               dim3(kDiffThreads), 0, stream, a);
+  return static_cast<int>(hipGetLastError());
+}
+
+template <typename QT>
+int dispatch_diff(const DiffArgs& a, int64_t head_dim, hipStream_t stream) {
+  if (head_dim == 64) return a.group <= 8 ? launch_diff<QT, 64, 1>(a, stream) : launch_diff<QT, 64, 2>(a, stream);
+  return a.group <= 8 ? launch_diff<QT, 128, 1>(a, stream) : launch_diff<QT, 128, 2>(a, stream);
+}
+
+size_t diff_prefix_bytes() { return (static_cast<size_t>(kDiffMaxBatch + 1) * 4 + 255) / 256 * 256; }
+int64_t diff_columns(int64_t group) { return group <= 8 ? 16 : 32; }
+
+}  // namespace
+
+// prefix | maxima and sums | partial rows, two slots per worker
+size_t diff_workspace_bytes(int64_t n_heads, int64_t n_pairs, int64_t head_dim) {
+  if (n_heads <= 0 || n_pairs <= 0 || n_heads % n_pairs != 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  const size_t cols = static_cast<size_t>(device_cu_count()) * kDiffWaves * 2 * diff_columns(n_heads / n_pairs);
+  return diff_prefix_bytes() + cols * 2 * 4 + cols * 2 * head_dim * 4;
+}
+
+int paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, void* out, const int32_t* block_table,
+                      int64_t table_stride, int64_t table_width, const int32_t* seq_lens, const float* lambda,
+                      int64_t lambda_batch_stride, int64_t lambda_head_stride, const void* norm_weight, float eps,
+                      float out_scale, int64_t batch, int64_t n_heads, int64_t n_kv_pairs, int64_t head_dim,
+                      int64_t block_size, int64_t num_blocks, int64_t q_token_stride, int64_t out_token_stride,
+                      int64_t window_left, float sm_scale, void* workspace, size_t workspace_bytes, int dtype,
+                      hipStream_t stream) {
+  if (batch == 0) return XLLM_MI355_OK;
+  if (q == nullptr || k_cache == nullptr || v_cache == nullptr || out == nullptr || block_table == nullptr ||
+      seq_lens == nullptr || lambda == nullptr)
+    return XLLM_MI355_EINVAL;
+  if (batch < 0 || n_heads <= 0 || n_kv_pairs <= 0 || n_heads % n_kv_pairs != 0 || n_heads > 65535 || block_size <= 0 ||
+      num_blocks <= 0 || table_width <= 0 || table_stride < table_width || !(sm_scale > 0.0f) || !(eps >= 0.0f) ||
+      lambda_batch_stride < 0 || lambda_head_stride < 0)
+    return XLLM_MI355_EINVAL;
+  if (dtype != XLLM_MI355_BF16 && dtype != XLLM_MI355_FP16) return XLLM_MI355_EDTYPE;
+  if (head_dim != 64 && head_dim != 128) return XLLM_MI355_ESHAPE;
+  if (block_size > 0x7fffffffLL || num_blocks > 0x7fffffffLL || num_blocks * block_size > 0x7fffffffLL)
+    return XLLM_MI355_ESHAPE;
+  if (q_token_stride < 2 * n_heads * head_dim || out_token_stride < 2 * n_heads * head_dim) return XLLM_MI355_EINVAL;
+  auto aligned = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || (q_token_stride & 7) != 0 || !aligned(out, 8) ||
+      (out_token_stride & 3) != 0 || !aligned(norm_weight, 8))
+    return XLLM_MI355_EALIGN;
+  const size_t need = diff_workspace_bytes(n_heads, n_kv_pairs, head_dim);
+  if (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < need) return XLLM_MI355_EWORKSPACE;
+
+  DiffArgs a = {};
+  a.n_heads = static_cast<int>(n_heads);
+  a.n_pairs = static_cast<int>(n_kv_pairs);
+  a.group = static_cast<int>(n_heads / n_kv_pairs);
+  const int per_block = a.group <= 8 ? 8 : 16;
+  a.hb_per_pair = (a.group + per_block - 1) / per_block;
+  a.block_size = static_cast<int>(block_size);
+  a.bs_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if ((1LL << s) == block_size) a.bs_shift = s;
+  a.num_blocks = static_cast<int>(num_blocks);
+  const bool long_table = table_width > (0x7fffffffLL - 16) / block_size;
+  a.max_len = long_table ? 0x7fffffff - 16 : static_cast<int>(table_width * block_size);
+  a.window_left = window_left < 0 ? -1 : static_cast<int>(window_left < 0x7fffffffLL ? window_left : 0x7fffffffLL);
+  a.n_workers = device_cu_count() * kDiffWaves;
+  a.scale_log2 = sm_scale * kLog2e;
+  a.eps = eps;
+  a.out_scale = out_scale;
+  a.k_cache = static_cast<const char*>(k_cache);
+  a.v_cache = static_cast<const char*>(v_cache);
+  a.norm_w = static_cast<const char*>(norm_weight);
+  a.table_stride = table_stride;
+  a.q_stride_bytes = q_token_stride * 2;
+  a.out_stride_bytes = out_token_stride * 2;
+  a.row_bytes = n_kv_pairs * head_dim * 4;
+  a.lambda_batch_stride = lambda_batch_stride;
+  a.lambda_head_stride = lambda_head_stride;
+  char* ws = static_cast<char*>(workspace);
+  const size_t cols = static_cast<size_t>(a.n_workers) * 2 * diff_columns(a.group);
+  a.ws_prefix = reinterpret_cast<int*>(ws);
+  a.ws_ml = reinterpret_cast<float*>(ws + diff_prefix_bytes());
+  a.ws_o = a.ws_ml + cols * 2;
+  // batches beyond the LDS prefix are decoded in slices, one launch pair after the other
+  for (int64_t b0 = 0; b0 < batch; b0 += kDiffMaxBatch) {
+    a.batch = static_cast<int>(batch - b0 < kDiffMaxBatch ? batch - b0 : kDiffMaxBatch);
+    a.q = static_cast<const char*>(q) + b0 * a.q_stride_bytes;
+    a.out = static_cast<char*>(out) + b0 * a.out_stride_bytes;
+    a.block_table = block_table + b0 * table_stride;
+    a.seq_lens = seq_lens + b0;
+    a.lambda = lambda + b0 * lambda_batch_stride;
+    const int rc = dtype == XLLM_MI355_BF16 ? dispatch_diff<BF16>(a, head_dim, stream) : dispatch_diff<FP16>(a, head_dim, stream);
+    if (rc != 0) return rc;
+  }
+  return XLLM_MI355_OK;
+}
+
+}  // namespace xllm_mi355

@@ -1,0 +1,663 @@
+// Rotary positions outside the fused qkv buffer (rope_and_cache.hip serves that one), for gfx950:
+//   rope_cos_sin             cos | sin rows of positions, from frequencies that may be scaled for long contexts
+//   rotary_embedding         rotation of q and k held in tensors of their own, part of the head, either pair layout, and
+//                            its transpose (the inverse rotation, which is also its gradient)
+//   mla_norm_rope_and_cache  the MLA counterpart of rope_and_cache: RMS norm of the latent, rotation of the rope keys and
+//                            queries, and the store into the latent cache
+//
+// Pairs are (a, b) = (x[2i], x[2i+1]) when interleaved, (x[i], x[i + R/2]) otherwise:
+//   (a, b) -> (a c_i - b s_i, b c_i + a s_i)
+// in fp32 between one load and one store.  All three are bound by the bytes they move (a few operations per element) or,
+// at decode sizes, by the launch: the kernels read and write 16 bytes per lane and instruction and keep several in flight.
+#include "common.cuh"
+#include "launch.h"
+
+namespace xllm_mi355 {
+
+namespace {
+
+constexpr int kRotThreads = 256;
+
+// ---- element types ------------------------------------------------------------------------------------------------
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<XLLM_MI355_BF16> {
+  using T = uint16_t;
+  static __device__ __forceinline__ float get(T x) { return BF16::to_f32(x); }
+  static __device__ __forceinline__ T put(float x) { return BF16::from_f32(x); }
+};
+template <>
+struct Elem<XLLM_MI355_FP16> {
+  using T = uint16_t;
+  static __device__ __forceinline__ float get(T x) { return FP16::to_f32(x); }
+  static __device__ __forceinline__ T put(float x) { return FP16::from_f32(x); }
+};
+template <>
+struct Elem<XLLM_MI355_FP32> {
+  using T = float;
+  static __device__ __forceinline__ float get(T x) { return x; }
+  static __device__ __forceinline__ T put(float x) { return x; }
+};
+
+// N elements as 16-byte words.
+template <int DT, int N>
+struct Pack {
+  using T = typename Elem<DT>::T;
+  static constexpr int kWords = N * static_cast<int>(sizeof(T)) / 16;
+  static_assert(kWords >= 1 && kWords * 16 == N * static_cast<int>(sizeof(T)), "whole 16-byte words");
+  u32x4 w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const u32x4*>(p)[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) reinterpret_cast<u32x4*>(p)[i] = w[i];
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (DT == XLLM_MI355_FP32) {
+      return as_f32(w[i / 4][i % 4]);
+    } else {
+      const u32 x = w[i / 8][(i / 2) % 4];
+      return Elem<DT>::get(static_cast<uint16_t>((i & 1) ? x >> 16 : x & 0xffffu));
+    }
+  }
+  // elements 2 i and 2 i + 1
+  __device__ __forceinline__ void put2(int i, float a, float b) {
+    if constexpr (DT == XLLM_MI355_FP32) {
+      w[i / 2][(2 * i) % 4] = as_u32(a);
+      w[i / 2][(2 * i) % 4 + 1] = as_u32(b);
+    } else if constexpr (DT == XLLM_MI355_BF16) {
+      w[i / 4][i % 4] = BF16::pack(a, b);
+    } else {
+      w[i / 4][i % 4] = FP16::pack(a, b);
+    }
+  }
+};
+
+// ---- cos | sin rows ------------------------------------------------------------------------------------------------
+
+// cos and sin of `angle` in 64 bits: the multiple of pi / 2 is taken off in two parts (its product with the leading part
+// is exact inside the fused multiply-add, so the remainder of angles up to 2^30 is good to 2^-52 of the quadrant), then
+// the Taylor polynomials on [-pi/4, pi/4], whose first omitted terms are below 2e-14 and 7e-16.
+__device__ __forceinline__ void cos_sin_64(double angle, double& c, double& s) {
+  const double q = __builtin_rint(angle * 0.63661977236758134308);
+  double r = __builtin_fma(-q, 1.5707963267948965580, angle);
+  r = __builtin_fma(-q, 6.1232339957367660359e-17, r);
+  const double z = r * r;
+  double ps = 1.0 / 6227020800.0;
+  ps = __builtin_fma(ps, z, -1.0 / 39916800.0);
+  ps = __builtin_fma(ps, z, 1.0 / 362880.0);
+  ps = __builtin_fma(ps, z, -1.0 / 5040.0);
+  ps = __builtin_fma(ps, z, 1.0 / 120.0);
+  ps = __builtin_fma(ps, z, -1.0 / 6.0);
+  const double sr = __builtin_fma(r * z, ps, r);
+  double pc = -1.0 / 87178291200.0;
+  pc = __builtin_fma(pc, z, 1.0 / 479001600.0);
+  pc = __builtin_fma(pc, z, -1.0 / 3628800.0);
+  pc = __builtin_fma(pc, z, 1.0 / 40320.0);
+  pc = __builtin_fma(pc, z, -1.0 / 720.0);
+  pc = __builtin_fma(pc, z, 1.0 / 24.0);
+  pc = __builtin_fma(pc, z, -0.5);
+  const double cr = __builtin_fma(pc, z, 1.0);
+  // the quadrant, q mod 4, without going through an integer that q may not fit
+  const double k = q - 4.0 * __builtin_floor(q * 0.25);
+  const bool swap = k == 1.0 || k == 3.0;
+  c = swap ? sr : cr;
+  s = swap ? cr : sr;
+  if (k == 1.0 || k == 2.0) c = -c;
+  if (k >= 2.0) s = -s;
+}
+
+// One lane makes V consecutive pairs of a row: V cosines and V sines, 16 bytes of each where the row allows it.
+template <int DT, int V>
+__global__ __launch_bounds__(kRotThreads) void rope_cos_sin_kernel(const double* inv_freq, const int64_t* positions,
+                                                                   int64_t first, int64_t n_units, int half, double factor,
+                                                                   typename Elem<DT>::T* out) {
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotThreads + threadIdx.x;
+  if (unit >= n_units) return;
+  const int per = half / V;
+  // (32-bit division where it fits, which is every table below 2^31 lanes)
+  const int64_t row = n_units <= 0x7fffffffLL ? static_cast<u32>(unit) / static_cast<u32>(per) : unit / per;
+  const int i0 = static_cast<int>(unit - row * per) * V;
+  const double pos = static_cast<double>(positions != nullptr ? positions[row] : first + row);
+  typename Elem<DT>::T* p = out + row * (2 * static_cast<int64_t>(half)) + i0;
+  float c[V], s[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    double cd, sd;
+    cos_sin_64(pos * inv_freq[i0 + i], cd, sd);
+    c[i] = static_cast<float>(cd * factor);
+    s[i] = static_cast<float>(sd * factor);
+  }
+  if constexpr (V == 1) {
+    p[0] = Elem<DT>::put(c[0]);
+    p[half] = Elem<DT>::put(s[0]);
+  } else {
+    Pack<DT, V> a, b;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      a.put2(i, c[2 * i], c[2 * i + 1]);
+      b.put2(i, s[2 * i], s[2 * i + 1]);
+    }
+    a.store(p);
+    b.store(p + half);
+  }
+}
+
+template <int DT>
+int launch_cos_sin(const double* inv_freq, const int64_t* positions, int64_t first, int64_t rows, int64_t half,
+                   double factor, void* out, hipStream_t stream) {
+  constexpr int V = DT == XLLM_MI355_FP32 ? 4 : 8;
+  using T = typename Elem<DT>::T;
+  const bool wide = half % V == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const int64_t units = rows * (wide ? half / V : half);
+  const int64_t groups = (units + kRotThreads - 1) / kRotThreads;
+  if (groups > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
+  const dim3 grid(static_cast<unsigned>(groups));
+  if (wide)
+    rope_cos_sin_kernel<DT, V><<<grid, kRotThreads, 0, stream>>>(inv_freq, positions, first, units, static_cast<int>(half),
+                                                                 factor, static_cast<T*>(out));
+  else
+    rope_cos_sin_kernel<DT, 1><<<grid, kRotThreads, 0, stream>>>(inv_freq, positions, first, units, static_cast<int>(half),
+                                                                 factor, static_cast<T*>(out));
+  return static_cast<int>(hipGetLastError());
+}
+
+// ---- rotation ------------------------------------------------------------------------------------------------------
+
+struct RotSide {            // q or k; strides in elements
+  const char* in;
+  char* out;
+  int64_t in_token, in_head, out_token, out_head;
+  int heads, dim, offset;
+};
+
+struct RotArgs {
+  RotSide q, k;
+  const int64_t* positions;
+  const char* cos_sin;
+  int64_t n_positions;      // rows of cos_sin; a position outside [0, n_positions) is not rotated
+  int64_t n_units;
+  int rot;                  // rotated dims R
+  int rot_units;            // lanes per head and rotated part
+  int units;                // lanes per head: the rotated part, and for out of place the rest of the wider side
+  int slots;                // groups of U heads per token: those of q, then those of k
+  int q_slots;
+};
+
+// cos and sin of pairs [i, i + P) of a table row.
+template <int CT, int P, bool VEC>
+__device__ __forceinline__ void rot_row(const char* table, int64_t row, int rot, int i, float (&c)[P], float (&s)[P]) {
+  using T = typename Elem<CT>::T;
+  const T* p = reinterpret_cast<const T*>(table) + row * rot + i;
+  if constexpr (VEC && P * sizeof(T) >= 16) {
+    Pack<CT, P> a, b;
+    a.load(p);
+    b.load(p + rot / 2);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      c[j] = a.get(j);
+      s[j] = b.get(j);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      c[j] = Elem<CT>::get(p[j]);
+      s[j] = Elem<CT>::get(p[rot / 2 + j]);
+    }
+  }
+}
+
+// A lane owns P pairs (P = 16 bytes of elements, so two 16-byte words: the pairs' two halves, or two neighbouring words
+// when interleaved) of U consecutive heads of a token: one set of cosines and sines serves all of them.  Lanes behind the
+// rotated part copy the rest of the head, 2 P elements each, when the result goes elsewhere.
+// VEC = false takes one pair (or two elements to copy) per lane, for operands that are not aligned to 16 bytes.
+template <int DT, int CT, bool INTERLEAVE, bool VEC, int U>
+__global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a, float sin_sign) {
+  using T = typename Elem<DT>::T;
+  constexpr int P = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  const int64_t idx = static_cast<int64_t>(blockIdx.x) * kRotThreads + threadIdx.x;
+  if (idx >= a.n_units) return;
+  int64_t rest, token;
+  int unit, slot;
+  if (a.n_units <= 0x7fffffffLL) {
+    const u32 r = static_cast<u32>(idx) / static_cast<u32>(a.units);
+    unit = static_cast<int>(static_cast<u32>(idx) - r * static_cast<u32>(a.units));
+    const u32 t = r / static_cast<u32>(a.slots);
+    slot = static_cast<int>(r - t * static_cast<u32>(a.slots));
+    token = t;
+  } else {
+    rest = idx / a.units;
+    unit = static_cast<int>(idx - rest * a.units);
+    token = rest / a.slots;
+    slot = static_cast<int>(rest - token * a.slots);
+  }
+  const bool is_q = slot < a.q_slots;
+  const RotSide& sd = is_q ? a.q : a.k;
+  const int head0 = (is_q ? slot : slot - a.q_slots) * U;
+  const T* in = reinterpret_cast<const T*>(sd.in) + token * sd.in_token + head0 * sd.in_head;
+  T* out = reinterpret_cast<T*>(sd.out) + token * sd.out_token + head0 * sd.out_head;
+  const int64_t in_head = sd.in_head, out_head = sd.out_head;
+  const int heads = min(U, sd.heads - head0);
+
+  if (unit >= a.rot_units) {   // the rest of the head: what lies before the rotated part, then what lies behind it
+    const int e0 = (unit - a.rot_units) * 2 * P;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int e = e0 + w * P;
+      if (e >= sd.dim - a.rot) break;
+      const int d = e < sd.offset ? e : e + a.rot;
+      if constexpr (VEC) {
+        Pack<DT, P> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u < heads) x[u].load(in + u * in_head + d);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u < heads) x[u].store(out + u * out_head + d);
+      } else {
+        for (int u = 0; u < heads; ++u) out[u * out_head + d] = in[u * in_head + d];
+      }
+    }
+    return;
+  }
+
+  const int i = unit * P;                                                    // first pair
+  const int da = sd.offset + (INTERLEAVE ? 2 * i : i);                       // where the pairs' words lie
+  const int db = sd.offset + (INTERLEAVE ? 2 * i + P : i + a.rot / 2);
+  if constexpr (VEC) {
+    Pack<DT, P> x[U], y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < heads) {
+        x[u].load(in + u * in_head + da);
+        y[u].load(in + u * in_head + db);
+      }
+    const int64_t pos = a.positions[token];
+    float c[P], s[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      c[j] = 1.0f;
+      s[j] = 0.0f;
+    }
+    const bool turn = pos >= 0 && pos < a.n_positions;
+    if (turn) rot_row<CT, P, true>(a.cos_sin, pos, a.rot, i, c, s);
+#pragma unroll
+    for (int j = 0; j < P; ++j) s[j] *= sin_sign;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u >= heads) continue;
+      if (turn) {
+        if constexpr (INTERLEAVE) {
+#pragma unroll
+          for (int j = 0; j < P; ++j) {
+            Pack<DT, P>& w = j < P / 2 ? x[u] : y[u];
+            const int e = j < P / 2 ? j : j - P / 2;
+            const float p0 = w.get(2 * e), p1 = w.get(2 * e + 1);
+            w.put2(e, __builtin_fmaf(p0, c[j], -(p1 * s[j])), __builtin_fmaf(p1, c[j], p0 * s[j]));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < P; j += 2) {
+            const float a0 = x[u].get(j), a1 = x[u].get(j + 1), b0 = y[u].get(j), b1 = y[u].get(j + 1);
+            x[u].put2(j / 2, __builtin_fmaf(a0, c[j], -(b0 * s[j])), __builtin_fmaf(a1, c[j + 1], -(b1 * s[j + 1])));
+            y[u].put2(j / 2, __builtin_fmaf(b0, c[j], a0 * s[j]), __builtin_fmaf(b1, c[j + 1], a1 * s[j + 1]));
+          }
+        }
+      }
+      x[u].store(out + u * out_head + da);
+      y[u].store(out + u * out_head + db);
+    }
+  } else {
+    const int64_t pos = a.positions[token];
+    float c[1] = {1.0f}, s[1] = {0.0f};
+    const bool turn = pos >= 0 && pos < a.n_positions;
+    if (turn) rot_row<CT, 1, false>(a.cos_sin, pos, a.rot, i, c, s);
+    s[0] *= sin_sign;
+    for (int u = 0; u < heads; ++u) {
+      const T xa = in[u * in_head + da], xb = in[u * in_head + db];
+      const float p0 = Elem<DT>::get(xa), p1 = Elem<DT>::get(xb);
+      out[u * out_head + da] = turn ? Elem<DT>::put(__builtin_fmaf(p0, c[0], -(p1 * s[0]))) : xa;
+      out[u * out_head + db] = turn ? Elem<DT>::put(__builtin_fmaf(p1, c[0], p0 * s[0])) : xb;
+    }
+  }
+}
+
+template <int DT, int CT, bool INTERLEAVE, bool VEC, int U>
+int launch_rotary(RotArgs a, bool copy_rest, int inverse, int64_t n_tokens, hipStream_t stream) {
+  constexpr int P = VEC ? 16 / static_cast<int>(sizeof(typename Elem<DT>::T)) : 1;
+  a.rot_units = a.rot / 2 / P;
+  const int wide = a.k.heads > 0 && a.k.dim > a.q.dim ? a.k.dim : a.q.dim;
+  a.units = a.rot_units + (copy_rest ? (wide - a.rot + 2 * P - 1) / (2 * P) : 0);
+  a.q_slots = (a.q.heads + U - 1) / U;
+  a.slots = a.q_slots + (a.k.heads + U - 1) / U;
+  a.n_units = n_tokens * a.slots * a.units;
+  const int64_t groups = (a.n_units + kRotThreads - 1) / kRotThreads;
+  if (groups > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
+  rotary_kernel<DT, CT, INTERLEAVE, VEC, U><<<dim3(static_cast<unsigned>(groups)), kRotThreads, 0, stream>>>(
+      a, inverse != 0 ? -1.0f : 1.0f);
+  return static_cast<int>(hipGetLastError());
+}
+
+template <int DT, int CT, bool INTERLEAVE>
+int dispatch_rotary_units(const RotArgs& a, bool vec, bool copy_rest, int inverse, int64_t n_tokens, hipStream_t stream) {
+  if (!vec) return launch_rotary<DT, CT, INTERLEAVE, false, 1>(a, copy_rest, inverse, n_tokens, stream);
+  // one head per lane while that keeps the launch small (decode), four beyond: see the figures at rotary_embedding
+  if (n_tokens * (a.q.heads + a.k.heads) * a.rot < (1LL << 22))
+    return launch_rotary<DT, CT, INTERLEAVE, true, 1>(a, copy_rest, inverse, n_tokens, stream);
+  return launch_rotary<DT, CT, INTERLEAVE, true, 4>(a, copy_rest, inverse, n_tokens, stream);
+}
+
+template <int DT>
+int dispatch_rotary(const RotArgs& a, int cos_sin_dtype, int interleave, bool vec, bool copy_rest, int inverse,
+                    int64_t n_tokens, hipStream_t stream) {
+#define XLLM_ROT(CT)                                                                                            \
+  (interleave != 0 ? dispatch_rotary_units<DT, CT, true>(a, vec, copy_rest, inverse, n_tokens, stream)          \
+                   : dispatch_rotary_units<DT, CT, false>(a, vec, copy_rest, inverse, n_tokens, stream))
+  switch (cos_sin_dtype) {
+    case XLLM_MI355_FP32: return XLLM_ROT(XLLM_MI355_FP32);
+    case XLLM_MI355_BF16: return XLLM_ROT(XLLM_MI355_BF16);
+    case XLLM_MI355_FP16: return XLLM_ROT(XLLM_MI355_FP16);
+    default: return XLLM_MI355_EDTYPE;
+  }
+#undef XLLM_ROT
+}
+
+// ---- MLA prologue --------------------------------------------------------------------------------------------------
+
+constexpr int kLatent = 512, kRopeDim = 64;   // the widths that the MLA decode reads
+
+struct MlaPrologueArgs {
+  const uint16_t* q;
+  uint16_t* q_out;
+  const uint16_t* kv;
+  uint16_t* kv_out;          // or null
+  const uint16_t* weight;
+  const char* cos_sin;
+  const int64_t* positions;
+  uint16_t* cache;           // or null
+  const int32_t* slots;
+  int64_t n_tokens, n_positions, n_slots;
+  int64_t q_token, q_head, q_out_token, q_out_head, kv_row, kv_out_row;
+  int64_t q_units;           // lanes of the query part
+  int heads, head_slots;     // head_slots: groups of U heads
+  int kv_blocks;             // workgroups of the latent part, the first ones of the grid
+  float eps;
+};
+
+// Eight pairs of one head's 64 rope dims: two 16-byte words (see rotary_kernel).
+template <int DT, bool INTERLEAVE>
+__device__ __forceinline__ void turn_words(Pack<DT, 8>& x, Pack<DT, 8>& y, const float (&c)[8], const float (&s)[8]) {
+  if constexpr (INTERLEAVE) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      Pack<DT, 8>& w = j < 4 ? x : y;
+      const int e = j & 3;
+      const float p0 = w.get(2 * e), p1 = w.get(2 * e + 1);
+      w.put2(e, __builtin_fmaf(p0, c[j], -(p1 * s[j])), __builtin_fmaf(p1, c[j], p0 * s[j]));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const float a0 = x.get(j), a1 = x.get(j + 1), b0 = y.get(j), b1 = y.get(j + 1);
+      x.put2(j / 2, __builtin_fmaf(a0, c[j], -(b0 * s[j])), __builtin_fmaf(a1, c[j + 1], -(b1 * s[j + 1])));
+      y.put2(j / 2, __builtin_fmaf(b0, c[j], a0 * s[j]), __builtin_fmaf(b1, c[j + 1], a1 * s[j + 1]));
+    }
+  }
+}
+
+// The first kv_blocks workgroups take the tokens' latent rows, one wavefront per row: eight latent values per lane (one
+// 16-byte word), their sum of squares over the wavefront, and the rope part in lanes 0-3.  The others rotate the rope
+// part of the query heads, four lanes per head and U heads per lane.
+template <int DT, int CT, bool INTERLEAVE, int U>
+__global__ __launch_bounds__(kRotThreads) void mla_prologue_kernel(MlaPrologueArgs a) {
+  constexpr int kUnits = kRopeDim / 16;
+  if (static_cast<int>(blockIdx.x) < a.kv_blocks) {
+    const int64_t token = static_cast<int64_t>(blockIdx.x) * (kRotThreads / kWave) + threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1);
+    if (token >= a.n_tokens) return;
+    const uint16_t* row = a.kv + token * a.kv_row;
+    Pack<DT, 8> x, w, ra, rb;
+    x.load(row + lane * 8);
+    w.load(a.weight + lane * 8);
+    const int unit = lane & (kUnits - 1);
+    const int da = kLatent + (INTERLEAVE ? unit * 16 : unit * 8);
+    const int db = kLatent + (INTERLEAVE ? unit * 16 + 8 : unit * 8 + kRopeDim / 2);
+    ra.load(row + da);
+    rb.load(row + db);
+    const int64_t pos = a.positions[token];
+    const bool turn = pos >= 0 && pos < a.n_positions;
+    float c[8], s[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      c[j] = 1.0f;
+      s[j] = 0.0f;
+    }
+    if (turn) rot_row<CT, 8, true>(a.cos_sin, pos, kRopeDim, unit * 8, c, s);
+    const int64_t slot = a.cache != nullptr ? a.slots[token] : -1;
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += x.get(j) * x.get(j);
+    ss = group_sum<32>(ss);
+    ss += __shfl_xor(ss, 32, kWave);
+    const float r = 1.0f / __builtin_sqrtf(ss * (1.0f / kLatent) + a.eps);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.put2(j, x.get(2 * j) * r * w.get(2 * j), x.get(2 * j + 1) * r * w.get(2 * j + 1));
+    if (turn) turn_words<DT, INTERLEAVE>(ra, rb, c, s);
+    if (a.kv_out != nullptr) {
+      uint16_t* o = a.kv_out + token * a.kv_out_row;
+      x.store(o + lane * 8);
+      if (lane < kUnits) {
+        ra.store(o + da);
+        rb.store(o + db);
+      }
+    }
+    if (slot >= 0 && slot < a.n_slots) {
+      uint16_t* o = a.cache + slot * (kLatent + kRopeDim);
+      x.store(o + lane * 8);
+      if (lane < kUnits) {
+        ra.store(o + da);
+        rb.store(o + db);
+      }
+    }
+    return;
+  }
+  const int64_t idx = static_cast<int64_t>(blockIdx.x - a.kv_blocks) * kRotThreads + threadIdx.x;
+  if (idx >= a.q_units) return;
+  const int unit = static_cast<int>(idx & (kUnits - 1));
+  const int64_t rest = idx / kUnits;
+  const int64_t token = a.q_units <= 0x7fffffffLL ? static_cast<u32>(rest) / static_cast<u32>(a.head_slots) : rest / a.head_slots;
+  const int head0 = static_cast<int>(rest - token * a.head_slots) * U;
+  const int heads = min(U, a.heads - head0);
+  const int da = INTERLEAVE ? unit * 16 : unit * 8;
+  const int db = INTERLEAVE ? unit * 16 + 8 : unit * 8 + kRopeDim / 2;
+  const uint16_t* in = a.q + token * a.q_token + head0 * a.q_head;
+  uint16_t* out = a.q_out + token * a.q_out_token + head0 * a.q_out_head;
+  Pack<DT, 8> x[U], y[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (u < heads) {
+      x[u].load(in + u * a.q_head + da);
+      y[u].load(in + u * a.q_head + db);
+    }
+  const int64_t pos = a.positions[token];
+  const bool turn = pos >= 0 && pos < a.n_positions;
+  float c[8], s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    c[j] = 1.0f;
+    s[j] = 0.0f;
+  }
+  if (turn) rot_row<CT, 8, true>(a.cos_sin, pos, kRopeDim, unit * 8, c, s);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (u >= heads) continue;
+    if (turn) turn_words<DT, INTERLEAVE>(x[u], y[u], c, s);
+    x[u].store(out + u * a.q_out_head + da);
+    y[u].store(out + u * a.q_out_head + db);
+  }
+}
+
+template <int DT, int CT, bool INTERLEAVE, int U>
+int launch_mla_prologue(MlaPrologueArgs a, hipStream_t stream) {
+  a.head_slots = (a.heads + U - 1) / U;
+  a.q_units = a.n_tokens * a.head_slots * (kRopeDim / 16);
+  const int64_t kv = (a.n_tokens + kRotThreads / kWave - 1) / (kRotThreads / kWave);
+  const int64_t groups = kv + (a.q_units + kRotThreads - 1) / kRotThreads;
+  if (groups > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
+  a.kv_blocks = static_cast<int>(kv);
+  mla_prologue_kernel<DT, CT, INTERLEAVE, U><<<dim3(static_cast<unsigned>(groups)), kRotThreads, 0, stream>>>(a);
+  return static_cast<int>(hipGetLastError());
+}
+
+template <int DT>
+int dispatch_mla_prologue(const MlaPrologueArgs& a, int interleave, int cos_sin_dtype, hipStream_t stream) {
+  const bool small = a.n_tokens * a.heads < 32768;   // one head per lane at decode sizes, four beyond
+#define XLLM_MLA_P(CT)                                                                                            \
+  (interleave != 0 ? (small ? launch_mla_prologue<DT, CT, true, 1>(a, stream) : launch_mla_prologue<DT, CT, true, 4>(a, stream)) \
+                   : (small ? launch_mla_prologue<DT, CT, false, 1>(a, stream) : launch_mla_prologue<DT, CT, false, 4>(a, stream)))
+  switch (cos_sin_dtype) {
+    case XLLM_MI355_FP32: return XLLM_MLA_P(XLLM_MI355_FP32);
+    case XLLM_MI355_BF16: return XLLM_MLA_P(XLLM_MI355_BF16);
+    case XLLM_MI355_FP16: return XLLM_MLA_P(XLLM_MI355_FP16);
+    default: return XLLM_MI355_EDTYPE;
+  }
+#undef XLLM_MLA_P
+}
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace
+
+int rope_cos_sin(const double* inv_freq, const int64_t* positions, int64_t first_position, int64_t n_rows, int64_t half,
+                 double factor, void* out, int out_dtype, hipStream_t stream) {
+  if (n_rows == 0) return XLLM_MI355_OK;
+  if (inv_freq == nullptr || out == nullptr || n_rows < 0 || half <= 0) return XLLM_MI355_EINVAL;
+  if (half > 4096 || n_rows > (1LL << 40)) return XLLM_MI355_ESHAPE;
+  switch (out_dtype) {
+    case XLLM_MI355_FP32: return launch_cos_sin<XLLM_MI355_FP32>(inv_freq, positions, first_position, n_rows, half, factor, out, stream);
+    case XLLM_MI355_BF16: return launch_cos_sin<XLLM_MI355_BF16>(inv_freq, positions, first_position, n_rows, half, factor, out, stream);
+    case XLLM_MI355_FP16: return launch_cos_sin<XLLM_MI355_FP16>(inv_freq, positions, first_position, n_rows, half, factor, out, stream);
+    default: return XLLM_MI355_EDTYPE;
+  }
+}
+
+int rotary_embedding(const int64_t* positions, const void* cos_sin, int64_t n_positions, const void* q, void* q_out,
+                     const void* k, void* k_out, int64_t n_tokens, int64_t n_heads_q, int64_t n_heads_k,
+                     int64_t head_dim_q, int64_t head_dim_k, int64_t rotary_offset_q, int64_t rotary_offset_k,
+                     int64_t rotary_dim, const int64_t* q_strides, const int64_t* q_out_strides,
+                     const int64_t* k_strides, const int64_t* k_out_strides, int interleave, int inverse, int dtype,
+                     int cos_sin_dtype, hipStream_t stream) {
+  if (n_tokens == 0) return XLLM_MI355_OK;
+  if (positions == nullptr || cos_sin == nullptr || q == nullptr || q_out == nullptr || q_strides == nullptr ||
+      q_out_strides == nullptr || n_tokens < 0 || n_positions <= 0 || n_heads_q <= 0 || n_heads_k < 0)
+    return XLLM_MI355_EINVAL;
+  if (n_heads_k > 0 && (k == nullptr || k_out == nullptr || k_strides == nullptr || k_out_strides == nullptr))
+    return XLLM_MI355_EINVAL;
+  if (dtype != XLLM_MI355_BF16 && dtype != XLLM_MI355_FP16 && dtype != XLLM_MI355_FP32) return XLLM_MI355_EDTYPE;
+  if (cos_sin_dtype != XLLM_MI355_BF16 && cos_sin_dtype != XLLM_MI355_FP16 && cos_sin_dtype != XLLM_MI355_FP32)
+    return XLLM_MI355_EDTYPE;
+  if (n_heads_q > 65535 || n_heads_k > 65535 || head_dim_q > 65536 || head_dim_k > 65536 || n_tokens > (1LL << 31))
+    return XLLM_MI355_ESHAPE;
+  if (rotary_dim <= 0 || rotary_dim % 2 != 0 || rotary_offset_q < 0 || rotary_offset_q + rotary_dim > head_dim_q)
+    return XLLM_MI355_ESHAPE;
+  if (n_heads_k > 0 && (rotary_offset_k < 0 || rotary_offset_k + rotary_dim > head_dim_k)) return XLLM_MI355_ESHAPE;
+  const int64_t es = dtype == XLLM_MI355_FP32 ? 4 : 2;
+  const int64_t word = 16 / es;   // elements of 16 bytes
+  const int64_t table_size = cos_sin_dtype == XLLM_MI355_FP32 ? 4 : 2;
+  RotArgs a = {};
+  auto side = [&](RotSide& s, const void* in, void* out, const int64_t* si, const int64_t* so, int64_t heads, int64_t dim,
+                  int64_t offset) {
+    s.in = static_cast<const char*>(in);
+    s.out = static_cast<char*>(out);
+    s.in_token = si[0];
+    s.in_head = si[1];
+    s.out_token = so[0];
+    s.out_head = so[1];
+    s.heads = static_cast<int>(heads);
+    s.dim = static_cast<int>(dim);
+    s.offset = static_cast<int>(offset);
+    if (si[0] < 0 || si[1] < 0 || so[0] < 0 || so[1] < 0) return false;
+    return in != out || (si[0] == so[0] && si[1] == so[1]);   // (in place the elements stay where they are)
+  };
+  bool copy_rest = false;
+  // 16 bytes per lane where every word of every head starts on one; element by element otherwise
+  bool vec = aligned(cos_sin, 16) && (rotary_dim / 2) % word == 0 && (rotary_dim / 2 * table_size) % 16 == 0;
+  auto add = [&](RotSide& s) {
+    vec = vec && aligned(s.in, 16) && aligned(s.out, 16) && s.in_token % word == 0 && s.in_head % word == 0 &&
+          s.out_token % word == 0 && s.out_head % word == 0 && s.offset % word == 0 && s.dim % word == 0;
+    copy_rest = copy_rest || (s.in != s.out && s.dim > rotary_dim);
+  };
+  if (!side(a.q, q, q_out, q_strides, q_out_strides, n_heads_q, head_dim_q, rotary_offset_q)) return XLLM_MI355_EINVAL;
+  add(a.q);
+  if (n_heads_k > 0) {
+    if (!side(a.k, k, k_out, k_strides, k_out_strides, n_heads_k, head_dim_k, rotary_offset_k)) return XLLM_MI355_EINVAL;
+    add(a.k);
+  }
+  a.positions = positions;
+  a.cos_sin = static_cast<const char*>(cos_sin);
+  a.n_positions = n_positions;
+  a.rot = static_cast<int>(rotary_dim);
+  switch (dtype) {
+    case XLLM_MI355_BF16: return dispatch_rotary<XLLM_MI355_BF16>(a, cos_sin_dtype, interleave, vec, copy_rest, inverse, n_tokens, stream);
+    case XLLM_MI355_FP16: return dispatch_rotary<XLLM_MI355_FP16>(a, cos_sin_dtype, interleave, vec, copy_rest, inverse, n_tokens, stream);
+    default: return dispatch_rotary<XLLM_MI355_FP32>(a, cos_sin_dtype, interleave, vec, copy_rest, inverse, n_tokens, stream);
+  }
+}
+
+int mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const void* kv, void* kv_out, const void* kv_weight, float eps,
+                            const void* cos_sin, int64_t n_positions, const int64_t* positions, void* k_cache,
+                            const int32_t* slots, int64_t n_tokens, int64_t n_heads, int64_t d_latent, int64_t d_rope,
+                            int64_t q_token_stride, int64_t q_head_stride, int64_t q_out_token_stride,
+                            int64_t q_out_head_stride, int64_t kv_row_stride, int64_t kv_out_row_stride,
+                            int64_t block_size, int64_t num_blocks, int interleave, int dtype, int cos_sin_dtype,
+                            hipStream_t stream) {
+  if (n_tokens == 0) return XLLM_MI355_OK;
+  if (q_pe == nullptr || q_pe_out == nullptr || kv == nullptr || kv_weight == nullptr || cos_sin == nullptr ||
+      positions == nullptr || n_tokens < 0 || n_heads <= 0 || n_positions <= 0 || !(eps >= 0.0f))
+    return XLLM_MI355_EINVAL;
+  if (k_cache == nullptr && kv_out == nullptr) return XLLM_MI355_EINVAL;
+  if (dtype != XLLM_MI355_BF16 && dtype != XLLM_MI355_FP16) return XLLM_MI355_EDTYPE;
+  if (d_latent != kLatent || d_rope != kRopeDim || n_heads > 65535 || n_tokens > (1LL << 31)) return XLLM_MI355_ESHAPE;
+  if (q_token_stride < 0 || q_head_stride < 0 || q_out_token_stride < 0 || q_out_head_stride < 0 ||
+      kv_row_stride < d_latent + d_rope || (kv_out != nullptr && kv_out_row_stride < d_latent + d_rope))
+    return XLLM_MI355_EINVAL;
+  if (k_cache != nullptr) {
+    if (slots == nullptr || block_size <= 0 || num_blocks <= 0) return XLLM_MI355_EINVAL;
+    if (block_size > 0x7fffffffLL || num_blocks > 0x7fffffffLL || block_size * num_blocks > 0x7fffffffLL)
+      return XLLM_MI355_ESHAPE;
+  }
+  if (!aligned(q_pe, 16) || !aligned(q_pe_out, 16) || !aligned(kv, 16) || !aligned(kv_out, 16) || !aligned(kv_weight, 16) ||
+      !aligned(cos_sin, 16) || !aligned(k_cache, 16) ||
+      ((q_token_stride | q_head_stride | q_out_token_stride | q_out_head_stride | kv_row_stride) & 7) != 0 ||
+      (kv_out != nullptr && (kv_out_row_stride & 7) != 0))
+    return XLLM_MI355_EALIGN;
+  MlaPrologueArgs a = {};
+  a.q = static_cast<const uint16_t*>(q_pe);
+  a.q_out = static_cast<uint16_t*>(q_pe_out);
+  a.kv = static_cast<const uint16_t*>(kv);
+  a.kv_out = static_cast<uint16_t*>(kv_out);
+  a.weight = static_cast<const uint16_t*>(kv_weight);
+  a.cos_sin = static_cast<const char*>(cos_sin);
+  a.positions = positions;
+  a.cache = static_cast<uint16_t*>(k_cache);
+  a.slots = slots;
+  a.n_tokens = n_tokens;
+  a.n_positions = n_positions;
+  a.n_slots = k_cache != nullptr ? block_size * num_blocks : 0;
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.q_out_token = q_out_token_stride;
+  a.q_out_head = q_out_head_stride;
+  a.kv_row = kv_row_stride;
+  a.kv_out_row = kv_out_row_stride;
+  a.heads = static_cast<int>(n_heads);
+  a.eps = eps;
+  return dtype == XLLM_MI355_BF16 ? dispatch_mla_prologue<XLLM_MI355_BF16>(a, interleave, cos_sin_dtype, stream)
+                                  : dispatch_mla_prologue<XLLM_MI355_FP16>(a, interleave, cos_sin_dtype, stream);
+}
+
+}  // namespace xllm_mi355

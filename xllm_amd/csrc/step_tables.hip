@@ -1,0 +1,295 @@
+// The tables of a step -- block table, positions, slots, lengths -- from the requests' lengths, on the GPU.
+//
+// B requests hold kv[b] tokens in the cache and want new[b] more; the step has room for T new tokens and the free list
+// holds page ids from entry `head` on.  With C = ceil(x / block_size):
+//   cu[b + 1]     = min(new[0] + .. + new[b], T)                    the step's tokens, request after request
+//   acc[b]        = cu[b + 1] - cu[b]                               (requests behind the budget wait)
+//   old[b]        = min(C(kv[b]), W),  need[b] = min(C(kv[b] + acc[b]), W) - old[b]        W: width of the table
+//   indptr[b + 1] = min(need[0] + .. + need[b], n_free - head)      pages taken, in the order of the free list
+//   table[b, j]   = the old entry for j < old[b], free[head + indptr[b] + j - old[b]] for the pages taken, -1 behind them
+//   token i of b  : position kv[b] + i - cu[b], slot table[b, position / bs] * bs + position % bs (-1 where no page was left)
+//   rows behind the last token: position 0, slot -1
+// Everything is integer arithmetic: the result does not depend on the order in which the lanes work.
+//
+// The two sums saturate at T and at the pages left (min(x + y, cap) is associative for x, y >= 0), so 32 bits hold them
+// whatever the lengths.  Up to kFusedBatch requests are one launch: every workgroup makes both sums for itself in LDS
+// (they come from L2 after the first) and takes its share of the tokens and of the table; a token finds its request by
+// bisection in LDS.  Beyond that a first launch of one workgroup makes the sums and the second reads them from memory.
+#include "common.cuh"
+#include "launch.h"
+
+namespace xllm_mi355 {
+
+namespace {
+
+constexpr int kStepThreads = 256;
+constexpr int kStepWaves = kStepThreads / kWave;
+constexpr int kFusedBatch = 4096;        // 2 sums of up to 16 KB in LDS
+constexpr int kStepCells = 1024;         // tokens, or table entries, of a workgroup
+
+struct StepArgs {
+  const int32_t* kv_lens;
+  const int32_t* new_lens;
+  const int32_t* table_in;
+  int32_t* table_out;
+  const int32_t* free_pages;
+  const int32_t* free_head;   // or null: 0
+  int32_t* seq_lens;
+  int32_t* cu;
+  int64_t* positions;
+  int32_t* slots;
+  int32_t* indptr;
+  int32_t* counters;
+  int64_t in_stride, out_stride;
+  int batch, width, block_size, bs_shift, budget, n_free;
+  int token_blocks;           // workgroups of the tokens, the first ones of the grid
+  int col_blocks;             // workgroups per table row
+  int rows_per_block;         // table rows of a workgroup when they are short
+};
+
+// Column of a position, and min(C(tokens), W).  (32-bit division: a context and the tokens of a step are below 2^32.)
+__device__ __forceinline__ u32 step_column(const StepArgs& a, u32 pos) {
+  return a.bs_shift >= 0 ? pos >> a.bs_shift : pos / static_cast<u32>(a.block_size);
+}
+__device__ __forceinline__ int step_pages(const StepArgs& a, u32 tokens) {
+  const u32 full = step_column(a, tokens);
+  const u32 n = full + (full * static_cast<u32>(a.block_size) != tokens ? 1u : 0u);
+  return static_cast<int>(min(n, static_cast<u32>(a.width)));
+}
+__device__ __forceinline__ int step_head(const StepArgs& a) {
+  return a.free_head != nullptr ? max(0, min(a.free_head[0], a.n_free)) : 0;
+}
+__device__ __forceinline__ int step_kv(const StepArgs& a, int b) { return max(0, a.kv_lens[b]); }
+__device__ __forceinline__ int step_new(const StepArgs& a, int b) { return max(0, min(a.new_lens[b], a.budget)); }
+
+// Saturating exclusive scan of one value per thread; `all` is the sum over the workgroup.  tmp: one word per wavefront.
+template <int WAVES>
+__device__ __forceinline__ int saturating_scan(int v, int cap, int& all, int* tmp) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int t = __shfl_up(v, d, kWave);
+    if (lane >= d) v = min(v + t, cap);
+  }
+  int excl = __shfl_up(v, 1, kWave);
+  if (lane == 0) excl = 0;
+  __syncthreads();   // (tmp may still be read from the scan before)
+  if (lane == kWave - 1) tmp[wave] = v;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const int t = tmp[w];
+    if (w < wave) excl = min(excl + t, cap);
+    all = min(all + t, cap);
+  }
+  return excl;
+}
+
+// Both sums over the batch into cu[0 .. batch] and indptr[0 .. batch] (LDS or global memory).  A thread takes a run of
+// requests, so that there are two scans whatever the batch.
+template <int WAVES>
+__device__ __forceinline__ void step_sums(const StepArgs& a, int32_t* cu, int32_t* indptr, int* tmp) {
+  const int tid = threadIdx.x;
+  const int per = (a.batch + WAVES * kWave - 1) / (WAVES * kWave);
+  const int lo = min(a.batch, tid * per), hi = min(a.batch, lo + per);
+  const int pages_left = a.n_free - step_head(a);
+  int all;
+  int sum = 0;
+  for (int b = lo; b < hi; ++b) sum = min(sum + step_new(a, b), a.budget);
+  int c = saturating_scan<WAVES>(sum, a.budget, all, tmp);
+  if (tid == 0) {
+    cu[0] = 0;
+    indptr[0] = 0;
+  }
+  const int c0 = c;
+  sum = 0;
+  for (int b = lo; b < hi; ++b) {
+    const int e = min(c + step_new(a, b), a.budget);
+    const u32 kv = step_kv(a, b);
+    sum = min(sum + (step_pages(a, kv + (e - c)) - step_pages(a, kv)), pages_left);
+    cu[b + 1] = e;
+    c = e;
+  }
+  int p = saturating_scan<WAVES>(sum, pages_left, all, tmp);
+  c = c0;
+  for (int b = lo; b < hi; ++b) {
+    const int e = min(c + step_new(a, b), a.budget);
+    const u32 kv = step_kv(a, b);
+    p = min(p + (step_pages(a, kv + (e - c)) - step_pages(a, kv)), pages_left);
+    indptr[b + 1] = p;
+    c = e;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ int request_of(const int32_t* cu, int batch, int token) {   // cu[b] <= token < cu[b + 1]
+  int lo = 0, hi = batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (cu[mid + 1] > token) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+// Entry j of request b's row; what lies behind its pages is -1.
+__device__ __forceinline__ int step_entry(const StepArgs& a, const int32_t* cu, const int32_t* indptr, int b, int j, int old,
+                                          int head) {
+  if (j < old) return a.table_in[b * a.in_stride + j];
+  const int p = indptr[b] + (j - old);
+  return p < indptr[b + 1] ? a.free_pages[head + p] : -1;
+}
+
+// What the first workgroup adds: lengths, sums and counters in the caller's arrays.
+template <int THREADS>
+__device__ __forceinline__ void step_outputs(const StepArgs& a, const int32_t* cu, const int32_t* indptr, bool copy, int* tmp) {
+  const int head = step_head(a);
+  int lost = 0;   // tokens that no page was left for: those from the end of the request's pages on
+  for (int b = threadIdx.x; b < a.batch; b += THREADS) {
+    const int64_t kv = step_kv(a, b), total = kv + (cu[b + 1] - cu[b]);
+    // (pages that cover the context and the pages taken)
+    a.seq_lens[b] = static_cast<int>(total < 0x7fffffffLL ? total : 0x7fffffffLL);
+    const int64_t held = static_cast<int64_t>(step_pages(a, static_cast<u32>(kv)) + (indptr[b + 1] - indptr[b])) * a.block_size;
+    const int64_t from = held > kv ? held : kv;
+    lost += static_cast<int>(total > from ? total - from : 0);
+  }
+  if (copy)
+    for (int b = threadIdx.x; b <= a.batch; b += THREADS) {
+      a.cu[b] = cu[b];
+      a.indptr[b] = indptr[b];
+    }
+  int sum;
+  saturating_scan<THREADS / kWave>(lost, a.budget, sum, tmp);   // (at most the tokens of the step)
+  if (threadIdx.x == 0) {
+    a.counters[0] = cu[a.batch];
+    a.counters[1] = head + indptr[a.batch];
+    a.counters[2] = sum;
+  }
+}
+
+__global__ __launch_bounds__(1024) void step_sums_kernel(StepArgs a) {
+  __shared__ int tmp[16];
+  step_sums<16>(a, a.cu, a.indptr, tmp);
+  __threadfence_block();
+  __syncthreads();
+  step_outputs<1024>(a, a.cu, a.indptr, false, tmp);
+}
+
+template <bool FUSED>
+__global__ __launch_bounds__(kStepThreads) void step_tables_kernel(StepArgs a) {
+  extern __shared__ int32_t lds[];
+  __shared__ int tmp[kStepWaves];
+  const int32_t *cu = a.cu, *indptr = a.indptr;
+  if constexpr (FUSED) {
+    int32_t* c = lds;
+    int32_t* p = lds + a.batch + 1;
+    step_sums<kStepWaves>(a, c, p, tmp);
+    cu = c;
+    indptr = p;
+    if (blockIdx.x == 0) step_outputs<kStepThreads>(a, c, p, true, tmp);
+  }
+  const int tid = threadIdx.x;
+  const int head = step_head(a);
+  if (static_cast<int>(blockIdx.x) < a.token_blocks) {
+    const int n_tokens = cu[a.batch];
+#pragma unroll
+    for (int k = 0; k < kStepCells / kStepThreads; ++k) {
+      const int i = static_cast<int>(blockIdx.x) * kStepCells + k * kStepThreads + tid;
+      if (i >= a.budget) continue;
+      int64_t pos = 0;
+      int slot = -1;
+      if (i < n_tokens) {
+        const int b = request_of(cu, a.batch, i);
+        const u32 kv = step_kv(a, b);
+        pos = kv + static_cast<u32>(i - cu[b]);
+        const u32 col = step_column(a, static_cast<u32>(pos));
+        if (col < static_cast<u32>(a.width)) {
+          const int64_t page = step_entry(a, cu, indptr, b, static_cast<int>(col), step_pages(a, kv), head);
+          const int64_t s = page * a.block_size + (pos - static_cast<int64_t>(col) * a.block_size);
+          if (page >= 0 && s <= 0x7fffffffLL) slot = static_cast<int>(s);
+        }
+      }
+      a.positions[i] = pos;
+      a.slots[i] = slot;
+    }
+    return;
+  }
+  // a piece of the table: part of a long row, or several short rows
+  const bool in_place = a.table_in == a.table_out;
+  const int t = static_cast<int>(blockIdx.x) - a.token_blocks;
+  const int b0 = t / a.col_blocks * a.rows_per_block;
+  const int c0 = t % a.col_blocks * kStepCells;
+  const int rows = min(a.rows_per_block, a.batch - b0);
+  const int cols = min(a.width - c0, kStepCells);
+  for (int i = tid; i < rows * cols; i += kStepThreads) {
+    const int r = i / cols;
+    const int b = b0 + r, j = c0 + i - r * cols;
+    const int old = step_pages(a, step_kv(a, b));
+    if (in_place && j < old) continue;
+    a.table_out[b * a.out_stride + j] = step_entry(a, cu, indptr, b, j, old, head);
+  }
+}
+
+}  // namespace
+
+int build_step_tables(const int32_t* kv_lens, const int32_t* new_lens, const int32_t* block_table_in,
+                      int64_t in_stride, int32_t* block_table_out, int64_t out_stride, int64_t table_width,
+                      const int32_t* free_pages, int64_t n_free, const int32_t* free_head, int32_t* seq_lens,
+                      int32_t* cu_new, int64_t* positions, int32_t* slots, int32_t* new_page_indptr,
+                      int32_t* counters, int64_t batch, int64_t block_size, int64_t max_new_tokens,
+                      hipStream_t stream) {
+  if (batch == 0) return XLLM_MI355_OK;
+  if (kv_lens == nullptr || new_lens == nullptr || block_table_in == nullptr || block_table_out == nullptr ||
+      (free_pages == nullptr && n_free != 0) || seq_lens == nullptr || cu_new == nullptr || new_page_indptr == nullptr ||
+      counters == nullptr || (max_new_tokens > 0 && (positions == nullptr || slots == nullptr)))
+    return XLLM_MI355_EINVAL;
+  if (batch < 0 || block_size <= 0 || table_width <= 0 || n_free < 0 || max_new_tokens < 0 || in_stride < table_width ||
+      out_stride < table_width)
+    return XLLM_MI355_EINVAL;
+  // (in place the rows must lie at the same addresses)
+  if (block_table_in == block_table_out && in_stride != out_stride) return XLLM_MI355_EINVAL;
+  constexpr int64_t kLimit = (1LL << 30) - 1;   // the sum of two stays inside 32 bits
+  if (max_new_tokens > kLimit || n_free > kLimit || table_width > kLimit || block_size > kLimit || batch > (1LL << 20))
+    return XLLM_MI355_ESHAPE;
+  StepArgs a = {};
+  a.kv_lens = kv_lens;
+  a.new_lens = new_lens;
+  a.table_in = block_table_in;
+  a.table_out = block_table_out;
+  a.free_pages = free_pages;
+  a.free_head = free_head;
+  a.seq_lens = seq_lens;
+  a.cu = cu_new;
+  a.positions = positions;
+  a.slots = slots;
+  a.indptr = new_page_indptr;
+  a.counters = counters;
+  a.in_stride = in_stride;
+  a.out_stride = out_stride;
+  a.batch = static_cast<int>(batch);
+  a.width = static_cast<int>(table_width);
+  a.block_size = static_cast<int>(block_size);
+  a.bs_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if ((1LL << s) == block_size) a.bs_shift = s;
+  a.budget = static_cast<int>(max_new_tokens);
+  a.n_free = static_cast<int>(n_free);
+  a.token_blocks = static_cast<int>((max_new_tokens + kStepCells - 1) / kStepCells);
+  a.col_blocks = static_cast<int>((table_width + kStepCells - 1) / kStepCells);
+  a.rows_per_block = table_width >= kStepCells ? 1 : static_cast<int>(kStepCells / table_width);
+  const int64_t table_blocks = (batch + a.rows_per_block - 1) / a.rows_per_block * a.col_blocks;
+  if (a.token_blocks + table_blocks > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
+  const dim3 grid(static_cast<unsigned>(a.token_blocks + table_blocks));
+  if (batch <= kFusedBatch) {
+    step_tables_kernel<true><<<grid, kStepThreads, (2 * batch + 2) * 4, stream>>>(a);
+    return static_cast<int>(hipGetLastError());
+  }
+  step_sums_kernel<<<1, 1024, 0, stream>>>(a);
+  const int rc = static_cast<int>(hipGetLastError());
+  if (rc != 0) return rc;
+  step_tables_kernel<false><<<grid, kStepThreads, 0, stream>>>(a);
+  return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace xllm_mi355

@@ -17,9 +17,18 @@ Reference interface mirrored here (paths relative to the xLLM source tree):
   gather_mla_latent_cache                         xllm/core/kernels/dcu/dcu_ops_api.h:74
   absorbed MLA products (bmm with w_kc_ / w_vc_)  xllm/core/layers/dcu/deepseek_v2_attention.cpp:231-238,428-430
   FlashAttentionImpl::paged_forward (q chunks)    xllm/core/layers/dcu/flash_attention.cpp:447-545
+Operators around the path that the reference does on the host, in its layers or not at all:
+  build_step_tables                               xllm/core/framework/batch/batch_input_builder.cpp (host)
+  rope_frequencies, build_cos_sin_cache, rotary_embedding
+                                                  xllm/core/layers/common/rotary_embedding*
+  mla_norm_rope_and_cache                         xllm/core/layers/dcu/deepseek_v2_attention.cpp:221-229 and the lines before
+  batch_decode_diff                               (no counterpart: the difference of two softmax maps)
 
 Errors: the reference CHECK-aborts; here every violated precondition raises.
 """
+import contextlib
+import ctypes
+import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -800,3 +809,440 @@ def absorbed_bmm(x, w, out=None):
         out.stride(1), _dtype_code(x), _stream(dev))
     capi.check(rc, "xllm_mi355_mla_absorbed_bmm")
     return out
+
+
+# ------------------------------------------------------------------------------------------
+# the tables of a step
+
+def _on_device(dev):
+    """Launches go to the tensors' device, whatever the current one is."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _byte_range(t):
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a, b):
+    if a is None or b is None or a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _byte_range(a), _byte_range(b)
+    return a0 < b1 and b0 < a1
+
+
+@dataclass
+class StepTables:
+    """What a step's calls read: block_table [B, W] and seq_lens [B] (batch_decode, paged_forward, dense_decode),
+    q_cu_seq_lens [B + 1] (paged_forward), position_ids [T] int64 and slot_mapping [T] int32 (rotary and cache writes), all
+    int32 but the positions.  new_page_indptr [B + 1]: offsets of the pages that the requests took, relative to the free
+    head.  counters [3]: tokens of the step, the free head of the next step, tokens that found no page."""
+    block_table: torch.Tensor
+    seq_lens: torch.Tensor
+    q_cu_seq_lens: torch.Tensor
+    position_ids: torch.Tensor
+    slot_mapping: torch.Tensor
+    new_page_indptr: torch.Tensor
+    counters: torch.Tensor
+
+
+_I32_FIELDS = ("block_table", "seq_lens", "q_cu_seq_lens", "slot_mapping", "new_page_indptr", "counters")
+
+
+def build_step_tables(kv_lens, new_lens, block_table, free_pages, block_size, max_new_tokens, free_head=None, out=None):
+    """The tables of a step on the GPU, from the requests' lengths: no host loop, no copy, capturable.
+    kv_lens [B] int32: tokens in the cache; new_lens [B] int32: tokens this step brings (1 for a decode, a chunk for a
+    prefill, 0 for an idle row); block_table [B, W] int32, whose first ceil(kv_lens / block_size) entries of a row are kept;
+    free_pages [F] int32: pages to take, in order, from entry free_head ([1] int32, None: 0) on.  max_new_tokens: the
+    step's token budget T, the size of position_ids and slot_mapping; requests behind it get fewer tokens or none.
+    Rows of position_ids / slot_mapping behind the last token hold 0 / -1; table entries behind a request's pages hold -1.
+    Where the free list or the table's width runs out, slots are -1 and counters[2] says how many: such a request must not
+    attend before its tokens are stored.
+    out: StepTables to write into (the persistent buffers of a captured step); its block_table may be block_table itself.
+    Returns StepTables."""
+    dev = _require_cuda(kv_lens, new_lens, block_table, free_pages, free_head)
+    for name, t in (("kv_lens", kv_lens), ("new_lens", new_lens), ("free_pages", free_pages)):
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 vector")
+    B, F, T, block_size = kv_lens.numel(), free_pages.numel(), int(max_new_tokens), int(block_size)
+    if new_lens.numel() != B:
+        raise ValueError("kv_lens and new_lens must have one entry per request")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or \
+            block_table.shape[0] != B or block_table.shape[1] == 0:
+        raise ValueError("block_table must be int32 [B, W] with unit column stride, one row per request")
+    if free_head is not None and (free_head.dtype != torch.int32 or free_head.numel() != 1):
+        raise ValueError("free_head must be int32 [1]")
+    if block_size <= 0 or T < 0:
+        raise ValueError("block_size must be positive and max_new_tokens not negative")
+    W = block_table.shape[1]
+    if B > 1 and block_table.stride(0) < W:
+        raise ValueError("block_table: rows must not overlap")
+    if out is None:
+        seq_lens, cu, indptr, counters, slots = torch.empty(
+            3 * B + 5 + T, dtype=torch.int32, device=dev).split([B, B + 1, B + 1, 3, T])
+        out = StepTables(torch.empty(B, W, dtype=torch.int32, device=dev), seq_lens, cu,
+                         torch.empty(T, dtype=torch.int64, device=dev), slots, indptr, counters)
+    else:
+        fields = [getattr(out, f) for f in _I32_FIELDS]
+        _require_cuda(kv_lens, out.position_ids, *fields)
+        sizes = dict(seq_lens=B, q_cu_seq_lens=B + 1, slot_mapping=T, new_page_indptr=B + 1, counters=3)
+        for f, t in zip(_I32_FIELDS, fields):
+            if t.dtype != torch.int32 or (f in sizes and (tuple(t.shape) != (sizes[f],) or not t.is_contiguous())):
+                raise ValueError(f"out.{f} must be contiguous int32 of its documented size")
+        if out.position_ids.dtype != torch.int64 or tuple(out.position_ids.shape) != (T,) or \
+                not out.position_ids.is_contiguous():
+            raise ValueError("out.position_ids must be contiguous int64 [max_new_tokens]")
+        tab = out.block_table
+        if tuple(tab.shape) != (B, W) or tab.stride(1) != 1 or (B > 1 and tab.stride(0) < W):
+            raise ValueError("out.block_table must be [B, W] with unit column stride")
+        same = tab.data_ptr() == block_table.data_ptr() and (B <= 1 or tab.stride(0) == block_table.stride(0))
+        written = fields + [out.position_ids]
+        for i, t in enumerate(written):
+            if any(_overlap(t, x) for x in (kv_lens, new_lens, free_pages, free_head)) or \
+                    (_overlap(t, block_table) and not (i == 0 and same)):
+                raise ValueError("an output of build_step_tables overlaps one of its inputs")
+            if any(_overlap(t, x) for x in written[:i]):
+                raise ValueError("two outputs of build_step_tables overlap")
+    if B == 0:
+        for t in (out.q_cu_seq_lens, out.new_page_indptr, out.counters, out.position_ids):
+            t.zero_()
+        if free_head is not None:
+            out.counters[1:2].copy_(free_head.view(1).clamp(0, F))
+        out.slot_mapping.fill_(-1)
+        return out
+    with _on_device(dev):
+        rc = capi.lib().xllm_mi355_build_step_tables(
+            kv_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), max(W, block_table.stride(0)),
+            out.block_table.data_ptr(), max(W, out.block_table.stride(0)), W, free_pages.data_ptr() if F else None, F,
+            _ptr(free_head), out.seq_lens.data_ptr(), out.q_cu_seq_lens.data_ptr(), _ptr(out.position_ids) or None,
+            _ptr(out.slot_mapping) or None, out.new_page_indptr.data_ptr(), out.counters.data_ptr(), B, block_size, T,
+            _stream(dev))
+    capi.check(rc, "xllm_mi355_build_step_tables")
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# rotary positions
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """How rotary frequencies are stretched for contexts beyond the trained length (the rope_scaling of a model's
+    configuration).
+      "linear"   every frequency divided by factor
+      "dynamic"  the base raised with the length, for lengths beyond original_max_position (pass seq_len)
+      "llama3"   frequencies that turn fewer than low_freq_factor times in original_max_position tokens divided by factor,
+                 those that turn more than high_freq_factor times kept, a straight line between
+      "yarn"     the same idea by dimension, between the dims that turn beta_fast and beta_slow times; cos and sin are also
+                 scaled: by attention_factor if given, else by m(mscale) / m(mscale_all_dim) with m(x) = 0.1 x ln(factor) + 1,
+                 where an mscale_all_dim of 0 makes the divisor 1"""
+    kind: str
+    factor: float = 1.0
+    original_max_position: int = 0
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    mscale: float = 1.0
+    mscale_all_dim: float = 0.0
+    attention_factor: Optional[float] = None
+
+
+def rope_frequencies(rotary_dim, base=10000.0, scaling=None, seq_len=0, device="cuda"):
+    """(inv_freq, attention_factor) of a rotary embedding: inv_freq [rotary_dim / 2] float64 on the device, made once per
+    model (with "dynamic" scaling: once per length) and handed to build_cos_sin_cache with the factor."""
+    if rotary_dim <= 0 or rotary_dim % 2 != 0:
+        raise ValueError("rotary_dim must be even and positive")
+    if not base > 0:
+        raise ValueError("base must be positive")
+    half = rotary_dim // 2
+    s, factor = scaling, 1.0
+    if s is not None:
+        if s.kind not in ("linear", "dynamic", "llama3", "yarn"):
+            raise ValueError(f"unknown rope scaling {s.kind!r}")
+        if not s.factor >= 1.0:
+            raise ValueError("the scaling factor must be at least 1")
+        if s.kind != "linear" and s.original_max_position <= 0:
+            raise ValueError(f"{s.kind} scaling needs original_max_position")
+    if s is not None and s.kind == "dynamic" and seq_len > s.original_max_position and rotary_dim > 2:
+        base = base * (s.factor * seq_len / s.original_max_position - (s.factor - 1)) ** (rotary_dim / (rotary_dim - 2))
+    inv = [base ** (-2.0 * i / rotary_dim) for i in range(half)]
+    if s is not None and s.kind == "linear":
+        inv = [f / s.factor for f in inv]
+    elif s is not None and s.kind == "llama3":
+        if not s.high_freq_factor > s.low_freq_factor:
+            raise ValueError("llama3 scaling needs high_freq_factor > low_freq_factor")
+        for i, f in enumerate(inv):
+            turns = s.original_max_position * f / (2 * math.pi)
+            keep = min(1.0, max(0.0, (turns - s.low_freq_factor) / (s.high_freq_factor - s.low_freq_factor)))
+            inv[i] = keep * f + (1 - keep) * f / s.factor
+    elif s is not None and s.kind == "yarn":
+        if not base > 1 or not s.beta_fast > 0 or not s.beta_slow > 0:
+            raise ValueError("yarn scaling needs base > 1 and positive beta_fast and beta_slow")
+
+        def dim_that_turns(times):
+            return rotary_dim * math.log(s.original_max_position / (times * 2 * math.pi)) / (2 * math.log(base))
+
+        low = max(math.floor(dim_that_turns(s.beta_fast)), 0)
+        high = min(math.ceil(dim_that_turns(s.beta_slow)), rotary_dim - 1)
+        for i, f in enumerate(inv):
+            stretch = min(1.0, max(0.0, (i - low) / max(high - low, 0.001)))
+            inv[i] = f * (1 - stretch) + f / s.factor * stretch
+
+        def magnitude(x):
+            return 0.1 * x * math.log(s.factor) + 1.0
+
+        factor = s.attention_factor if s.attention_factor is not None else \
+            magnitude(s.mscale) / (magnitude(s.mscale_all_dim) if s.mscale_all_dim else 1.0)
+    return torch.tensor(inv, dtype=torch.float64, device=device), float(factor)
+
+
+def build_cos_sin_cache(inv_freq, num_positions=0, position_ids=None, first_position=0, attention_factor=1.0,
+                        dtype=torch.float32, out=None):
+    """cos | sin rows [rows, rotary_dim] for fused_qk_norm_rope, rotary_embedding and mla_norm_rope_and_cache, angles in 64
+    bits, rounded once to dtype (float32, bfloat16 or float16).  Rows of position_ids [rows] int64 -- one step's rows,
+    shared by all layers, which then index them by 0 .. rows - 1 -- or of first_position .. first_position + num_positions - 1.
+    inv_freq, attention_factor: from rope_frequencies.  Returns the rows (out, if given)."""
+    dev = _require_cuda(inv_freq, position_ids, out)
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.numel() == 0:
+        raise ValueError("inv_freq must be a contiguous float64 vector (rope_frequencies)")
+    if position_ids is not None:
+        if position_ids.dtype != torch.int64 or position_ids.dim() != 1 or not position_ids.is_contiguous():
+            raise ValueError("position_ids must be a contiguous int64 vector")
+        if first_position != 0 or num_positions not in (0, position_ids.numel()):
+            raise ValueError("give position_ids or a range of positions, not both")
+        rows = position_ids.numel()
+    else:
+        rows = int(num_positions)
+        if rows <= 0 or first_position < 0:
+            raise ValueError("num_positions must be positive and first_position not negative")
+    shape = (rows, 2 * inv_freq.numel())
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=dev)
+    elif tuple(out.shape) != shape or not out.is_contiguous():
+        raise ValueError("out must be contiguous [rows, rotary_dim]")
+    elif _overlap(out, inv_freq) or _overlap(out, position_ids):
+        raise ValueError("out overlaps an input")
+    if out.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError("cos_sin rows are float32, bfloat16 or float16")
+    if rows == 0:
+        return out
+    with _on_device(dev):
+        rc = capi.lib().xllm_mi355_rope_cos_sin(
+            inv_freq.data_ptr(), _ptr(position_ids), int(first_position), rows, inv_freq.numel(), float(attention_factor),
+            out.data_ptr(), _dtype_code(out), _stream(dev))
+    capi.check(rc, "xllm_mi355_rope_cos_sin")
+    return out
+
+
+_Strides = ctypes.c_int64 * 2
+
+
+def _check_cos_sin(cos_sin_cache, position_ids, n_tokens):
+    if position_ids.dtype != torch.int64 or not position_ids.is_contiguous() or position_ids.numel() != n_tokens:
+        raise ValueError("position_ids must be a contiguous int64 tensor [tokens]")
+    if cos_sin_cache.dim() != 2 or not cos_sin_cache.is_contiguous() or cos_sin_cache.shape[0] == 0:
+        raise ValueError("cos_sin_cache must be [max_position, rotary_dim], contiguous")
+    if cos_sin_cache.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError("cos_sin_cache must be float32, bfloat16 or float16")
+
+
+def _head_strides(x):
+    """(token, head) strides; 0 where there is only one of them (its stride then means nothing)."""
+    return x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0
+
+
+def _check_rotated(name, x, out, inputs):
+    """x [T, H, D] and where its result goes: x itself, or a tensor apart from every input."""
+    if x.dim() != 3 or x.shape[1] == 0 or (x.numel() > 0 and x.stride(2) != 1):
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], contiguous in its last dim")
+    if out is not x:
+        if out.shape != x.shape or out.dtype != x.dtype or (x.numel() > 0 and out.stride(2) != 1):
+            raise ValueError(f"out_{name} must have {name}'s shape and dtype, contiguous in its last dim")
+        same = out.data_ptr() == x.data_ptr() and _head_strides(out) == _head_strides(x)
+        if any(_overlap(out, t) for t in inputs if not (same and t is x)):
+            raise ValueError(f"out_{name} overlaps an input (in place means {name} itself)")
+    (ts, hs), (T, H, D) = _head_strides(out), out.shape
+    # every element written once: heads inside tokens or tokens inside heads
+    if not ((H == 1 or hs >= D) and (T <= 1 or ts >= (H - 1) * hs + D)) and \
+            not ((T <= 1 or ts >= D) and (H == 1 or hs >= (T - 1) * ts + D)):
+        raise ValueError(f"{name}: the heads of the result overlap each other")
+
+
+def rotary_embedding(position_ids, query, key, cos_sin_cache, interleave=False, rotary_offset=0, key_rotary_offset=None,
+                     inverse=False, out_query=None, out_key=None):
+    """Rotary embedding of q and k in tensors of their own (fused_qk_norm_rope is the one for a fused qkv buffer).
+    query [T, Hq, D], key [T, Hk, D'] or None, in bfloat16, float16 or float32, any token and head strides;
+    cos_sin_cache [max_position, rotary_dim] (build_cos_sin_cache); position_ids [T] int64: a position outside the cache is
+    not rotated.  rotary_offset: where the rotated part of a head begins (key_rotary_offset: of a key head, if elsewhere).
+    interleave: pairs (2i, 2i + 1), else (i, i + rotary_dim / 2).  inverse: the transposed map, which undoes a rotation by
+    unscaled rows and turns the gradient of the result into the gradient of the input.
+    Works in place, or into out_query / out_key.  Returns (query's result, key's result or None)."""
+    dev = _require_cuda(position_ids, query, key, cos_sin_cache, out_query, out_key)
+    oq = query if out_query is None else out_query
+    ok = key if out_key is None else out_key
+    if key is None and out_key is not None:
+        raise ValueError("out_key without a key")
+    if query.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError("query must be bfloat16, float16 or float32")
+    inputs = [t for t in (query, key, cos_sin_cache, position_ids) if t is not None]
+    _check_rotated("query", query, oq, inputs)
+    T, Hq, D = query.shape
+    _check_cos_sin(cos_sin_cache, position_ids, T)
+    R = cos_sin_cache.shape[1]
+    Hk = Dk = 0
+    if key is not None:
+        _check_rotated("key", key, ok, inputs)
+        if key.shape[0] != T or key.dtype != query.dtype:
+            raise ValueError("key must have query's tokens and dtype")
+        if oq.data_ptr() == ok.data_ptr() and T > 0:
+            raise ValueError("the results of query and key overlap")
+        Hk, Dk = key.shape[1], key.shape[2]
+    k_off = rotary_offset if key_rotary_offset is None else key_rotary_offset
+    if R % 2 != 0 or R == 0:
+        raise ValueError("the rotary dim must be even")
+    if rotary_offset < 0 or rotary_offset + R > D or (key is not None and (k_off < 0 or k_off + R > Dk)):
+        raise ValueError("the rotated part must lie inside the head")
+    if T == 0:
+        return oq, ok
+    with _on_device(dev):
+        rc = capi.lib().xllm_mi355_rotary_embedding(
+            position_ids.data_ptr(), cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], query.data_ptr(), oq.data_ptr(),
+            _ptr(key), _ptr(ok), T, Hq, Hk, D, Dk, rotary_offset, k_off if Hk else 0, R, _Strides(*_head_strides(query)),
+            _Strides(*_head_strides(oq)), _Strides(*_head_strides(key)) if Hk else None,
+            _Strides(*_head_strides(ok)) if Hk else None, 1 if interleave else 0, 1 if inverse else 0, _dtype_code(query),
+            _dtype_code(cos_sin_cache), _stream(dev))
+    capi.check(rc, "xllm_mi355_rotary_embedding")
+    return oq, ok
+
+
+def mla_norm_rope_and_cache(q_pe, kv, kv_norm_weight, eps, cos_sin_cache, interleave, position_ids, k_cache=None,
+                            slot_mapping=None, out_q_pe=None, out_kv=None):
+    """The MLA prologue in one launch (what fused_qk_norm_rope is for GQA): the latent kv[:, :512] is RMS normalised with
+    kv_norm_weight [512], the rope key kv[:, 512:] and the queries' rope part q_pe [T, H, 64] (a slice of the queries) are
+    rotated by the cos | sin row of their position, and the rows go to k_cache [P, bs, 1, 576] at slot_mapping [T] int32
+    (negative slots and slots beyond the cache are skipped) and / or to out_kv [T, 576] (kv itself: in place).
+    out_q_pe [T, H, 64]: contiguous is what dense_decode reads; None: in place.  bfloat16 or float16.
+    Returns (q_pe's result, out_kv)."""
+    dev = _require_cuda(q_pe, kv, kv_norm_weight, cos_sin_cache, position_ids, k_cache, slot_mapping, out_q_pe, out_kv)
+    oq = q_pe if out_q_pe is None else out_q_pe
+    if q_pe.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("q_pe must be bfloat16 or float16")
+    inputs = (q_pe, kv, kv_norm_weight, cos_sin_cache, position_ids, slot_mapping)
+    _check_rotated("q_pe", q_pe, oq, [t for t in inputs if t is not None])
+    T, H, d_rope = q_pe.shape
+    d_latent = kv_norm_weight.numel()
+    if kv.dim() != 2 or kv.shape[0] != T or kv.shape[1] != d_latent + d_rope or (T > 0 and kv.stride(1) != 1):
+        raise ValueError("kv must be [tokens, latent + rope dims] with contiguous rows")
+    if not (kv.dtype == kv_norm_weight.dtype == q_pe.dtype) or not kv_norm_weight.is_contiguous():
+        raise TypeError("kv and kv_norm_weight must have q_pe's dtype, the weight contiguous")
+    _check_cos_sin(cos_sin_cache, position_ids, T)
+    if cos_sin_cache.shape[1] != d_rope:
+        raise ValueError("cos_sin_cache must have the rope dims")
+    if (k_cache is None) != (slot_mapping is None):
+        raise ValueError("k_cache and slot_mapping come together")
+    if k_cache is None and out_kv is None:
+        raise ValueError("the latent rows need a place: k_cache or out_kv")
+    if out_kv is not None:
+        if out_kv.shape != kv.shape or out_kv.dtype != kv.dtype or (T > 0 and out_kv.stride(1) != 1) or \
+                (T > 1 and out_kv.stride(0) < out_kv.shape[1]):
+            raise ValueError("out_kv must have kv's shape and dtype, with contiguous rows apart from each other")
+        same = out_kv.data_ptr() == kv.data_ptr() and (T <= 1 or out_kv.stride(0) == kv.stride(0))
+        if any(_overlap(out_kv, t) for t in inputs if t is not None and not (same and t is kv)):
+            raise ValueError("out_kv overlaps an input (in place means kv itself)")
+    if k_cache is not None:
+        if k_cache.dim() != 4 or k_cache.shape[2] != 1 or k_cache.shape[3] != d_latent + d_rope or \
+                k_cache.dtype != kv.dtype or not k_cache.is_contiguous():
+            raise ValueError("k_cache must be contiguous [P, bs, 1, latent + rope dims] of kv's dtype")
+        if slot_mapping.dtype != torch.int32 or not slot_mapping.is_contiguous() or slot_mapping.numel() != T:
+            raise ValueError("slot_mapping must be contiguous int32 [tokens]")
+        if any(_overlap(k_cache, t) for t in inputs if t is not None):
+            raise ValueError("k_cache overlaps an input")
+    if T == 0:
+        return oq, out_kv
+    row = d_latent + d_rope
+    with _on_device(dev):
+        rc = capi.lib().xllm_mi355_mla_norm_rope_and_cache(
+            q_pe.data_ptr(), oq.data_ptr(), kv.data_ptr(), _ptr(out_kv), kv_norm_weight.data_ptr(), float(eps),
+            cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], position_ids.data_ptr(), _ptr(k_cache), _ptr(slot_mapping),
+            T, H, d_latent, d_rope, *_head_strides(q_pe), *_head_strides(oq), kv.stride(0) if T > 1 else row,
+            0 if out_kv is None else out_kv.stride(0) if T > 1 else row, 0 if k_cache is None else k_cache.shape[1],
+            0 if k_cache is None else k_cache.shape[0], 1 if interleave else 0, _dtype_code(q_pe),
+            _dtype_code(cos_sin_cache), _stream(dev))
+    capi.check(rc, "xllm_mi355_mla_norm_rope_and_cache")
+    return oq, out_kv
+
+
+# ------------------------------------------------------------------------------------------
+# differential attention
+
+def batch_decode_diff(query, k_cache, v_cache, output, block_table, seq_lens, lambda_, scale=None, norm_weight=None,
+                      eps=1e-5, out_scale=1.0, window_left=-1):
+    """Paged decode of differential attention: head h attends with two maps, and the second one's result, times lambda, is
+    taken from the first one's:
+        o = (softmax(scale q[2h] K[2j]^T) - lambda softmax(scale q[2h + 1] K[2j + 1]^T)) V[j],  j = h / (H / pairs)
+        output[h] = out_scale * norm_weight * o / sqrt(mean(o^2) + eps)      (norm_weight None: out_scale * o)
+    query [B, 2 H, D]; k_cache [P, bs, 2 pairs, D]; v_cache [P, bs, pairs, 2 D] (a value cache of 2 pairs heads of D, viewed:
+    the same bytes, so reshape_paged_cache stores both); output [B, H, 2 D]; block_table [B, W] and seq_lens [B] int32 as in
+    batch_decode: an empty sequence gets zeros, a context beyond the table is cut there.  lambda_: the layer's learned
+    weight as float32, one value, [H], or [B, H].  norm_weight [2 D] of query's dtype; out_scale: usually 1 - lambda_init.
+    window_left >= 0: the last window_left + 1 tokens only.  bfloat16 or float16; D 64 or 128.  Returns output."""
+    dev = _require_cuda(query, k_cache, v_cache, output, block_table, seq_lens, lambda_, norm_weight)
+    if query.dim() != 3 or query.shape[1] % 2 != 0 or query.shape[1] == 0:
+        raise ValueError("query must be [B, 2 H, D]")
+    B, H2, D = query.shape
+    H = H2 // 2
+    if query.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("query must be bfloat16 or float16")
+    if not (query.stride(2) == 1 and query.stride(1) == D):
+        raise ValueError("query: last two dims must be contiguous")
+    if tuple(output.shape) != (B, H, 2 * D) or output.dtype != query.dtype or \
+            not (output.stride(2) == 1 and (H == 1 or output.stride(1) == 2 * D)):
+        raise ValueError("output must be [B, H, 2 D] of query's dtype with contiguous last two dims")
+    if k_cache.dim() != 4 or k_cache.shape[2] % 2 != 0 or k_cache.shape[2] == 0 or k_cache.shape[3] != D or \
+            not k_cache.is_contiguous():
+        raise ValueError("k_cache must be contiguous [P, bs, 2 pairs, D]")
+    P, bs, pairs = k_cache.shape[0], k_cache.shape[1], k_cache.shape[2] // 2
+    if tuple(v_cache.shape) != (P, bs, pairs, 2 * D) or not v_cache.is_contiguous():
+        raise ValueError("v_cache must be contiguous [P, bs, pairs, 2 D]")
+    if k_cache.dtype != query.dtype or v_cache.dtype != query.dtype:
+        raise TypeError("the caches must have query's dtype")
+    if H % pairs != 0:
+        raise ValueError("the heads must be a multiple of the KV pairs")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or \
+            block_table.shape[0] != B:
+        raise ValueError("block_table must be int32 [B, W] with unit column stride, one row per sequence")
+    if seq_lens.dtype != torch.int32 or seq_lens.numel() != B or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be contiguous int32 [B]")
+    if lambda_.dtype != torch.float32:
+        raise TypeError("lambda_ must be float32")
+    if lambda_.numel() == 1:
+        lam_b = lam_h = 0
+    elif tuple(lambda_.shape) == (H,):
+        lam_b, lam_h = 0, lambda_.stride(0)
+    elif tuple(lambda_.shape) == (B, H):
+        lam_b, lam_h = lambda_.stride()
+    else:
+        raise ValueError("lambda_ must hold one value, or be [H] or [B, H]")
+    if norm_weight is not None and (norm_weight.dtype != query.dtype or norm_weight.numel() != 2 * D or
+                                    not norm_weight.is_contiguous()):
+        raise ValueError("norm_weight must be contiguous [2 D] of query's dtype")
+    if B > 1 and output.stride(0) < 2 * H * D:
+        raise ValueError("output: rows must not overlap")
+    if any(_overlap(output, t) for t in (query, k_cache, v_cache, block_table, seq_lens, lambda_, norm_weight)):
+        raise ValueError("output overlaps an input")
+    if scale is None:
+        scale = D ** -0.5
+    if B == 0:
+        return output
+    lib = capi.lib()
+    with _on_device(dev):
+        # (a workspace of the call's own: calls on other streams and captured graphs never meet in it)
+        ws = torch.empty(max(1, lib.xllm_mi355_paged_decode_diff_workspace_bytes(H, pairs, D)), dtype=torch.uint8, device=dev)
+        rc = lib.xllm_mi355_paged_decode_diff(
+            query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), output.data_ptr(), block_table.data_ptr(),
+            max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], seq_lens.data_ptr(),
+            lambda_.data_ptr(), lam_b, lam_h, _ptr(norm_weight), float(eps), float(out_scale), B, H, pairs, D, bs, P,
+            query.stride(0) if B > 1 else H2 * D, output.stride(0) if B > 1 else H2 * D, int(window_left), float(scale),
+            ws.data_ptr(), ws.numel(), _dtype_code(query), _stream(dev))
+    capi.check(rc, "xllm_mi355_paged_decode_diff")
+    return output
