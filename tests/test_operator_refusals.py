@@ -7,6 +7,7 @@ import torch
 from xllm_amd import capi, ops
 
 FAKE = 1 << 20   # an aligned non-null address: the calls below return before anything is launched
+APART = [1 << (24 + i) for i in range(16)]   # aligned addresses whose tensors do not meet
 BF16, FP16, FP32, FP8 = capi.BF16, capi.FP16, capi.FP32, capi.FP8_E4M3
 EINVAL, EDTYPE, ESHAPE, EWORKSPACE, EALIGN = -1, -2, -3, -4, -5
 
@@ -104,6 +105,58 @@ def test_differential_decode():
         assert call(fn, base, **change) == EALIGN, change
     for change in (dict(ws=None), dict(ws=FAKE + 64), dict(ws_bytes=size(16, 4, 128) - 1)):
         assert call(fn, base, **change) == EWORKSPACE, change
+
+
+def test_outputs_that_meet_inputs_or_each_other():
+    """Addresses far apart, then one output moved onto each of the other operands in turn."""
+    lib = capi.lib()
+
+    def spread(base, names):
+        at = dict(zip(names, APART))
+        return dict(base, **at), at
+
+    st = strides(512, 128)
+    tables, at = spread(dict(kv=0, new=0, tin=0, in_stride=8, tout=0, out_stride=8, width=8, free=0, n_free=9, head=0, seq=0,
+                             cu=0, pos=0, slots=0, indptr=0, counters=0, batch=4, bs=16, budget=8, stream=None),
+                        ("kv", "new", "tin", "tout", "free", "head", "seq", "cu", "pos", "slots", "indptr", "counters"))
+    for out in ("tout", "seq", "cu", "pos", "slots", "indptr", "counters"):
+        for other in at:
+            if other != out and (out, other) != ("tout", "tin"):
+                got = call(lib.xllm_mi355_build_step_tables, tables, **{out: at[other]})
+                assert got == EINVAL, (out, other)
+    assert call(lib.xllm_mi355_build_step_tables, tables, tout=at["tin"] + 4) == EINVAL
+    rot, at = spread(dict(pos=0, table=0, rows=10, q=0, qo=0, k=0, ko=0, T=4, hq=4, hk=4, dq=128, dk=128, oq=0, ok=0, R=64,
+                          sq=st, sqo=st, sk=st, sko=st, interleave=0, inverse=0, dtype=BF16, ctype=FP32, stream=None),
+                     ("pos", "table", "q", "qo", "k", "ko"))
+    for out, others in (("qo", ("pos", "table", "k", "ko")), ("ko", ("pos", "table", "q", "qo"))):
+        for other in others:
+            assert call(lib.xllm_mi355_rotary_embedding, rot, **{out: at[other]}) == EINVAL, (out, other)
+    assert call(lib.xllm_mi355_rotary_embedding, rot, qo=at["q"] + 16) == EINVAL
+    assert call(lib.xllm_mi355_rotary_embedding, rot, qo=at["q"], sqo=strides(512, 64)) == EINVAL   # heads meet
+    assert call(lib.xllm_mi355_rotary_embedding, rot, sqo=strides(256, 128)) == EINVAL              # tokens meet
+    mla, at = spread(dict(q=0, qo=0, kv=0, kvo=0, w=0, eps=1e-6, table=0, rows=10, pos=0, cache=0, slots=0, T=4, H=8, dl=512,
+                          dr=64, qt=1536, qh=192, qot=512, qoh=64, kvs=576, kvos=576, bs=16, P=4, interleave=1, dtype=BF16,
+                          ctype=FP32, stream=None),
+                     ("q", "qo", "kv", "kvo", "w", "table", "pos", "cache", "slots"))
+    for out in ("qo", "kvo", "cache"):
+        for other in at:
+            if other != out and (out, other) != ("kvo", "kv"):
+                got = call(lib.xllm_mi355_mla_norm_rope_and_cache, mla, **{out: at[other]})
+                assert got == EINVAL, (out, other)
+    assert call(lib.xllm_mi355_mla_norm_rope_and_cache, mla, kvo=at["kv"] + 16) == EINVAL
+    rows, at = spread(dict(inv=0, pos=0, first=0, rows=4, half=32, factor=1.0, out=0, dtype=FP32, stream=None), ("inv", "pos", "out"))
+    for other in ("inv", "pos"):
+        assert call(lib.xllm_mi355_rope_cos_sin, rows, out=at[other]) == EINVAL
+    need = lib.xllm_mi355_paged_decode_diff_workspace_bytes(4, 2, 64)
+    diff, at = spread(dict(q=0, k=0, v=0, out=0, table=0, stride=8, width=8, lens=0, lam=0, lb=0, lh=1, w=0, eps=1e-5,
+                           out_scale=1.0, batch=2, H=4, pairs=2, D=64, bs=16, P=4, qs=512, os=512, window=-1, scale=0.1,
+                           ws=0, ws_bytes=need, dtype=BF16, stream=None),
+                      ("q", "k", "v", "out", "table", "lens", "lam", "w", "ws"))
+    diff["ws"] = at["ws"] = 1 << 45
+    for out in ("out", "ws"):
+        for other in at:
+            if other != out:
+                assert call(lib.xllm_mi355_paged_decode_diff, diff, **{out: at[other]}) == EINVAL, (out, other)
 
 
 def test_cpu_tensors_are_refused():

@@ -215,6 +215,18 @@ int mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const void* kv, vo
                             int64_t block_size, int64_t num_blocks, int interleave, int dtype, int cos_sin_dtype,
                             hipStream_t stream);
 
+// Memory that a tensor argument spans, for the refusal of outputs that overlap inputs.
+struct Span {
+  uintptr_t lo = 0, hi = 0;
+  Span() = default;
+  Span(const void* p, int64_t bytes) : lo(reinterpret_cast<uintptr_t>(p)), hi(p == nullptr ? 0 : lo + static_cast<uintptr_t>(bytes)) {}
+  bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
+};
+// [n0, n1, inner] elements with strides s0, s1 and a contiguous last dim.
+inline Span span_of(const void* p, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t inner, int64_t elem_bytes) {
+  return Span(p, ((n0 - 1) * s0 + (n1 - 1) * s1 + inner) * elem_bytes);
+}
+
 // Kernel attributes (dynamic LDS size) are set per device.  Returns true the first time it is called with
 // `seen` on the current device (devices 0..63; beyond that always true: setting them again is harmless).
 inline bool first_use_on_current_device(std::atomic<uint64_t>& seen) {

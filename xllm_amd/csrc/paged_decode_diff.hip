@@ -676,6 +676,16 @@ int paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, v
   const size_t need = diff_workspace_bytes(n_heads, n_kv_pairs, head_dim);
   if (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < need) return XLLM_MI355_EWORKSPACE;
 
+  {
+    const int64_t cache = num_blocks * block_size * n_kv_pairs * head_dim * 4, row = 2 * n_heads * head_dim;
+    const Span out_rows = span_of(out, batch, out_token_stride, 1, 0, row, 2), space(workspace, static_cast<int64_t>(need));
+    for (const Span& r : {span_of(q, batch, q_token_stride, 1, 0, row, 2), Span(k_cache, cache), Span(v_cache, cache),
+                          span_of(block_table, batch, table_stride, 1, 0, table_width, 4), Span(seq_lens, batch * 4),
+                          span_of(lambda, batch, lambda_batch_stride, n_heads, lambda_head_stride, 1, 4),
+                          Span(norm_weight, norm_weight != nullptr ? 4 * head_dim : 0)})
+      if (out_rows.meets(r) || space.meets(r)) return XLLM_MI355_EINVAL;
+    if (out_rows.meets(space)) return XLLM_MI355_EINVAL;
+  }
   DiffArgs a = {};
   a.n_heads = static_cast<int>(n_heads);
   a.n_pairs = static_cast<int>(n_kv_pairs);

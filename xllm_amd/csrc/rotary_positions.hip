@@ -528,6 +528,11 @@ int dispatch_mla_prologue(const MlaPrologueArgs& a, int interleave, int cos_sin_
 #undef XLLM_MLA_P
 }
 
+// Rows of `inner` elements at n0 strides of s0 and n1 strides of s1: does each lie apart from the others?
+bool rows_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t inner) {
+  return ((n1 == 1 || s1 >= inner) && (n0 == 1 || s0 >= (n1 - 1) * s1 + inner)) ||
+         ((n0 == 1 || s0 >= inner) && (n1 == 1 || s1 >= (n0 - 1) * s0 + inner));
+}
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 }  // namespace
@@ -537,6 +542,9 @@ int rope_cos_sin(const double* inv_freq, const int64_t* positions, int64_t first
   if (n_rows == 0) return XLLM_MI355_OK;
   if (inv_freq == nullptr || out == nullptr || n_rows < 0 || half <= 0) return XLLM_MI355_EINVAL;
   if (half > 4096 || n_rows > (1LL << 40)) return XLLM_MI355_ESHAPE;
+  if (out_dtype != XLLM_MI355_FP32 && out_dtype != XLLM_MI355_BF16 && out_dtype != XLLM_MI355_FP16) return XLLM_MI355_EDTYPE;
+  const Span w(out, n_rows * half * (out_dtype == XLLM_MI355_FP32 ? 8 : 4));
+  if (w.meets(Span(inv_freq, half * 8)) || w.meets(Span(positions, n_rows * 8))) return XLLM_MI355_EINVAL;
   switch (out_dtype) {
     case XLLM_MI355_FP32: return launch_cos_sin<XLLM_MI355_FP32>(inv_freq, positions, first_position, n_rows, half, factor, out, stream);
     case XLLM_MI355_BF16: return launch_cos_sin<XLLM_MI355_BF16>(inv_freq, positions, first_position, n_rows, half, factor, out, stream);
@@ -580,8 +588,7 @@ int rotary_embedding(const int64_t* positions, const void* cos_sin, int64_t n_po
     s.heads = static_cast<int>(heads);
     s.dim = static_cast<int>(dim);
     s.offset = static_cast<int>(offset);
-    if (si[0] < 0 || si[1] < 0 || so[0] < 0 || so[1] < 0) return false;
-    return in != out || (si[0] == so[0] && si[1] == so[1]);   // (in place the elements stay where they are)
+    return !(si[0] < 0 || si[1] < 0 || so[0] < 0 || so[1] < 0);
   };
   bool copy_rest = false;
   // 16 bytes per lane where every word of every head starts on one; element by element otherwise
@@ -597,6 +604,22 @@ int rotary_embedding(const int64_t* positions, const void* cos_sin, int64_t n_po
     if (!side(a.k, k, k_out, k_strides, k_out_strides, n_heads_k, head_dim_k, rotary_offset_k)) return XLLM_MI355_EINVAL;
     add(a.k);
   }
+  // A result goes to its own operand, element for element, or apart from everything that is read; its heads do not meet.
+  const Span read[4] = {span_of(q, n_tokens, a.q.in_token, n_heads_q, a.q.in_head, head_dim_q, es),
+                        n_heads_k > 0 ? span_of(k, n_tokens, a.k.in_token, n_heads_k, a.k.in_head, head_dim_k, es) : Span(),
+                        Span(cos_sin, n_positions * rotary_dim * table_size), Span(positions, n_tokens * 8)};
+  for (const RotSide* s : {&a.q, &a.k}) {
+    if (s->heads == 0) continue;
+    if (!rows_apart(n_tokens, s->out_token, s->heads, s->out_head, s->dim)) return XLLM_MI355_EINVAL;
+    if (s->in == s->out) {
+      if (s->in_token != s->out_token || s->in_head != s->out_head) return XLLM_MI355_EINVAL;
+      continue;
+    }
+    const Span w = span_of(s->out, n_tokens, s->out_token, s->heads, s->out_head, s->dim, es);
+    for (const Span& r : read)
+      if (w.meets(r)) return XLLM_MI355_EINVAL;
+  }
+  if (n_heads_k > 0 && a.q.out == a.k.out) return XLLM_MI355_EINVAL;
   a.positions = positions;
   a.cos_sin = static_cast<const char*>(cos_sin);
   a.n_positions = n_positions;
@@ -621,6 +644,8 @@ int mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const void* kv, vo
     return XLLM_MI355_EINVAL;
   if (k_cache == nullptr && kv_out == nullptr) return XLLM_MI355_EINVAL;
   if (dtype != XLLM_MI355_BF16 && dtype != XLLM_MI355_FP16) return XLLM_MI355_EDTYPE;
+  if (cos_sin_dtype != XLLM_MI355_BF16 && cos_sin_dtype != XLLM_MI355_FP16 && cos_sin_dtype != XLLM_MI355_FP32)
+    return XLLM_MI355_EDTYPE;
   if (d_latent != kLatent || d_rope != kRopeDim || n_heads > 65535 || n_tokens > (1LL << 31)) return XLLM_MI355_ESHAPE;
   if (q_token_stride < 0 || q_head_stride < 0 || q_out_token_stride < 0 || q_out_head_stride < 0 ||
       kv_row_stride < d_latent + d_rope || (kv_out != nullptr && kv_out_row_stride < d_latent + d_rope))
@@ -635,6 +660,25 @@ int mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const void* kv, vo
       ((q_token_stride | q_head_stride | q_out_token_stride | q_out_head_stride | kv_row_stride) & 7) != 0 ||
       (kv_out != nullptr && (kv_out_row_stride & 7) != 0))
     return XLLM_MI355_EALIGN;
+  {
+    const int64_t table_size = cos_sin_dtype == XLLM_MI355_FP32 ? 4 : 2, row = kLatent + kRopeDim;
+    const Span sq = span_of(q_pe, n_tokens, q_token_stride, n_heads, q_head_stride, kRopeDim, 2);
+    const Span skv = span_of(kv, n_tokens, kv_row_stride, 1, 0, row, 2);
+    const Span rest[4] = {Span(kv_weight, kLatent * 2), Span(cos_sin, n_positions * kRopeDim * table_size),
+                          Span(positions, n_tokens * 8), Span(slots, k_cache != nullptr ? n_tokens * 4 : 0)};
+    const Span wq = span_of(q_pe_out, n_tokens, q_out_token_stride, n_heads, q_out_head_stride, kRopeDim, 2);
+    const Span wkv = kv_out != nullptr ? span_of(kv_out, n_tokens, kv_out_row_stride, 1, 0, row, 2) : Span();
+    const Span wc = Span(k_cache, k_cache != nullptr ? num_blocks * block_size * row * 2 : 0);
+    if (!rows_apart(n_tokens, q_out_token_stride, n_heads, q_out_head_stride, kRopeDim)) return XLLM_MI355_EINVAL;
+    if (q_pe_out == q_pe ? q_out_token_stride != q_token_stride || q_out_head_stride != q_head_stride
+                         : wq.meets(sq) || wq.meets(skv))
+      return XLLM_MI355_EINVAL;
+    if (kv_out == kv ? kv_out_row_stride != kv_row_stride : wkv.meets(skv) || wkv.meets(sq)) return XLLM_MI355_EINVAL;
+    if (q_pe_out != q_pe && kv_out != kv && wq.meets(wkv)) return XLLM_MI355_EINVAL;
+    if (wc.meets(sq) || wc.meets(skv) || wc.meets(wq) || wc.meets(wkv)) return XLLM_MI355_EINVAL;
+    for (const Span& r : rest)
+      if (wq.meets(r) || wkv.meets(r) || wc.meets(r)) return XLLM_MI355_EINVAL;
+  }
   MlaPrologueArgs a = {};
   a.q = static_cast<const uint16_t*>(q_pe);
   a.q_out = static_cast<uint16_t*>(q_pe_out);

@@ -247,11 +247,25 @@ int build_step_tables(const int32_t* kv_lens, const int32_t* new_lens, const int
   if (batch < 0 || block_size <= 0 || table_width <= 0 || n_free < 0 || max_new_tokens < 0 || in_stride < table_width ||
       out_stride < table_width)
     return XLLM_MI355_EINVAL;
-  // (in place the rows must lie at the same addresses)
-  if (block_table_in == block_table_out && in_stride != out_stride) return XLLM_MI355_EINVAL;
   constexpr int64_t kLimit = (1LL << 30) - 1;   // the sum of two stays inside 32 bits
   if (max_new_tokens > kLimit || n_free > kLimit || table_width > kLimit || block_size > kLimit || batch > (1LL << 20))
     return XLLM_MI355_ESHAPE;
+  // No output meets an input or another output, but for the table in place, entry for entry.
+  {
+    const bool in_place = block_table_in == block_table_out;
+    if (in_place && in_stride != out_stride) return XLLM_MI355_EINVAL;
+    const Span read[5] = {Span(kv_lens, batch * 4), Span(new_lens, batch * 4), Span(free_pages, n_free * 4),
+                          Span(free_head, 4), span_of(block_table_in, batch, in_stride, 1, 0, table_width, 4)};
+    const Span written[7] = {span_of(block_table_out, batch, out_stride, 1, 0, table_width, 4), Span(seq_lens, batch * 4),
+                             Span(cu_new, batch * 4 + 4), Span(positions, max_new_tokens * 8), Span(slots, max_new_tokens * 4),
+                             Span(new_page_indptr, batch * 4 + 4), Span(counters, 12)};
+    for (int i = 0; i < 7; ++i) {
+      for (int j = 0; j < 5; ++j)
+        if (written[i].meets(read[j]) && !(in_place && i == 0 && j == 4)) return XLLM_MI355_EINVAL;
+      for (int j = 0; j < i; ++j)
+        if (written[i].meets(written[j])) return XLLM_MI355_EINVAL;
+    }
+  }
   StepArgs a = {};
   a.kv_lens = kv_lens;
   a.new_lens = new_lens;

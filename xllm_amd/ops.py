@@ -26,8 +26,8 @@ Operators around the path that the reference does on the host, in its layers or 
 
 Errors: the reference CHECK-aborts; here every violated precondition raises.
 """
-import contextlib
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -48,6 +48,8 @@ def _dtype_code(t):
 
 
 def _stream(device):
+    if device.index is not None:   # (the stream's handle without a Stream object around it: 0.1 us instead of 2 us)
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -814,21 +816,24 @@ def absorbed_bmm(x, w, out=None):
 # ------------------------------------------------------------------------------------------
 # the tables of a step
 
-def _on_device(dev):
-    """Launches go to the tensors' device, whatever the current one is."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _launch(dev, name, *args):
+    """The entry point `name` of the library on dev's current stream, with dev as the current device."""
+    fn = getattr(capi.lib(), name)
+    if torch.cuda.current_device() == dev.index:
+        return fn(*args, _stream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, _stream(dev))
 
 
-def _byte_range(t):
-    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+_EINVAL = -1
 
 
-def _overlap(a, b):
-    if a is None or b is None or a.numel() == 0 or b.numel() == 0:
-        return False
-    (a0, a1), (b0, b1) = _byte_range(a), _byte_range(b)
-    return a0 < b1 and b0 < a1
+def _check_launch(rc, name, what):
+    """The library refuses operands that overlap; `what` says so in the words of the Python call, whose other arguments
+    were found good before."""
+    if rc == _EINVAL:
+        raise ValueError(what)
+    capi.check(rc, name)
 
 
 @dataclass
@@ -861,48 +866,44 @@ def build_step_tables(kv_lens, new_lens, block_table, free_pages, block_size, ma
     out: StepTables to write into (the persistent buffers of a captured step); its block_table may be block_table itself.
     Returns StepTables."""
     dev = _require_cuda(kv_lens, new_lens, block_table, free_pages, free_head)
+    i32 = torch.int32
     for name, t in (("kv_lens", kv_lens), ("new_lens", new_lens), ("free_pages", free_pages)):
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        if t.dtype != i32 or t.dim() != 1 or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 vector")
     B, F, T, block_size = kv_lens.numel(), free_pages.numel(), int(max_new_tokens), int(block_size)
     if new_lens.numel() != B:
         raise ValueError("kv_lens and new_lens must have one entry per request")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or \
-            block_table.shape[0] != B or block_table.shape[1] == 0:
+    if block_table.dtype != i32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] == 0 or \
+            block_table.stride(1) != 1:
         raise ValueError("block_table must be int32 [B, W] with unit column stride, one row per request")
-    if free_head is not None and (free_head.dtype != torch.int32 or free_head.numel() != 1):
+    if free_head is not None and (free_head.dtype != i32 or free_head.numel() != 1):
         raise ValueError("free_head must be int32 [1]")
     if block_size <= 0 or T < 0:
         raise ValueError("block_size must be positive and max_new_tokens not negative")
     W = block_table.shape[1]
-    if B > 1 and block_table.stride(0) < W:
+    in_stride = block_table.stride(0) if B > 1 else W
+    if in_stride < W:
         raise ValueError("block_table: rows must not overlap")
     if out is None:
-        seq_lens, cu, indptr, counters, slots = torch.empty(
-            3 * B + 5 + T, dtype=torch.int32, device=dev).split([B, B + 1, B + 1, 3, T])
-        out = StepTables(torch.empty(B, W, dtype=torch.int32, device=dev), seq_lens, cu,
+        seq_lens, cu, indptr, counters, slots = torch.empty(3 * B + 5 + T, dtype=i32, device=dev).split(
+            (B, B + 1, B + 1, 3, T))
+        out = StepTables(torch.empty((B, W), dtype=i32, device=dev), seq_lens, cu,
                          torch.empty(T, dtype=torch.int64, device=dev), slots, indptr, counters)
+        out_stride = W
     else:
         fields = [getattr(out, f) for f in _I32_FIELDS]
         _require_cuda(kv_lens, out.position_ids, *fields)
         sizes = dict(seq_lens=B, q_cu_seq_lens=B + 1, slot_mapping=T, new_page_indptr=B + 1, counters=3)
         for f, t in zip(_I32_FIELDS, fields):
-            if t.dtype != torch.int32 or (f in sizes and (tuple(t.shape) != (sizes[f],) or not t.is_contiguous())):
+            if t.dtype != i32 or (f in sizes and (tuple(t.shape) != (sizes[f],) or not t.is_contiguous())):
                 raise ValueError(f"out.{f} must be contiguous int32 of its documented size")
         if out.position_ids.dtype != torch.int64 or tuple(out.position_ids.shape) != (T,) or \
                 not out.position_ids.is_contiguous():
             raise ValueError("out.position_ids must be contiguous int64 [max_new_tokens]")
         tab = out.block_table
-        if tuple(tab.shape) != (B, W) or tab.stride(1) != 1 or (B > 1 and tab.stride(0) < W):
+        out_stride = tab.stride(0) if B > 1 else W
+        if tuple(tab.shape) != (B, W) or tab.stride(1) != 1 or out_stride < W:
             raise ValueError("out.block_table must be [B, W] with unit column stride")
-        same = tab.data_ptr() == block_table.data_ptr() and (B <= 1 or tab.stride(0) == block_table.stride(0))
-        written = fields + [out.position_ids]
-        for i, t in enumerate(written):
-            if any(_overlap(t, x) for x in (kv_lens, new_lens, free_pages, free_head)) or \
-                    (_overlap(t, block_table) and not (i == 0 and same)):
-                raise ValueError("an output of build_step_tables overlaps one of its inputs")
-            if any(_overlap(t, x) for x in written[:i]):
-                raise ValueError("two outputs of build_step_tables overlap")
     if B == 0:
         for t in (out.q_cu_seq_lens, out.new_page_indptr, out.counters, out.position_ids):
             t.zero_()
@@ -910,14 +911,12 @@ def build_step_tables(kv_lens, new_lens, block_table, free_pages, block_size, ma
             out.counters[1:2].copy_(free_head.view(1).clamp(0, F))
         out.slot_mapping.fill_(-1)
         return out
-    with _on_device(dev):
-        rc = capi.lib().xllm_mi355_build_step_tables(
-            kv_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), max(W, block_table.stride(0)),
-            out.block_table.data_ptr(), max(W, out.block_table.stride(0)), W, free_pages.data_ptr() if F else None, F,
-            _ptr(free_head), out.seq_lens.data_ptr(), out.q_cu_seq_lens.data_ptr(), _ptr(out.position_ids) or None,
-            _ptr(out.slot_mapping) or None, out.new_page_indptr.data_ptr(), out.counters.data_ptr(), B, block_size, T,
-            _stream(dev))
-    capi.check(rc, "xllm_mi355_build_step_tables")
+    rc = _launch(dev, "xllm_mi355_build_step_tables", kv_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
+                 in_stride, out.block_table.data_ptr(), out_stride, W, free_pages.data_ptr(), F, _ptr(free_head),
+                 out.seq_lens.data_ptr(), out.q_cu_seq_lens.data_ptr(), out.position_ids.data_ptr(),
+                 out.slot_mapping.data_ptr(), out.new_page_indptr.data_ptr(), out.counters.data_ptr(), B, block_size, T)
+    _check_launch(rc, "xllm_mi355_build_step_tables",
+                  "an output of build_step_tables overlaps an input or another output (in place means block_table itself)")
     return out
 
 
@@ -1020,17 +1019,13 @@ def build_cos_sin_cache(inv_freq, num_positions=0, position_ids=None, first_posi
         out = torch.empty(shape, dtype=dtype, device=dev)
     elif tuple(out.shape) != shape or not out.is_contiguous():
         raise ValueError("out must be contiguous [rows, rotary_dim]")
-    elif _overlap(out, inv_freq) or _overlap(out, position_ids):
-        raise ValueError("out overlaps an input")
     if out.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise TypeError("cos_sin rows are float32, bfloat16 or float16")
     if rows == 0:
         return out
-    with _on_device(dev):
-        rc = capi.lib().xllm_mi355_rope_cos_sin(
-            inv_freq.data_ptr(), _ptr(position_ids), int(first_position), rows, inv_freq.numel(), float(attention_factor),
-            out.data_ptr(), _dtype_code(out), _stream(dev))
-    capi.check(rc, "xllm_mi355_rope_cos_sin")
+    rc = _launch(dev, "xllm_mi355_rope_cos_sin", inv_freq.data_ptr(), _ptr(position_ids), int(first_position), rows,
+                 inv_freq.numel(), float(attention_factor), out.data_ptr(), _dtype_code(out))
+    _check_launch(rc, "xllm_mi355_rope_cos_sin", "out overlaps an input")
     return out
 
 
@@ -1046,26 +1041,24 @@ def _check_cos_sin(cos_sin_cache, position_ids, n_tokens):
         raise TypeError("cos_sin_cache must be float32, bfloat16 or float16")
 
 
-def _head_strides(x):
-    """(token, head) strides; 0 where there is only one of them (its stride then means nothing)."""
-    return x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0
-
-
-def _check_rotated(name, x, out, inputs):
-    """x [T, H, D] and where its result goes: x itself, or a tensor apart from every input."""
-    if x.dim() != 3 or x.shape[1] == 0 or (x.numel() > 0 and x.stride(2) != 1):
+def _check_rotated(name, x, out):
+    """x [T, H, D] and where its result goes: their shape, and {token, head} strides for the library (0 where there is only
+    one of them: its stride then means nothing)."""
+    if x.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim]")
+    T, H, D = x.shape
+    ts, hs, es = x.stride()
+    if H == 0 or D == 0 or (es != 1 and T > 0):
         raise ValueError(f"{name} must be [tokens, heads, head_dim], contiguous in its last dim")
-    if out is not x:
-        if out.shape != x.shape or out.dtype != x.dtype or (x.numel() > 0 and out.stride(2) != 1):
-            raise ValueError(f"out_{name} must have {name}'s shape and dtype, contiguous in its last dim")
-        same = out.data_ptr() == x.data_ptr() and _head_strides(out) == _head_strides(x)
-        if any(_overlap(out, t) for t in inputs if not (same and t is x)):
-            raise ValueError(f"out_{name} overlaps an input (in place means {name} itself)")
-    (ts, hs), (T, H, D) = _head_strides(out), out.shape
-    # every element written once: heads inside tokens or tokens inside heads
-    if not ((H == 1 or hs >= D) and (T <= 1 or ts >= (H - 1) * hs + D)) and \
-            not ((T <= 1 or ts >= D) and (H == 1 or hs >= (T - 1) * ts + D)):
-        raise ValueError(f"{name}: the heads of the result overlap each other")
+    strides = _Strides(ts if T > 1 else 0, hs if H > 1 else 0)
+    if out is x:
+        return T, H, D, strides, strides
+    if out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError(f"out_{name} must have {name}'s shape and dtype")
+    ts, hs, es = out.stride()
+    if es != 1 and T > 0:
+        raise ValueError(f"out_{name} must be contiguous in its last dim")
+    return T, H, D, strides, _Strides(ts if T > 1 else 0, hs if H > 1 else 0)
 
 
 def rotary_embedding(position_ids, query, key, cos_sin_cache, interleave=False, rotary_offset=0, key_rotary_offset=None,
@@ -1082,36 +1075,30 @@ def rotary_embedding(position_ids, query, key, cos_sin_cache, interleave=False, 
     ok = key if out_key is None else out_key
     if key is None and out_key is not None:
         raise ValueError("out_key without a key")
-    if query.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    code = _dtype_code(query)
+    if code == capi.FP8_E4M3:
         raise TypeError("query must be bfloat16, float16 or float32")
-    inputs = [t for t in (query, key, cos_sin_cache, position_ids) if t is not None]
-    _check_rotated("query", query, oq, inputs)
-    T, Hq, D = query.shape
+    T, Hq, D, q_st, oq_st = _check_rotated("query", query, oq)
     _check_cos_sin(cos_sin_cache, position_ids, T)
-    R = cos_sin_cache.shape[1]
-    Hk = Dk = 0
-    if key is not None:
-        _check_rotated("key", key, ok, inputs)
-        if key.shape[0] != T or key.dtype != query.dtype:
-            raise ValueError("key must have query's tokens and dtype")
-        if oq.data_ptr() == ok.data_ptr() and T > 0:
-            raise ValueError("the results of query and key overlap")
-        Hk, Dk = key.shape[1], key.shape[2]
+    rows, R = cos_sin_cache.shape
     k_off = rotary_offset if key_rotary_offset is None else key_rotary_offset
+    Hk = Dk = 0
+    k_st = ok_st = None
+    if key is not None:
+        Tk, Hk, Dk, k_st, ok_st = _check_rotated("key", key, ok)
+        if Tk != T or key.dtype != query.dtype:
+            raise ValueError("key must have query's tokens and dtype")
     if R % 2 != 0 or R == 0:
         raise ValueError("the rotary dim must be even")
-    if rotary_offset < 0 or rotary_offset + R > D or (key is not None and (k_off < 0 or k_off + R > Dk)):
+    if rotary_offset < 0 or rotary_offset + R > D or (Hk and (k_off < 0 or k_off + R > Dk)):
         raise ValueError("the rotated part must lie inside the head")
     if T == 0:
         return oq, ok
-    with _on_device(dev):
-        rc = capi.lib().xllm_mi355_rotary_embedding(
-            position_ids.data_ptr(), cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], query.data_ptr(), oq.data_ptr(),
-            _ptr(key), _ptr(ok), T, Hq, Hk, D, Dk, rotary_offset, k_off if Hk else 0, R, _Strides(*_head_strides(query)),
-            _Strides(*_head_strides(oq)), _Strides(*_head_strides(key)) if Hk else None,
-            _Strides(*_head_strides(ok)) if Hk else None, 1 if interleave else 0, 1 if inverse else 0, _dtype_code(query),
-            _dtype_code(cos_sin_cache), _stream(dev))
-    capi.check(rc, "xllm_mi355_rotary_embedding")
+    rc = _launch(dev, "xllm_mi355_rotary_embedding", position_ids.data_ptr(), cos_sin_cache.data_ptr(), rows,
+                 query.data_ptr(), oq.data_ptr(), _ptr(key), _ptr(ok), T, Hq, Hk, D, Dk, rotary_offset, k_off if Hk else 0, R,
+                 q_st, oq_st, k_st, ok_st, 1 if interleave else 0, 1 if inverse else 0, code, _dtype_code(cos_sin_cache))
+    _check_launch(rc, "xllm_mi355_rotary_embedding",
+                  "a result of rotary_embedding overlaps itself, the other one or an input (in place means the operand itself)")
     return oq, ok
 
 
@@ -1125,15 +1112,15 @@ def mla_norm_rope_and_cache(q_pe, kv, kv_norm_weight, eps, cos_sin_cache, interl
     Returns (q_pe's result, out_kv)."""
     dev = _require_cuda(q_pe, kv, kv_norm_weight, cos_sin_cache, position_ids, k_cache, slot_mapping, out_q_pe, out_kv)
     oq = q_pe if out_q_pe is None else out_q_pe
-    if q_pe.dtype not in (torch.bfloat16, torch.float16):
+    dtype = q_pe.dtype
+    if dtype != torch.bfloat16 and dtype != torch.float16:
         raise TypeError("q_pe must be bfloat16 or float16")
-    inputs = (q_pe, kv, kv_norm_weight, cos_sin_cache, position_ids, slot_mapping)
-    _check_rotated("q_pe", q_pe, oq, [t for t in inputs if t is not None])
-    T, H, d_rope = q_pe.shape
+    T, H, d_rope, q_st, oq_st = _check_rotated("q_pe", q_pe, oq)
     d_latent = kv_norm_weight.numel()
-    if kv.dim() != 2 or kv.shape[0] != T or kv.shape[1] != d_latent + d_rope or (T > 0 and kv.stride(1) != 1):
+    row = d_latent + d_rope
+    if kv.dim() != 2 or kv.shape[0] != T or kv.shape[1] != row or (T > 0 and kv.stride(1) != 1):
         raise ValueError("kv must be [tokens, latent + rope dims] with contiguous rows")
-    if not (kv.dtype == kv_norm_weight.dtype == q_pe.dtype) or not kv_norm_weight.is_contiguous():
+    if kv.dtype != dtype or kv_norm_weight.dtype != dtype or not kv_norm_weight.is_contiguous():
         raise TypeError("kv and kv_norm_weight must have q_pe's dtype, the weight contiguous")
     _check_cos_sin(cos_sin_cache, position_ids, T)
     if cos_sin_cache.shape[1] != d_rope:
@@ -1142,38 +1129,47 @@ def mla_norm_rope_and_cache(q_pe, kv, kv_norm_weight, eps, cos_sin_cache, interl
         raise ValueError("k_cache and slot_mapping come together")
     if k_cache is None and out_kv is None:
         raise ValueError("the latent rows need a place: k_cache or out_kv")
+    out_row = blocks = block_size = 0
     if out_kv is not None:
-        if out_kv.shape != kv.shape or out_kv.dtype != kv.dtype or (T > 0 and out_kv.stride(1) != 1) or \
-                (T > 1 and out_kv.stride(0) < out_kv.shape[1]):
-            raise ValueError("out_kv must have kv's shape and dtype, with contiguous rows apart from each other")
-        same = out_kv.data_ptr() == kv.data_ptr() and (T <= 1 or out_kv.stride(0) == kv.stride(0))
-        if any(_overlap(out_kv, t) for t in inputs if t is not None and not (same and t is kv)):
-            raise ValueError("out_kv overlaps an input (in place means kv itself)")
+        if out_kv.shape != kv.shape or out_kv.dtype != dtype or (T > 0 and out_kv.stride(1) != 1):
+            raise ValueError("out_kv must have kv's shape and dtype, with contiguous rows")
+        out_row = out_kv.stride(0) if T > 1 else row
+        if out_row < row:
+            raise ValueError("out_kv: rows must not overlap")
     if k_cache is not None:
-        if k_cache.dim() != 4 or k_cache.shape[2] != 1 or k_cache.shape[3] != d_latent + d_rope or \
-                k_cache.dtype != kv.dtype or not k_cache.is_contiguous():
+        if k_cache.dim() != 4 or k_cache.shape[2] != 1 or k_cache.shape[3] != row or k_cache.dtype != dtype or \
+                not k_cache.is_contiguous():
             raise ValueError("k_cache must be contiguous [P, bs, 1, latent + rope dims] of kv's dtype")
         if slot_mapping.dtype != torch.int32 or not slot_mapping.is_contiguous() or slot_mapping.numel() != T:
             raise ValueError("slot_mapping must be contiguous int32 [tokens]")
-        if any(_overlap(k_cache, t) for t in inputs if t is not None):
-            raise ValueError("k_cache overlaps an input")
+        blocks, block_size = k_cache.shape[0], k_cache.shape[1]
+        if blocks == 0 or block_size == 0:
+            raise ValueError("k_cache is empty")
     if T == 0:
         return oq, out_kv
-    row = d_latent + d_rope
-    with _on_device(dev):
-        rc = capi.lib().xllm_mi355_mla_norm_rope_and_cache(
-            q_pe.data_ptr(), oq.data_ptr(), kv.data_ptr(), _ptr(out_kv), kv_norm_weight.data_ptr(), float(eps),
-            cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], position_ids.data_ptr(), _ptr(k_cache), _ptr(slot_mapping),
-            T, H, d_latent, d_rope, *_head_strides(q_pe), *_head_strides(oq), kv.stride(0) if T > 1 else row,
-            0 if out_kv is None else out_kv.stride(0) if T > 1 else row, 0 if k_cache is None else k_cache.shape[1],
-            0 if k_cache is None else k_cache.shape[0], 1 if interleave else 0, _dtype_code(q_pe),
-            _dtype_code(cos_sin_cache), _stream(dev))
-    capi.check(rc, "xllm_mi355_mla_norm_rope_and_cache")
+    kv_row = kv.stride(0) if T > 1 else row
+    if kv_row < row:
+        raise ValueError("kv: rows must not overlap")
+    if eps < 0:
+        raise ValueError("eps must not be negative")
+    rc = _launch(dev, "xllm_mi355_mla_norm_rope_and_cache", q_pe.data_ptr(), oq.data_ptr(), kv.data_ptr(), _ptr(out_kv),
+                 kv_norm_weight.data_ptr(), float(eps), cos_sin_cache.data_ptr(), cos_sin_cache.shape[0],
+                 position_ids.data_ptr(), _ptr(k_cache), _ptr(slot_mapping), T, H, d_latent, d_rope, q_st[0], q_st[1],
+                 oq_st[0], oq_st[1], kv_row, out_row, block_size, blocks, 1 if interleave else 0, _dtype_code(q_pe),
+                 _dtype_code(cos_sin_cache))
+    _check_launch(rc, "xllm_mi355_mla_norm_rope_and_cache",
+                  "a result of mla_norm_rope_and_cache overlaps itself, another one or an input (in place means the operand itself)")
     return oq, out_kv
 
 
 # ------------------------------------------------------------------------------------------
 # differential attention
+
+@functools.lru_cache(maxsize=256)
+def _diff_workspace_bytes(dev, n_heads, n_pairs, head_dim):
+    with torch.cuda.device(dev):   # (the size goes by the device's compute units)
+        return int(capi.lib().xllm_mi355_paged_decode_diff_workspace_bytes(n_heads, n_pairs, head_dim))
+
 
 def batch_decode_diff(query, k_cache, v_cache, output, block_table, seq_lens, lambda_, scale=None, norm_weight=None,
                       eps=1e-5, out_scale=1.0, window_left=-1):
@@ -1187,30 +1183,38 @@ def batch_decode_diff(query, k_cache, v_cache, output, block_table, seq_lens, la
     weight as float32, one value, [H], or [B, H].  norm_weight [2 D] of query's dtype; out_scale: usually 1 - lambda_init.
     window_left >= 0: the last window_left + 1 tokens only.  bfloat16 or float16; D 64 or 128.  Returns output."""
     dev = _require_cuda(query, k_cache, v_cache, output, block_table, seq_lens, lambda_, norm_weight)
+    dtype = query.dtype
     if query.dim() != 3 or query.shape[1] % 2 != 0 or query.shape[1] == 0:
         raise ValueError("query must be [B, 2 H, D]")
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise TypeError("query must be bfloat16 or float16")
     B, H2, D = query.shape
     H = H2 // 2
-    if query.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError("query must be bfloat16 or float16")
-    if not (query.stride(2) == 1 and query.stride(1) == D):
+    q_row, q_head, q_elem = query.stride()
+    if q_elem != 1 or q_head != D:
         raise ValueError("query: last two dims must be contiguous")
-    if tuple(output.shape) != (B, H, 2 * D) or output.dtype != query.dtype or \
-            not (output.stride(2) == 1 and (H == 1 or output.stride(1) == 2 * D)):
-        raise ValueError("output must be [B, H, 2 D] of query's dtype with contiguous last two dims")
-    if k_cache.dim() != 4 or k_cache.shape[2] % 2 != 0 or k_cache.shape[2] == 0 or k_cache.shape[3] != D or \
-            not k_cache.is_contiguous():
+    if output.dim() != 3 or output.dtype != dtype or tuple(output.shape) != (B, H, 2 * D):
+        raise ValueError("output must be [B, H, 2 D] of query's dtype")
+    o_row, o_head, o_elem = output.stride()
+    if o_elem != 1 or (H > 1 and o_head != 2 * D) or (B > 1 and o_row < H2 * D):
+        raise ValueError("output: last two dims must be contiguous and rows apart")
+    if k_cache.dim() != 4 or not k_cache.is_contiguous():
         raise ValueError("k_cache must be contiguous [P, bs, 2 pairs, D]")
-    P, bs, pairs = k_cache.shape[0], k_cache.shape[1], k_cache.shape[2] // 2
+    P, bs, k_heads, k_dim = k_cache.shape
+    pairs = k_heads // 2
+    if k_heads % 2 != 0 or k_dim != D or P == 0 or bs == 0 or pairs == 0:
+        raise ValueError("k_cache must be contiguous [P, bs, 2 pairs, D]")
     if tuple(v_cache.shape) != (P, bs, pairs, 2 * D) or not v_cache.is_contiguous():
         raise ValueError("v_cache must be contiguous [P, bs, pairs, 2 D]")
-    if k_cache.dtype != query.dtype or v_cache.dtype != query.dtype:
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise TypeError("the caches must have query's dtype")
     if H % pairs != 0:
         raise ValueError("the heads must be a multiple of the KV pairs")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or \
-            block_table.shape[0] != B:
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or \
+            block_table.shape[1] == 0 or block_table.stride(1) != 1:
         raise ValueError("block_table must be int32 [B, W] with unit column stride, one row per sequence")
+    W = block_table.shape[1]
+    t_row = block_table.stride(0) if B > 1 else W
     if seq_lens.dtype != torch.int32 or seq_lens.numel() != B or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be contiguous int32 [B]")
     if lambda_.dtype != torch.float32:
@@ -1223,26 +1227,22 @@ def batch_decode_diff(query, k_cache, v_cache, output, block_table, seq_lens, la
         lam_b, lam_h = lambda_.stride()
     else:
         raise ValueError("lambda_ must hold one value, or be [H] or [B, H]")
-    if norm_weight is not None and (norm_weight.dtype != query.dtype or norm_weight.numel() != 2 * D or
+    if norm_weight is not None and (norm_weight.dtype != dtype or norm_weight.numel() != 2 * D or
                                     not norm_weight.is_contiguous()):
         raise ValueError("norm_weight must be contiguous [2 D] of query's dtype")
-    if B > 1 and output.stride(0) < 2 * H * D:
-        raise ValueError("output: rows must not overlap")
-    if any(_overlap(output, t) for t in (query, k_cache, v_cache, block_table, seq_lens, lambda_, norm_weight)):
-        raise ValueError("output overlaps an input")
     if scale is None:
         scale = D ** -0.5
+    if not scale > 0 or not eps >= 0:
+        raise ValueError("scale must be positive and eps not negative")
+    if t_row < W or (B > 1 and q_row < H2 * D):
+        raise ValueError("block_table and query: rows must not overlap")
     if B == 0:
         return output
-    lib = capi.lib()
-    with _on_device(dev):
-        # (a workspace of the call's own: calls on other streams and captured graphs never meet in it)
-        ws = torch.empty(max(1, lib.xllm_mi355_paged_decode_diff_workspace_bytes(H, pairs, D)), dtype=torch.uint8, device=dev)
-        rc = lib.xllm_mi355_paged_decode_diff(
-            query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), output.data_ptr(), block_table.data_ptr(),
-            max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], seq_lens.data_ptr(),
-            lambda_.data_ptr(), lam_b, lam_h, _ptr(norm_weight), float(eps), float(out_scale), B, H, pairs, D, bs, P,
-            query.stride(0) if B > 1 else H2 * D, output.stride(0) if B > 1 else H2 * D, int(window_left), float(scale),
-            ws.data_ptr(), ws.numel(), _dtype_code(query), _stream(dev))
-    capi.check(rc, "xllm_mi355_paged_decode_diff")
+    # (a workspace of the call's own: calls on other streams and captured graphs never meet in it)
+    ws = torch.empty(_diff_workspace_bytes(dev, H, pairs, D), dtype=torch.uint8, device=dev)
+    rc = _launch(dev, "xllm_mi355_paged_decode_diff", query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                 output.data_ptr(), block_table.data_ptr(), t_row, W, seq_lens.data_ptr(), lambda_.data_ptr(), lam_b, lam_h,
+                 _ptr(norm_weight), float(eps), float(out_scale), B, H, pairs, D, bs, P, q_row if B > 1 else H2 * D,
+                 o_row if B > 1 else H2 * D, int(window_left), float(scale), ws.data_ptr(), ws.numel(), _dtype_code(query))
+    _check_launch(rc, "xllm_mi355_paged_decode_diff", "output overlaps an input")
     return output
