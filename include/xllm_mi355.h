@@ -568,7 +568,7 @@ int xllm_mi355_decode_metadata_update(const int32_t* src_tokens, const int32_t* 
  *                   table's width ran out): their slots are -1, and their requests must not attend before they are stored
  * A slot that would not fit 31 bits, or whose kept entry is negative, is -1 as well.  Outputs must not overlap kv_lens,
  * new_lens, free_pages or free_head.  max_new_tokens, n_free, table_width and block_size below 2^30, batch up to 2^20.
- * One launch for up to 1024 requests, two beyond; integer arithmetic only, the same result every time.
+ * One launch for up to 4096 requests, two beyond; integer arithmetic only, the same result every time.
  */
 int xllm_mi355_build_step_tables(const int32_t* kv_lens, const int32_t* new_lens,
                                  const int32_t* block_table_in, int64_t in_stride,

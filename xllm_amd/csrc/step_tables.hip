@@ -22,10 +22,15 @@ namespace xllm_mi355 {
 
 namespace {
 
-constexpr int kStepThreads = 256;
-constexpr int kStepWaves = kStepThreads / kWave;
-constexpr int kFusedBatch = 4096;        // 2 sums of up to 16 KB in LDS
-constexpr int kStepCells = 1024;         // tokens, or table entries, of a workgroup
+// Requests of the one-launch forms: a thread holds a run of them in registers.  Workgroups of 256 threads up to 256
+// requests, whose barriers are cheaper (64 decode rows: 3.3 us, with 1024 threads 5.8 us; 256 rows: 3.8 and 6.0 us); of
+// 1024 threads beyond; two launches where the sums no longer fit LDS (1024 rows: 6.2 us in one launch, 15 us in two; 4096
+// rows: 9.2 and 21 us).
+constexpr int kSmallThreads = 256, kSmallRun = 1;
+constexpr int kLargeThreads = 1024, kLargeRun = 4;
+constexpr int kFusedBatch = kLargeThreads * kLargeRun;   // 3 arrays of up to 16 KB in LDS
+constexpr int kStepCells = 1024;         // tokens of a piece
+constexpr int kStepCols = 8;             // table entries of a lane, their loads in flight together
 
 struct StepArgs {
   const int32_t* kv_lens;
@@ -42,9 +47,9 @@ struct StepArgs {
   int32_t* counters;
   int64_t in_stride, out_stride;
   int batch, width, block_size, bs_shift, budget, n_free;
-  int token_blocks;           // workgroups of the tokens, the first ones of the grid
-  int col_blocks;             // workgroups per table row
-  int rows_per_block;         // table rows of a workgroup when they are short
+  int token_pieces;           // pieces of the tokens, the first ones; then those of the table
+  int segments;               // of a table row; a wavefront takes one
+  int segment_cols;           // at most kWave * kStepCols
 };
 
 // Column of a position, and min(C(tokens), W).  (32-bit division: a context and the tokens of a step are below 2^32.)
@@ -66,13 +71,14 @@ __device__ __forceinline__ int step_new(const StepArgs& a, int b) { return max(0
 template <int WAVES>
 __device__ __forceinline__ int saturating_scan(int v, int cap, int& all, int* tmp) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int t = __shfl_up(v, d, kWave);
-    if (lane >= d) v = min(v + t, cap);
-  }
-  int excl = __shfl_up(v, 1, kWave);
-  if (lane == 0) excl = 0;
+  // inside the wavefront by lane moves: rows of 16 lanes first, then the rows' last lanes into the rows behind them
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false), cap);   // row_shr:1
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false), cap);   // row_shr:2
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false), cap);   // row_shr:4
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false), cap);   // row_shr:8
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false), cap);   // row_bcast:15 into rows 1 and 3
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false), cap);   // row_bcast:31 into rows 2 and 3
+  int excl = __builtin_amdgcn_update_dpp(0, v, 0x138, 0xf, 0xf, false);          // wave_shr:1
   __syncthreads();   // (tmp may still be read from the scan before)
   if (lane == kWave - 1) tmp[wave] = v;
   __syncthreads();
@@ -86,8 +92,7 @@ __device__ __forceinline__ int saturating_scan(int v, int cap, int& all, int* tm
   return excl;
 }
 
-// Both sums over the batch into cu[0 .. batch] and indptr[0 .. batch] (LDS or global memory).  A thread takes a run of
-// requests, so that there are two scans whatever the batch.
+// Both sums over the batch into cu[0 .. batch] and indptr[0 .. batch], in global memory and any length of batch.
 template <int WAVES>
 __device__ __forceinline__ void step_sums(const StepArgs& a, int32_t* cu, int32_t* indptr, int* tmp) {
   const int tid = threadIdx.x;
@@ -123,6 +128,50 @@ __device__ __forceinline__ void step_sums(const StepArgs& a, int32_t* cu, int32_
   __syncthreads();
 }
 
+// The same into LDS, with the pages that each request keeps: a thread's RUN requests stay in registers, so that the
+// lengths are read once.
+template <int THREADS, int RUN>
+__device__ __forceinline__ void step_sums_lds(const StepArgs& a, int32_t* cu, int32_t* indptr, int32_t* old, int* tmp) {
+  const int tid = threadIdx.x, lo = tid * RUN;
+  int n[RUN], need[RUN];
+  u32 kv[RUN];
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) {
+    const bool on = lo + i < a.batch;
+    n[i] = on ? step_new(a, lo + i) : 0;
+    kv[i] = on ? step_kv(a, lo + i) : 0;
+  }
+  const int pages_left = a.n_free - step_head(a);
+  int all, sum = 0;
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) sum = min(sum + n[i], a.budget);
+  int c = saturating_scan<THREADS / kWave>(sum, a.budget, all, tmp);
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) {
+    const int e = min(c + n[i], a.budget);
+    const int keep = step_pages(a, kv[i]);
+    need[i] = step_pages(a, kv[i] + (e - c)) - keep;
+    sum = min(sum + need[i], pages_left);
+    if (lo + i < a.batch) {
+      cu[lo + i + 1] = e;
+      old[lo + i] = keep;
+    }
+    c = e;
+  }
+  int p = saturating_scan<THREADS / kWave>(sum, pages_left, all, tmp);
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) {
+    p = min(p + need[i], pages_left);
+    if (lo + i < a.batch) indptr[lo + i + 1] = p;
+  }
+  if (tid == 0) {
+    cu[0] = 0;
+    indptr[0] = 0;
+  }
+  __syncthreads();
+}
+
 __device__ __forceinline__ int request_of(const int32_t* cu, int batch, int token) {   // cu[b] <= token < cu[b + 1]
   int lo = 0, hi = batch - 1;
   while (lo < hi) {
@@ -133,12 +182,12 @@ __device__ __forceinline__ int request_of(const int32_t* cu, int batch, int toke
   return lo;
 }
 
-// Entry j of request b's row; what lies behind its pages is -1.
-__device__ __forceinline__ int step_entry(const StepArgs& a, const int32_t* cu, const int32_t* indptr, int b, int j, int old,
-                                          int head) {
-  if (j < old) return a.table_in[b * a.in_stride + j];
-  const int p = indptr[b] + (j - old);
-  return p < indptr[b + 1] ? a.free_pages[head + p] : -1;
+// Where entry j of request b's row comes from; null: the entry is -1.
+__device__ __forceinline__ const int32_t* step_source(const StepArgs& a, const int32_t* cu, const int32_t* indptr, int b, int j,
+                                                      int keep, int head) {
+  const int p = indptr[b] + (j - keep);
+  const int32_t* src = p < indptr[b + 1] ? a.free_pages + head + p : nullptr;
+  return j < keep ? a.table_in + b * a.in_stride + j : src;
 }
 
 // What the first workgroup adds: lengths, sums and counters in the caller's arrays.
@@ -176,26 +225,23 @@ __global__ __launch_bounds__(1024) void step_sums_kernel(StepArgs a) {
   step_outputs<1024>(a, a.cu, a.indptr, false, tmp);
 }
 
-template <bool FUSED>
-__global__ __launch_bounds__(kStepThreads) void step_tables_kernel(StepArgs a) {
-  extern __shared__ int32_t lds[];
-  __shared__ int tmp[kStepWaves];
-  const int32_t *cu = a.cu, *indptr = a.indptr;
-  if constexpr (FUSED) {
-    int32_t* c = lds;
-    int32_t* p = lds + a.batch + 1;
-    step_sums<kStepWaves>(a, c, p, tmp);
-    cu = c;
-    indptr = p;
-    if (blockIdx.x == 0) step_outputs<kStepThreads>(a, c, p, true, tmp);
-  }
+template <int THREADS>
+__host__ __device__ __forceinline__ int64_t step_pieces(const StepArgs& a) {
+  const int64_t units = static_cast<int64_t>(a.batch) * a.segments;
+  return a.token_pieces + (units + THREADS / kWave - 1) / (THREADS / kWave);
+}
+
+// One piece of the tokens, or of the table.  OLD: the pages that the requests keep are in `old`.
+template <int THREADS, bool OLD>
+__device__ __forceinline__ void step_piece(const StepArgs& a, int64_t piece, const int32_t* cu, const int32_t* indptr,
+                                           const int32_t* old, int head) {
   const int tid = threadIdx.x;
-  const int head = step_head(a);
-  if (static_cast<int>(blockIdx.x) < a.token_blocks) {
+  auto kept = [&](int b) { return OLD ? old[b] : step_pages(a, step_kv(a, b)); };
+  if (piece < a.token_pieces) {
     const int n_tokens = cu[a.batch];
 #pragma unroll
-    for (int k = 0; k < kStepCells / kStepThreads; ++k) {
-      const int i = static_cast<int>(blockIdx.x) * kStepCells + k * kStepThreads + tid;
+    for (int k = 0; k < kStepCells / THREADS; ++k) {
+      const int i = static_cast<int>(piece) * kStepCells + k * THREADS + tid;
       if (i >= a.budget) continue;
       int64_t pos = 0;
       int slot = -1;
@@ -205,7 +251,8 @@ __global__ __launch_bounds__(kStepThreads) void step_tables_kernel(StepArgs a) {
         pos = kv + static_cast<u32>(i - cu[b]);
         const u32 col = step_column(a, static_cast<u32>(pos));
         if (col < static_cast<u32>(a.width)) {
-          const int64_t page = step_entry(a, cu, indptr, b, static_cast<int>(col), step_pages(a, kv), head);
+          const int32_t* src = step_source(a, cu, indptr, b, static_cast<int>(col), kept(b), head);
+          const int64_t page = src != nullptr ? *src : -1;
           const int64_t s = page * a.block_size + (pos - static_cast<int64_t>(col) * a.block_size);
           if (page >= 0 && s <= 0x7fffffffLL) slot = static_cast<int>(s);
         }
@@ -215,20 +262,61 @@ __global__ __launch_bounds__(kStepThreads) void step_tables_kernel(StepArgs a) {
     }
     return;
   }
-  // a piece of the table: part of a long row, or several short rows
+  // A wavefront per segment of a row: the request and its pages are the same in all lanes, which leaves a comparison and
+  // a load per entry (with a lane per entry of the flat table the divisions and look-ups were most of the launch: 13.6 us
+  // for 2 M entries).  The lanes' loads are issued before the first is used: an entry without a source reads the row's
+  // first one, so that no load hangs off a branch.
   const bool in_place = a.table_in == a.table_out;
-  const int t = static_cast<int>(blockIdx.x) - a.token_blocks;
-  const int b0 = t / a.col_blocks * a.rows_per_block;
-  const int c0 = t % a.col_blocks * kStepCells;
-  const int rows = min(a.rows_per_block, a.batch - b0);
-  const int cols = min(a.width - c0, kStepCells);
-  for (int i = tid; i < rows * cols; i += kStepThreads) {
-    const int r = i / cols;
-    const int b = b0 + r, j = c0 + i - r * cols;
-    const int old = step_pages(a, step_kv(a, b));
-    if (in_place && j < old) continue;
-    a.table_out[b * a.out_stride + j] = step_entry(a, cu, indptr, b, j, old, head);
+  const int64_t unit = (piece - a.token_pieces) * (THREADS / kWave) + __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int lane = tid & (kWave - 1);
+  const int64_t row_of = unit <= 0x7fffffffLL ? static_cast<u32>(unit) / static_cast<u32>(a.segments) : unit / a.segments;
+  if (row_of >= a.batch) return;
+  const int b = static_cast<int>(row_of);
+  const int c0 = static_cast<int>(unit - row_of * a.segments) * a.segment_cols, c1 = min(a.width, c0 + a.segment_cols);
+  const int keep = __builtin_amdgcn_readfirstlane(kept(b));
+  const int first = __builtin_amdgcn_readfirstlane(indptr[b]);
+  const int end = keep + __builtin_amdgcn_readfirstlane(indptr[b + 1]) - first;   // entries from here on are -1
+  const int32_t* row = a.table_in + b * a.in_stride;
+  const int32_t* fresh = a.free_pages + head + first - keep;
+  int32_t* out = a.table_out + b * a.out_stride;
+  int32_t value[kStepCols];
+#pragma unroll
+  for (int k = 0; k < kStepCols; ++k) {
+    const int j = c0 + k * kWave + lane;
+    const bool old = j < keep && j < c1 && !in_place;
+    const int32_t* src = old ? row + j : row;
+    src = j >= keep && j < end && j < c1 ? fresh + j : src;
+    value[k] = c0 + k * kWave < min(c1, end) ? *src : -1;
   }
+#pragma unroll
+  for (int k = 0; k < kStepCols; ++k) {
+    const int j = c0 + k * kWave + lane;
+    if (j < c1 && !(in_place && j < keep)) out[j] = j < end ? value[k] : -1;
+  }
+}
+
+template <int THREADS, int RUN>
+__global__ __launch_bounds__(THREADS) void step_tables_kernel(StepArgs a) {
+  extern __shared__ int32_t lds[];
+  __shared__ int tmp[THREADS / kWave];
+  int32_t* cu = lds;
+  int32_t* indptr = cu + a.batch + 1;
+  int32_t* old = indptr + a.batch + 1;
+  step_sums_lds<THREADS, RUN>(a, cu, indptr, old, tmp);
+  if (blockIdx.x == 0) {   // (a workgroup of its own for the per-request outputs: with pieces on top it would end last)
+    step_outputs<THREADS>(a, cu, indptr, true, tmp);
+    return;
+  }
+  const int head = step_head(a);
+  const int64_t n = step_pieces<THREADS>(a);
+  for (int64_t p = blockIdx.x - 1; p < n; p += gridDim.x - 1) step_piece<THREADS, true>(a, p, cu, indptr, old, head);
+}
+
+__global__ __launch_bounds__(kSmallThreads) void step_tables_from_sums_kernel(StepArgs a) {
+  const int head = step_head(a);
+  const int64_t n = step_pieces<kSmallThreads>(a);
+  for (int64_t p = blockIdx.x; p < n; p += gridDim.x)
+    step_piece<kSmallThreads, false>(a, p, a.cu, a.indptr, nullptr, head);
 }
 
 }  // namespace
@@ -289,20 +377,27 @@ int build_step_tables(const int32_t* kv_lens, const int32_t* new_lens, const int
     if ((1LL << s) == block_size) a.bs_shift = s;
   a.budget = static_cast<int>(max_new_tokens);
   a.n_free = static_cast<int>(n_free);
-  a.token_blocks = static_cast<int>((max_new_tokens + kStepCells - 1) / kStepCells);
-  a.col_blocks = static_cast<int>((table_width + kStepCells - 1) / kStepCells);
-  a.rows_per_block = table_width >= kStepCells ? 1 : static_cast<int>(kStepCells / table_width);
-  const int64_t table_blocks = (batch + a.rows_per_block - 1) / a.rows_per_block * a.col_blocks;
-  if (a.token_blocks + table_blocks > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
-  const dim3 grid(static_cast<unsigned>(a.token_blocks + table_blocks));
+  a.token_pieces = static_cast<int>((max_new_tokens + kStepCells - 1) / kStepCells);
+  a.segments = static_cast<int>((table_width + kWave * kStepCols - 1) / (kWave * kStepCols));
+  a.segment_cols = static_cast<int>((table_width + a.segments - 1) / a.segments);
+  // Every workgroup of the one-launch forms makes the sums for itself, so there are no more of them than run at once: one
+  // per CU of 1024 threads (2048 requests, 2 M table entries, 65536 tokens: 9.8 us, of which the sums are 5; with two per
+  // CU 13 us; with one per piece of work 91 us).
+  const int cus = device_cu_count();
+  const size_t lds = static_cast<size_t>(3 * batch + 2) * 4;
+  auto grid = [](int64_t groups, int64_t most) { return dim3(static_cast<unsigned>(groups < most ? groups : most)); };
+  if (batch <= kSmallThreads * kSmallRun) {
+    step_tables_kernel<kSmallThreads, kSmallRun><<<grid(step_pieces<kSmallThreads>(a) + 1, 8LL * cus), kSmallThreads, lds, stream>>>(a);
+    return static_cast<int>(hipGetLastError());
+  }
   if (batch <= kFusedBatch) {
-    step_tables_kernel<true><<<grid, kStepThreads, (2 * batch + 2) * 4, stream>>>(a);
+    step_tables_kernel<kLargeThreads, kLargeRun><<<grid(step_pieces<kLargeThreads>(a) + 1, 1LL * cus), kLargeThreads, lds, stream>>>(a);
     return static_cast<int>(hipGetLastError());
   }
   step_sums_kernel<<<1, 1024, 0, stream>>>(a);
   const int rc = static_cast<int>(hipGetLastError());
   if (rc != 0) return rc;
-  step_tables_kernel<false><<<grid, kStepThreads, 0, stream>>>(a);
+  step_tables_from_sums_kernel<<<grid(step_pieces<kSmallThreads>(a), 16LL * cus), kSmallThreads, 0, stream>>>(a);
   return static_cast<int>(hipGetLastError());
 }
 
