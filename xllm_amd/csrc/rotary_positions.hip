@@ -79,38 +79,37 @@ struct Pack {
 
 // ---- cos | sin rows ------------------------------------------------------------------------------------------------
 
-// cos and sin of `angle` in 64 bits: the multiple of pi / 2 is taken off in two parts (its product with the leading part
-// is exact inside the fused multiply-add, so the remainder of angles up to 2^30 is good to 2^-52 of the quadrant), then
-// the Taylor polynomials on [-pi/4, pi/4], whose first omitted terms are below 2e-14 and 7e-16.
-__device__ __forceinline__ void cos_sin_64(double angle, double& c, double& s) {
+// factor * cos and factor * sin of `angle`, in 64 bits up to the one rounding to fp32: the multiple of pi / 2 is taken off
+// in two parts (its product with the leading part is exact inside the fused multiply-add, so what is left of angles up to
+// 2^50 is good to 2^-52 of the angle), then the Taylor polynomials on [-pi/4, pi/4], whose first omitted terms are below
+// 8e-12 and 2e-10, a two-hundredth of half an fp32 step.  Quadrant and signs are settled on the rounded results:
+// comparisons in 64 bits were a fifth of the operations.
+__device__ __forceinline__ void cos_sin_64(double angle, double factor, float& c, float& s) {
   const double q = __builtin_rint(angle * 0.63661977236758134308);
   double r = __builtin_fma(-q, 1.5707963267948965580, angle);
   r = __builtin_fma(-q, 6.1232339957367660359e-17, r);
   const double z = r * r;
-  double ps = 1.0 / 6227020800.0;
-  ps = __builtin_fma(ps, z, -1.0 / 39916800.0);
+  double ps = -1.0 / 39916800.0;
   ps = __builtin_fma(ps, z, 1.0 / 362880.0);
   ps = __builtin_fma(ps, z, -1.0 / 5040.0);
   ps = __builtin_fma(ps, z, 1.0 / 120.0);
   ps = __builtin_fma(ps, z, -1.0 / 6.0);
-  const double sr = __builtin_fma(r * z, ps, r);
-  double pc = -1.0 / 87178291200.0;
-  pc = __builtin_fma(pc, z, 1.0 / 479001600.0);
-  pc = __builtin_fma(pc, z, -1.0 / 3628800.0);
+  const float sr = static_cast<float>(__builtin_fma(r * z, ps, r) * factor);
+  double pc = -1.0 / 3628800.0;
   pc = __builtin_fma(pc, z, 1.0 / 40320.0);
   pc = __builtin_fma(pc, z, -1.0 / 720.0);
   pc = __builtin_fma(pc, z, 1.0 / 24.0);
   pc = __builtin_fma(pc, z, -0.5);
-  const double cr = __builtin_fma(pc, z, 1.0);
-  // the quadrant, q mod 4, without going through an integer that q may not fit
-  const double k = q - 4.0 * __builtin_floor(q * 0.25);
-  const bool swap = k == 1.0 || k == 3.0;
-  c = swap ? sr : cr;
-  s = swap ? cr : sr;
-  if (k == 1.0 || k == 2.0) c = -c;
-  if (k >= 2.0) s = -s;
+  const float cr = static_cast<float>(__builtin_fma(pc, z, 1.0) * factor);
+  // the quadrant, q mod 4 (taken before it becomes an integer, which q may not fit)
+  const u32 k = static_cast<u32>(static_cast<int>(__builtin_fma(-4.0, __builtin_floor(q * 0.25), q)));
+  const bool swap = (k & 1u) != 0;
+  c = as_f32(as_u32(swap ? sr : cr) ^ ((k + 1u) & 2u) << 30);
+  s = as_f32(as_u32(swap ? cr : sr) ^ (k & 2u) << 30);
 }
 
+// Bound by the stores of the rows and, on top of them, by the operations in 64 bits: 131072 rows of 128 fp32 values (67 MB)
+// take 16.2 us, the stores alone 11.9 us (a plain fill of as many bytes 11.4 us).
 // One lane makes V consecutive pairs of a row: V cosines and V sines, 16 bytes of each where the row allows it.
 template <int DT, int V>
 __global__ __launch_bounds__(kRotThreads) void rope_cos_sin_kernel(const double* inv_freq, const int64_t* positions,
@@ -126,12 +125,7 @@ __global__ __launch_bounds__(kRotThreads) void rope_cos_sin_kernel(const double*
   typename Elem<DT>::T* p = out + row * (2 * static_cast<int64_t>(half)) + i0;
   float c[V], s[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    double cd, sd;
-    cos_sin_64(pos * inv_freq[i0 + i], cd, sd);
-    c[i] = static_cast<float>(cd * factor);
-    s[i] = static_cast<float>(sd * factor);
-  }
+  for (int i = 0; i < V; ++i) cos_sin_64(pos * inv_freq[i0 + i], factor, c[i], s[i]);
   if constexpr (V == 1) {
     p[0] = Elem<DT>::put(c[0]);
     p[half] = Elem<DT>::put(s[0]);
@@ -184,8 +178,6 @@ struct RotArgs {
   int rot;                  // rotated dims R
   int rot_units;            // lanes per head and rotated part
   int units;                // lanes per head: the rotated part, and for out of place the rest of the wider side
-  int slots;                // groups of U heads per token: those of q, then those of k
-  int q_slots;
 };
 
 // cos and sin of pairs [i, i + P) of a table row.
@@ -211,55 +203,73 @@ __device__ __forceinline__ void rot_row(const char* table, int64_t row, int rot,
   }
 }
 
-// A lane owns P pairs (P = 16 bytes of elements, so two 16-byte words: the pairs' two halves, or two neighbouring words
-// when interleaved) of U consecutive heads of a token: one set of cosines and sines serves all of them.  Lanes behind the
-// rotated part copy the rest of the head, 2 P elements each, when the result goes elsewhere.
+// P pairs in two 16-byte words: their first and second elements, or P / 2 pairs in each word when interleaved.
+template <int DT, int P, bool INTERLEAVE>
+__device__ __forceinline__ void turn_words(Pack<DT, P>& x, Pack<DT, P>& y, const float (&c)[P], const float (&s)[P]) {
+  if constexpr (INTERLEAVE) {
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      Pack<DT, P>& w = j < P / 2 ? x : y;
+      const int e = j < P / 2 ? j : j - P / 2;
+      const float p0 = w.get(2 * e), p1 = w.get(2 * e + 1);
+      w.put2(e, __builtin_fmaf(p0, c[j], -(p1 * s[j])), __builtin_fmaf(p1, c[j], p0 * s[j]));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; j += 2) {
+      const float a0 = x.get(j), a1 = x.get(j + 1), b0 = y.get(j), b1 = y.get(j + 1);
+      x.put2(j / 2, __builtin_fmaf(a0, c[j], -(b0 * s[j])), __builtin_fmaf(a1, c[j + 1], -(b1 * s[j + 1])));
+      y.put2(j / 2, __builtin_fmaf(b0, c[j], a0 * s[j]), __builtin_fmaf(b1, c[j + 1], a1 * s[j + 1]));
+    }
+  }
+}
+
+// A lane owns P pairs of a head (P = 16 bytes of elements, so two 16-byte words: the pairs' two halves, or two neighbouring
+// words when interleaved).  Lanes behind the rotated part copy the rest of the head when the result goes elsewhere, two
+// words each, at neighbouring words in neighbouring lanes.  One head per lane: with four (one set of cosines and sines for
+// all of them, four times the bytes in flight per lane) 8192 tokens of 40 heads took the same 27 us, 4097 tokens of 20
+// heads with a copied rest 28 instead of 19 us, for want of wavefronts.
 // VEC = false takes one pair (or two elements to copy) per lane, for operands that are not aligned to 16 bytes.
-template <int DT, int CT, bool INTERLEAVE, bool VEC, int U>
+template <int DT, int CT, bool INTERLEAVE, bool VEC>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a, float sin_sign) {
   using T = typename Elem<DT>::T;
   constexpr int P = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
   const int64_t idx = static_cast<int64_t>(blockIdx.x) * kRotThreads + threadIdx.x;
   if (idx >= a.n_units) return;
-  int64_t rest, token;
-  int unit, slot;
+  const int heads = a.q.heads + a.k.heads;
+  int64_t token;
+  int unit, head;
   if (a.n_units <= 0x7fffffffLL) {
     const u32 r = static_cast<u32>(idx) / static_cast<u32>(a.units);
     unit = static_cast<int>(static_cast<u32>(idx) - r * static_cast<u32>(a.units));
-    const u32 t = r / static_cast<u32>(a.slots);
-    slot = static_cast<int>(r - t * static_cast<u32>(a.slots));
+    const u32 t = r / static_cast<u32>(heads);
+    head = static_cast<int>(r - t * static_cast<u32>(heads));
     token = t;
   } else {
-    rest = idx / a.units;
-    unit = static_cast<int>(idx - rest * a.units);
-    token = rest / a.slots;
-    slot = static_cast<int>(rest - token * a.slots);
+    const int64_t r = idx / a.units;
+    unit = static_cast<int>(idx - r * a.units);
+    token = r / heads;
+    head = static_cast<int>(r - token * heads);
   }
-  const bool is_q = slot < a.q_slots;
+  const bool is_q = head < a.q.heads;
   const RotSide& sd = is_q ? a.q : a.k;
-  const int head0 = (is_q ? slot : slot - a.q_slots) * U;
-  const T* in = reinterpret_cast<const T*>(sd.in) + token * sd.in_token + head0 * sd.in_head;
-  T* out = reinterpret_cast<T*>(sd.out) + token * sd.out_token + head0 * sd.out_head;
-  const int64_t in_head = sd.in_head, out_head = sd.out_head;
-  const int heads = min(U, sd.heads - head0);
+  if (!is_q) head -= a.q.heads;
+  const T* in = reinterpret_cast<const T*>(sd.in) + token * sd.in_token + head * sd.in_head;
+  T* out = reinterpret_cast<T*>(sd.out) + token * sd.out_token + head * sd.out_head;
 
   if (unit >= a.rot_units) {   // the rest of the head: what lies before the rotated part, then what lies behind it
-    const int e0 = (unit - a.rot_units) * 2 * P;
+    if (sd.in == sd.out) return;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      const int e = e0 + w * P;
+      const int e = (unit - a.rot_units + w * (a.units - a.rot_units)) * P;
       if (e >= sd.dim - a.rot) break;
       const int d = e < sd.offset ? e : e + a.rot;
       if constexpr (VEC) {
-        Pack<DT, P> x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (u < heads) x[u].load(in + u * in_head + d);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (u < heads) x[u].store(out + u * out_head + d);
+        Pack<DT, P> x;
+        x.load(in + d);
+        x.store(out + d);
       } else {
-        for (int u = 0; u < heads; ++u) out[u * out_head + d] = in[u * in_head + d];
+        out[d] = in[d];
       }
     }
     return;
@@ -268,95 +278,54 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a, float si
   const int i = unit * P;                                                    // first pair
   const int da = sd.offset + (INTERLEAVE ? 2 * i : i);                       // where the pairs' words lie
   const int db = sd.offset + (INTERLEAVE ? 2 * i + P : i + a.rot / 2);
+  const int64_t pos = a.positions[token];
+  const bool turn = pos >= 0 && pos < a.n_positions;
   if constexpr (VEC) {
-    Pack<DT, P> x[U], y[U];
+    Pack<DT, P> x, y;
+    x.load(in + da);
+    y.load(in + db);
+    if (turn) {
+      float c[P], s[P];
+      rot_row<CT, P, true>(a.cos_sin, pos, a.rot, i, c, s);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (u < heads) {
-        x[u].load(in + u * in_head + da);
-        y[u].load(in + u * in_head + db);
-      }
-    const int64_t pos = a.positions[token];
-    float c[P], s[P];
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-      c[j] = 1.0f;
-      s[j] = 0.0f;
+      for (int j = 0; j < P; ++j) s[j] *= sin_sign;
+      turn_words<DT, P, INTERLEAVE>(x, y, c, s);
     }
-    const bool turn = pos >= 0 && pos < a.n_positions;
-    if (turn) rot_row<CT, P, true>(a.cos_sin, pos, a.rot, i, c, s);
-#pragma unroll
-    for (int j = 0; j < P; ++j) s[j] *= sin_sign;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (u >= heads) continue;
-      if (turn) {
-        if constexpr (INTERLEAVE) {
-#pragma unroll
-          for (int j = 0; j < P; ++j) {
-            Pack<DT, P>& w = j < P / 2 ? x[u] : y[u];
-            const int e = j < P / 2 ? j : j - P / 2;
-            const float p0 = w.get(2 * e), p1 = w.get(2 * e + 1);
-            w.put2(e, __builtin_fmaf(p0, c[j], -(p1 * s[j])), __builtin_fmaf(p1, c[j], p0 * s[j]));
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < P; j += 2) {
-            const float a0 = x[u].get(j), a1 = x[u].get(j + 1), b0 = y[u].get(j), b1 = y[u].get(j + 1);
-            x[u].put2(j / 2, __builtin_fmaf(a0, c[j], -(b0 * s[j])), __builtin_fmaf(a1, c[j + 1], -(b1 * s[j + 1])));
-            y[u].put2(j / 2, __builtin_fmaf(b0, c[j], a0 * s[j]), __builtin_fmaf(b1, c[j + 1], a1 * s[j + 1]));
-          }
-        }
-      }
-      x[u].store(out + u * out_head + da);
-      y[u].store(out + u * out_head + db);
-    }
+    x.store(out + da);
+    y.store(out + db);
   } else {
-    const int64_t pos = a.positions[token];
+    const T xa = in[da], xb = in[db];
     float c[1] = {1.0f}, s[1] = {0.0f};
-    const bool turn = pos >= 0 && pos < a.n_positions;
     if (turn) rot_row<CT, 1, false>(a.cos_sin, pos, a.rot, i, c, s);
     s[0] *= sin_sign;
-    for (int u = 0; u < heads; ++u) {
-      const T xa = in[u * in_head + da], xb = in[u * in_head + db];
-      const float p0 = Elem<DT>::get(xa), p1 = Elem<DT>::get(xb);
-      out[u * out_head + da] = turn ? Elem<DT>::put(__builtin_fmaf(p0, c[0], -(p1 * s[0]))) : xa;
-      out[u * out_head + db] = turn ? Elem<DT>::put(__builtin_fmaf(p1, c[0], p0 * s[0])) : xb;
-    }
+    const float p0 = Elem<DT>::get(xa), p1 = Elem<DT>::get(xb);
+    out[da] = turn ? Elem<DT>::put(__builtin_fmaf(p0, c[0], -(p1 * s[0]))) : xa;
+    out[db] = turn ? Elem<DT>::put(__builtin_fmaf(p1, c[0], p0 * s[0])) : xb;
   }
 }
 
-template <int DT, int CT, bool INTERLEAVE, bool VEC, int U>
+template <int DT, int CT, bool INTERLEAVE, bool VEC>
 int launch_rotary(RotArgs a, bool copy_rest, int inverse, int64_t n_tokens, hipStream_t stream) {
   constexpr int P = VEC ? 16 / static_cast<int>(sizeof(typename Elem<DT>::T)) : 1;
   a.rot_units = a.rot / 2 / P;
   const int wide = a.k.heads > 0 && a.k.dim > a.q.dim ? a.k.dim : a.q.dim;
   a.units = a.rot_units + (copy_rest ? (wide - a.rot + 2 * P - 1) / (2 * P) : 0);
-  a.q_slots = (a.q.heads + U - 1) / U;
-  a.slots = a.q_slots + (a.k.heads + U - 1) / U;
-  a.n_units = n_tokens * a.slots * a.units;
+  a.n_units = n_tokens * (a.q.heads + a.k.heads) * a.units;
   const int64_t groups = (a.n_units + kRotThreads - 1) / kRotThreads;
   if (groups > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
-  rotary_kernel<DT, CT, INTERLEAVE, VEC, U><<<dim3(static_cast<unsigned>(groups)), kRotThreads, 0, stream>>>(
+  rotary_kernel<DT, CT, INTERLEAVE, VEC><<<dim3(static_cast<unsigned>(groups)), kRotThreads, 0, stream>>>(
       a, inverse != 0 ? -1.0f : 1.0f);
   return static_cast<int>(hipGetLastError());
-}
-
-template <int DT, int CT, bool INTERLEAVE>
-int dispatch_rotary_units(const RotArgs& a, bool vec, bool copy_rest, int inverse, int64_t n_tokens, hipStream_t stream) {
-  if (!vec) return launch_rotary<DT, CT, INTERLEAVE, false, 1>(a, copy_rest, inverse, n_tokens, stream);
-  // one head per lane while that keeps the launch small (decode), four beyond: see the figures at rotary_embedding
-  if (n_tokens * (a.q.heads + a.k.heads) * a.rot < (1LL << 22))
-    return launch_rotary<DT, CT, INTERLEAVE, true, 1>(a, copy_rest, inverse, n_tokens, stream);
-  return launch_rotary<DT, CT, INTERLEAVE, true, 4>(a, copy_rest, inverse, n_tokens, stream);
 }
 
 template <int DT>
 int dispatch_rotary(const RotArgs& a, int cos_sin_dtype, int interleave, bool vec, bool copy_rest, int inverse,
                     int64_t n_tokens, hipStream_t stream) {
 #define XLLM_ROT(CT)                                                                                            \
-  (interleave != 0 ? dispatch_rotary_units<DT, CT, true>(a, vec, copy_rest, inverse, n_tokens, stream)          \
-                   : dispatch_rotary_units<DT, CT, false>(a, vec, copy_rest, inverse, n_tokens, stream))
+  (interleave != 0 ? (vec ? launch_rotary<DT, CT, true, true>(a, copy_rest, inverse, n_tokens, stream)          \
+                          : launch_rotary<DT, CT, true, false>(a, copy_rest, inverse, n_tokens, stream))        \
+                   : (vec ? launch_rotary<DT, CT, false, true>(a, copy_rest, inverse, n_tokens, stream)         \
+                          : launch_rotary<DT, CT, false, false>(a, copy_rest, inverse, n_tokens, stream)))
   switch (cos_sin_dtype) {
     case XLLM_MI355_FP32: return XLLM_ROT(XLLM_MI355_FP32);
     case XLLM_MI355_BF16: return XLLM_ROT(XLLM_MI355_BF16);
@@ -383,36 +352,15 @@ struct MlaPrologueArgs {
   int64_t n_tokens, n_positions, n_slots;
   int64_t q_token, q_head, q_out_token, q_out_head, kv_row, kv_out_row;
   int64_t q_units;           // lanes of the query part
-  int heads, head_slots;     // head_slots: groups of U heads
+  int heads;
   int kv_blocks;             // workgroups of the latent part, the first ones of the grid
   float eps;
 };
 
-// Eight pairs of one head's 64 rope dims: two 16-byte words (see rotary_kernel).
-template <int DT, bool INTERLEAVE>
-__device__ __forceinline__ void turn_words(Pack<DT, 8>& x, Pack<DT, 8>& y, const float (&c)[8], const float (&s)[8]) {
-  if constexpr (INTERLEAVE) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      Pack<DT, 8>& w = j < 4 ? x : y;
-      const int e = j & 3;
-      const float p0 = w.get(2 * e), p1 = w.get(2 * e + 1);
-      w.put2(e, __builtin_fmaf(p0, c[j], -(p1 * s[j])), __builtin_fmaf(p1, c[j], p0 * s[j]));
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const float a0 = x.get(j), a1 = x.get(j + 1), b0 = y.get(j), b1 = y.get(j + 1);
-      x.put2(j / 2, __builtin_fmaf(a0, c[j], -(b0 * s[j])), __builtin_fmaf(a1, c[j + 1], -(b1 * s[j + 1])));
-      y.put2(j / 2, __builtin_fmaf(b0, c[j], a0 * s[j]), __builtin_fmaf(b1, c[j + 1], a1 * s[j + 1]));
-    }
-  }
-}
-
 // The first kv_blocks workgroups take the tokens' latent rows, one wavefront per row: eight latent values per lane (one
 // 16-byte word), their sum of squares over the wavefront, and the rope part in lanes 0-3.  The others rotate the rope
-// part of the query heads, four lanes per head and U heads per lane.
-template <int DT, int CT, bool INTERLEAVE, int U>
+// part of the query heads, four lanes per head.
+template <int DT, int CT, bool INTERLEAVE>
 __global__ __launch_bounds__(kRotThreads) void mla_prologue_kernel(MlaPrologueArgs a) {
   constexpr int kUnits = kRopeDim / 16;
   if (static_cast<int>(blockIdx.x) < a.kv_blocks) {
@@ -446,7 +394,7 @@ __global__ __launch_bounds__(kRotThreads) void mla_prologue_kernel(MlaPrologueAr
     const float r = 1.0f / __builtin_sqrtf(ss * (1.0f / kLatent) + a.eps);
 #pragma unroll
     for (int j = 0; j < 4; ++j) x.put2(j, x.get(2 * j) * r * w.get(2 * j), x.get(2 * j + 1) * r * w.get(2 * j + 1));
-    if (turn) turn_words<DT, INTERLEAVE>(ra, rb, c, s);
+    if (turn) turn_words<DT, 8, INTERLEAVE>(ra, rb, c, s);
     if (a.kv_out != nullptr) {
       uint16_t* o = a.kv_out + token * a.kv_out_row;
       x.store(o + lane * 8);
@@ -469,56 +417,41 @@ __global__ __launch_bounds__(kRotThreads) void mla_prologue_kernel(MlaPrologueAr
   if (idx >= a.q_units) return;
   const int unit = static_cast<int>(idx & (kUnits - 1));
   const int64_t rest = idx / kUnits;
-  const int64_t token = a.q_units <= 0x7fffffffLL ? static_cast<u32>(rest) / static_cast<u32>(a.head_slots) : rest / a.head_slots;
-  const int head0 = static_cast<int>(rest - token * a.head_slots) * U;
-  const int heads = min(U, a.heads - head0);
+  const int64_t token = a.q_units <= 0x7fffffffLL ? static_cast<u32>(rest) / static_cast<u32>(a.heads) : rest / a.heads;
+  const int head = static_cast<int>(rest - token * a.heads);
   const int da = INTERLEAVE ? unit * 16 : unit * 8;
   const int db = INTERLEAVE ? unit * 16 + 8 : unit * 8 + kRopeDim / 2;
-  const uint16_t* in = a.q + token * a.q_token + head0 * a.q_head;
-  uint16_t* out = a.q_out + token * a.q_out_token + head0 * a.q_out_head;
-  Pack<DT, 8> x[U], y[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (u < heads) {
-      x[u].load(in + u * a.q_head + da);
-      y[u].load(in + u * a.q_head + db);
-    }
+  const uint16_t* in = a.q + token * a.q_token + head * a.q_head;
+  uint16_t* out = a.q_out + token * a.q_out_token + head * a.q_out_head;
+  Pack<DT, 8> x, y;
+  x.load(in + da);
+  y.load(in + db);
   const int64_t pos = a.positions[token];
-  const bool turn = pos >= 0 && pos < a.n_positions;
-  float c[8], s[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    c[j] = 1.0f;
-    s[j] = 0.0f;
+  if (pos >= 0 && pos < a.n_positions) {
+    float c[8], s[8];
+    rot_row<CT, 8, true>(a.cos_sin, pos, kRopeDim, unit * 8, c, s);
+    turn_words<DT, 8, INTERLEAVE>(x, y, c, s);
   }
-  if (turn) rot_row<CT, 8, true>(a.cos_sin, pos, kRopeDim, unit * 8, c, s);
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (u >= heads) continue;
-    if (turn) turn_words<DT, INTERLEAVE>(x[u], y[u], c, s);
-    x[u].store(out + u * a.q_out_head + da);
-    y[u].store(out + u * a.q_out_head + db);
-  }
+  x.store(out + da);
+  y.store(out + db);
 }
 
-template <int DT, int CT, bool INTERLEAVE, int U>
+template <int DT, int CT, bool INTERLEAVE>
 int launch_mla_prologue(MlaPrologueArgs a, hipStream_t stream) {
-  a.head_slots = (a.heads + U - 1) / U;
-  a.q_units = a.n_tokens * a.head_slots * (kRopeDim / 16);
+  a.q_units = a.n_tokens * a.heads * (kRopeDim / 16);
   const int64_t kv = (a.n_tokens + kRotThreads / kWave - 1) / (kRotThreads / kWave);
   const int64_t groups = kv + (a.q_units + kRotThreads - 1) / kRotThreads;
   if (groups > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
   a.kv_blocks = static_cast<int>(kv);
-  mla_prologue_kernel<DT, CT, INTERLEAVE, U><<<dim3(static_cast<unsigned>(groups)), kRotThreads, 0, stream>>>(a);
+  mla_prologue_kernel<DT, CT, INTERLEAVE><<<dim3(static_cast<unsigned>(groups)), kRotThreads, 0, stream>>>(a);
   return static_cast<int>(hipGetLastError());
 }
 
 template <int DT>
 int dispatch_mla_prologue(const MlaPrologueArgs& a, int interleave, int cos_sin_dtype, hipStream_t stream) {
-  const bool small = a.n_tokens * a.heads < 32768;   // one head per lane at decode sizes, four beyond
-#define XLLM_MLA_P(CT)                                                                                            \
-  (interleave != 0 ? (small ? launch_mla_prologue<DT, CT, true, 1>(a, stream) : launch_mla_prologue<DT, CT, true, 4>(a, stream)) \
-                   : (small ? launch_mla_prologue<DT, CT, false, 1>(a, stream) : launch_mla_prologue<DT, CT, false, 4>(a, stream)))
+#define XLLM_MLA_P(CT)                                                        \
+  (interleave != 0 ? launch_mla_prologue<DT, CT, true>(a, stream)             \
+                   : launch_mla_prologue<DT, CT, false>(a, stream))
   switch (cos_sin_dtype) {
     case XLLM_MI355_FP32: return XLLM_MLA_P(XLLM_MI355_FP32);
     case XLLM_MI355_BF16: return XLLM_MLA_P(XLLM_MI355_BF16);
