@@ -9,25 +9,28 @@
 // A decode step reads every key and value once for a few operations per byte, so the kernel is HBM bound and is built
 // to keep bytes in flight; both maps are taken in the one pass over the rows (two ordinary decodes would read V twice).
 //
-// Schedule.  The context of every (sequence, head block) is cut into stages of 16 tokens; the stages of the batch form
-// one list ordered (sequence, head block, stage).  A worker is one wavefront, four to a workgroup, one workgroup per CU;
-// every worker streams an equal range of the list, whatever the mix of lengths, and meets no other worker after the
-// common prefix sum of the lengths.  A range that holds a whole context writes the output row, a part of a context goes
-// to the workspace as (o, max, sum) in fp32 and diff_merge_kernel joins the parts.
+// Schedule.  The context of every (sequence, head block) is cut into stages of 16 tokens.  A worker is one wavefront, four
+// to a workgroup, one workgroup per CU; a team is the 4, 2 or 1 workers of a workgroup (as the head blocks divide) that
+// walk the same stages of adjacent head blocks side by side, so that what they ask for at a time is one run of memory: a
+// token's pairs lie next to each other.  The stages of the batch form one list ordered (sequence, group of head blocks,
+// stage); every team streams an equal range of it, whatever the mix of lengths, and its workers meet neither each other
+// nor other teams after the common prefix sum of the lengths.  A range that holds a whole context writes the output rows,
+// a part of a context goes to the workspace as (o, max, sum) in fp32 and diff_merge_kernel joins the parts.
 //
 // Data path.  Rows travel from global memory straight into a ring of the worker's own LDS (32 KB: two stages of 512-byte
 // rows, four of 256-byte rows), and the place of a stage's keys is filled again as soon as they are in registers, the
 // place of its values likewise.  Page-table entries take the same path two ring lengths ahead, so that no load of the
 // loop waits in a register (such a wait would also wait for every younger row in flight: the counter is in order).
 //   S^T[token, column] = K[token, dims] . Q^T        v_mfma_f32_16x16x32, K read from LDS, Q^T in registers
-//   O^T[dim, column]  += V^T[dim, token] . P^T       v_mfma_f32_16x16x16, V^T by the transposing LDS read, P^T straight
+//   O^T[dim, column]  += V^T[dim, token] . P^T       v_mfma_f32_16x16x32, V^T by the transposing LDS read, P^T straight
 //                                                    from the accumulators of S^T
 // The 16 columns hold both maps of up to eight heads (map 0 in columns 0-7, map 1 in 8-15: each map's query rows are
 // zero in the other's columns, so the two products add into one accumulator).  Groups of more than eight heads take two
 // blocks of 16 columns, one per map, so that rows are still read once for sixteen heads.
 // P is rounded to the 16-bit type in two parts, p = hi + lo, and both go through the matrix cores: the difference of the
 // maps can cancel most of o, which would leave the rounding of a single 16-bit P as the error of what remains (the norm
-// scales it up).  The second product costs 16 (8) more MFMAs per 16 KB (8 KB) of rows, which HBM leaves time for.
+// scales it up).  It is free: a stage's 16 tokens fill half the depth of a 16x16x32 MFMA, and the other half takes the same
+// values against lo.
 // Softmax statistics, sums and the norm are in fp32.
 #include "common.cuh"
 #include "launch.h"
@@ -36,14 +39,18 @@ namespace xllm_mi355 {
 
 namespace {
 
+// One worker per SIMD.  (Two, each with half the ring, measured the same: 97 and 96 us for 64 sequences, 775 and 774 us for
+// 256; the loop waits for memory, not for its own instructions: without its P.V products it took 2 % less.)
 constexpr int kDiffWaves = 4;
 constexpr int kDiffThreads = kDiffWaves * kWave;
 constexpr int kDiffTokens = 16;               // tokens of a stage
 constexpr int kDiffRing = 32768;              // ring bytes of a worker
-constexpr int kDiffMaxBatch = kWsMaxBatch;    // sequences per launch (their prefix and lengths lie in LDS)
+constexpr int kDiffMaxBatch = 1024;           // sequences per launch (their prefix and lengths lie in LDS)
 // A worker takes at least this many stages: with fewer, short batches would be cut into pieces whose partial rows cost
 // more than their keys and values.
-constexpr int kDiffMinStages = 4;
+constexpr int kDiffMinStages = 2;
+// Output rows up to which the parts of a row are joined by a workgroup of 16 wavefronts, and of 4 (one wavefront beyond).
+constexpr int64_t kDiffSplit16 = 256, kDiffSplit4 = 2048;
 constexpr float kDiffSlack = 8.0f;            // a maximum moves when a score exceeds it by this much (log2 units)
 
 typedef __attribute__((address_space(3))) s16x4 diff_lds_s16x4;
@@ -77,6 +84,11 @@ struct DiffArgs {
   int max_len;          // what the table can hold
   int window_left;
   int n_workers;
+  int team_shift;       // log2 of the workers of a team (1, 2 or 4)
+  // The list in two pools, 9 : 8, one for the workgroups of even number and one for the others (0: one list).  On the full
+  // chip (256 CUs, workgroup i on XCD i % 8) the odd XCDs stream slower with equal shares: 9 : 8 takes 4 % off the launch
+  // (256 sequences: 771 -> 742 us; 16 : 15 740, 16 : 17 769).  A tuned share and no more: every device computes the same.
+  int pools;
   float scale_log2;
   float eps;
   float out_scale;
@@ -89,12 +101,58 @@ __device__ __forceinline__ int diff_first(const DiffArgs& a, int L) {
 __device__ __forceinline__ int diff_stages(const DiffArgs& a, int L) {
   return L > 0 ? (L + kDiffTokens - 1) / kDiffTokens - diff_first(a, L) / kDiffTokens : 0;
 }
-// How many workers take part, and where the range of worker w begins.
-__device__ __forceinline__ int diff_used(const DiffArgs& a, int64_t total) {
-  const int64_t n = total / kDiffMinStages;
-  return static_cast<int>(n < 1 ? 1 : (n < a.n_workers ? n : a.n_workers));
+// How the list is dealt: stages in equal ranges, the first `rem` of them one longer.  With two pools (below) the first
+// `half` teams share the stages before `cut` that way, the others those behind it.
+// (Divisions are what this is careful with: 40 dependent instructions each in 32 bits, a hundred in 64, all of them before
+// a wavefront's first load.)
+__device__ __forceinline__ int64_t diff_div(int64_t x, int64_t y) {
+  return ((x | y) >> 32) == 0 ? static_cast<u32>(x) / static_cast<u32>(y) : x / y;
 }
-__device__ __forceinline__ int64_t diff_start(int64_t w, int64_t total, int used) { return w * total / used; }
+struct DiffShare {   // `n` ranges over `total` stages
+  int64_t per, rem;
+  __device__ __forceinline__ DiffShare(int64_t total, int n) : per(diff_div(total, n)), rem(total - per * n) {}
+  __device__ __forceinline__ int64_t start(int w) const { return w * per + (w < rem ? w : rem); }
+  __device__ __forceinline__ int owner(int64_t id) const {
+    const int64_t big = rem * (per + 1);   // (stages of the longer ranges; per is positive where they end before id)
+    return static_cast<int>(id < big ? diff_div(id, per + 1) : rem + diff_div(id - big, per));
+  }
+};
+constexpr int kPoolEven = 9, kPoolOdd = 8;
+struct DiffDeal {
+  int64_t total, cut;
+  int used, half;
+};
+__device__ __forceinline__ DiffDeal diff_deal(const DiffArgs& a, int64_t total) {
+  DiffDeal d;
+  d.total = total;
+  const int most = a.n_workers >> a.team_shift;
+  const int64_t n = total / kDiffMinStages;
+  d.used = static_cast<int>(n < 1 ? 1 : (n < most ? n : most));
+  const bool pools = a.pools != 0 && d.used == most;
+  d.half = pools ? most / 2 : 0;
+  d.cut = pools ? total * kPoolEven / (kPoolEven + kPoolOdd) : 0;
+  return d;
+}
+// The range [begin, end) of team w.
+__device__ __forceinline__ void diff_range(const DiffDeal& d, int w, int64_t& begin, int64_t& end) {
+  const bool second = w >= d.half;
+  const int n = d.half == 0 ? d.used : second ? d.used - d.half : d.half;
+  const int64_t base = second ? d.cut : 0;
+  const DiffShare share((second ? d.total : d.cut) - base, n);
+  const int q = second ? w - d.half : w;
+  begin = base + share.start(q);
+  end = base + share.start(q + 1);
+}
+// The team whose range holds stage `id`, and where that range begins.
+__device__ __forceinline__ int diff_team_of(const DiffDeal& d, int64_t id, int64_t& begin) {
+  const bool second = id >= d.cut;
+  const int n = d.half == 0 ? d.used : second ? d.used - d.half : d.half;
+  const int64_t base = second ? d.cut : 0;
+  const DiffShare share((second ? d.total : d.cut) - base, n);
+  const int q = share.owner(id - base);
+  begin = base + share.start(q);
+  return q + (second ? d.half : 0);
+}
 
 __device__ __forceinline__ void diff_dma16(const char* p, u32 lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(p) : "memory");
@@ -132,8 +190,9 @@ __device__ __forceinline__ float diff_of(float v0, float lam, float v1) {
 
 // A stage of the list.  Every field is the same in all lanes.
 struct DiffCursor {
-  int b, hb, st, n;    // sequence, head block, stage, stages of the context
+  int b, hg, st, n;    // sequence, group of head blocks, stage, stages of the context
   int L, lo;           // context length, first attended token
+  int pair, head0;     // the worker's KV pair and first head
 };
 
 template <int D, int NB>
@@ -147,17 +206,27 @@ struct DiffShape {
   static constexpr int kPageSlots = 2 * kStages;           // page-table entries are fetched two ring lengths ahead
   static constexpr int kCols = 16 * NB;
   static constexpr int kHeads = NB == 1 ? 8 : 16;          // heads of a head block
-  // LDS: rings | page entries [waves][kPageSlots][64] | scan scratch [8] | lengths [batch] | prefix [batch + 1]
+  // Query rows and lambdas of a context take the LDS path too, but for the one shape whose queries do not fit beside the
+  // rings: there they are fetched into registers, which waits for all rows in flight at every change of context.
+  static constexpr bool kQueryLds = !(D == 128 && NB == 2);
+  static constexpr int kQueryBytes = kQueryLds ? kHeads * kRow : 0;
+  static constexpr int kQueryLoads = kQueryBytes / (kWave * 16);
+  // LDS: rings | page entries [waves][kPageSlots][16] | queries [waves] | lambdas [waves][64] | norm weights | scan scratch
+  //      [8] | lengths [batch] | prefix [batch + 1]
   static constexpr int kPageOff = kDiffWaves * kDiffRing;
-  static constexpr int kTmpOff = kPageOff + kDiffWaves * kPageSlots * kWave * 4;
+  static constexpr int kQueryOff = kPageOff + kDiffWaves * kPageSlots * 64;
+  static constexpr int kLambdaOff = kQueryOff + kDiffWaves * kQueryBytes;
+  static constexpr int kNormOff = kLambdaOff + kDiffWaves * kWave * 4;
+  static constexpr int kTmpOff = kNormOff + 4 * D;
   static constexpr int kLensOff = kTmpOff + 32;
-  static size_t lds_bytes(int batch) { return kLensOff + static_cast<size_t>(2 * batch + 1) * 4; }
+  static constexpr size_t lds_bytes(int batch) { return kLensOff + static_cast<size_t>(2 * batch + 1) * 4; }
+  static_assert(lds_bytes(kDiffMaxBatch) <= 163840, "LDS of a CU");
 };
 
 // One head's finished row: o0 and o1 are the normalised results of the two maps for the lane's dims
-// 16 mb + 4 (lane / 16) + r.  All four lanes of a head (l, l ^ 16, l ^ 32, l ^ 48) call it together.
+// 16 mb + 4 (lane / 16) + r; norm: the weights in LDS.  All four lanes of a head (l, l ^ 16, l ^ 32, l ^ 48) call it together.
 template <typename QT, int MB>
-__device__ __forceinline__ void diff_store_row(const DiffArgs& a, const f32x4 (&o)[MB], int b, int head, bool on, int g) {
+__device__ __forceinline__ void diff_store_row(const DiffArgs& a, const char* norm, const f32x4 (&o)[MB], int b, int head, bool on, int g) {
   float ss = 0.0f;
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb)
@@ -172,7 +241,7 @@ __device__ __forceinline__ void diff_store_row(const DiffArgs& a, const f32x4 (&
   for (int mb = 0; mb < MB; ++mb) {
     f32x4 w = {1.0f, 1.0f, 1.0f, 1.0f};
     if (a.norm_w != nullptr) {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(a.norm_w + (mb * 16 + 4 * g) * 2);
+      const u32x2 x = *reinterpret_cast<const u32x2*>(norm + (mb * 16 + 4 * g) * 2);
       w = f32x4{QT::lo(x[0]), QT::hi(x[0]), QT::lo(x[1]), QT::hi(x[1])};
     }
     const u32x2 y = {QT::pack(o[mb][0] * f * w[0], o[mb][1] * f * w[1]), QT::pack(o[mb][2] * f * w[2], o[mb][3] * f * w[3])};
@@ -188,6 +257,7 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
   constexpr int NS = S::kStages;
   constexpr int NL = S::kLoads;
   constexpr int kStageOps = 1 + 2 * NL;   // vector memory operations of a stage: page entries, keys, values
+  static_assert(NS >= 2, "the wait for query rows leaves one younger stage in flight");
 
   extern __shared__ __align__(16) char smem[];
   int* tmp = reinterpret_cast<int*>(smem + S::kTmpOff);
@@ -197,9 +267,12 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
   const int lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
-  const int n_hb = a.n_pairs * a.hb_per_pair;
+  const int n_hg = (a.n_pairs * a.hb_per_pair) >> a.team_shift;
 
-  // ---- lengths and the exclusive prefix sum of the stages
+  // ---- norm weights, lengths and the exclusive prefix sum of the stages
+  if (a.norm_w != nullptr)
+    for (int i = tid; i < D; i += kDiffThreads)
+      reinterpret_cast<u32*>(smem + S::kNormOff)[i] = reinterpret_cast<const u32*>(a.norm_w)[i];
   {
     const int per = (a.batch + kDiffThreads - 1) / kDiffThreads;
     const int lo = min(a.batch, tid * per), hi = min(a.batch, lo + per);
@@ -229,13 +302,17 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
   if (blockIdx.x == 0)
     for (int b = tid; b <= a.batch; b += kDiffThreads) a.ws_prefix[b] = prefix[b];
 
-  const int64_t total = static_cast<int64_t>(prefix[a.batch]) * n_hb;
-  const int used = diff_used(a, total);
+  const int64_t total = static_cast<int64_t>(prefix[a.batch]) * n_hg;
+  if (total == 0) return;
+  const DiffDeal deal = diff_deal(a, total);
   // neighbours in the list sit on different CUs, so that a short list still spreads over the chip
-  const int worker = wave * gridDim.x + blockIdx.x;
-  if (total == 0 || worker >= used) return;
-  const int64_t begin = diff_start(worker, total, used);
-  const int N = static_cast<int>(diff_start(worker + 1, total, used) - begin);
+  const int member = wave & ((1 << a.team_shift) - 1), set = wave >> a.team_shift;
+  const int team = deal.half == 0 ? set * gridDim.x + blockIdx.x
+                                  : (blockIdx.x & 1) * deal.half + set * (gridDim.x / 2) + (blockIdx.x >> 1);
+  if (team >= deal.used) return;
+  int64_t begin, end;
+  diff_range(deal, team, begin, end);
+  const int N = static_cast<int>(end - begin);
   if (N <= 0) return;
 
   auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
@@ -244,35 +321,46 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
     c.lo = diff_first(a, c.L);
     c.n = diff_stages(a, c.L);
   };
+  auto place = [&](DiffCursor& c) {   // the fields of the worker's head block
+    const int hb = (c.hg << a.team_shift) + member;
+    c.pair = a.hb_per_pair == 1 ? hb : hb / a.hb_per_pair;
+    c.head0 = c.pair * a.group + (hb - c.pair * a.hb_per_pair) * S::kHeads;
+  };
   auto advance = [&](DiffCursor& c) {
     if (++c.st < c.n) return;
     c.st = 0;
-    if (++c.hb < n_hb) return;
-    c.hb = 0;
-    do ++c.b; while (c.b < a.batch - 1 && uniform(prefix[c.b + 1]) == uniform(prefix[c.b]));
-    if (c.b < a.batch) enter(c);
+    if (++c.hg == n_hg) {
+      c.hg = 0;
+      do ++c.b; while (c.b < a.batch - 1 && uniform(prefix[c.b + 1]) == uniform(prefix[c.b]));
+      enter(c);
+    }
+    place(c);
   };
   DiffCursor cc;   // computing
   {
     int lo = 0, hi = a.batch - 1;   // the last sequence that begins at or before the range (its stages hold it)
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if (static_cast<int64_t>(prefix[mid]) * n_hb <= begin) lo = mid;
+      if (static_cast<int64_t>(prefix[mid]) * n_hg <= begin) lo = mid;
       else hi = mid - 1;
     }
     cc.b = uniform(lo);
     enter(cc);
-    const int rest = uniform(static_cast<int>(begin - static_cast<int64_t>(prefix[cc.b]) * n_hb));
-    cc.hb = rest / cc.n;
-    cc.st = rest - cc.hb * cc.n;
+    const int rest = uniform(static_cast<int>(begin - static_cast<int64_t>(prefix[cc.b]) * n_hg));
+    cc.hg = rest < cc.n ? 0 : rest / cc.n;
+    cc.st = rest - cc.hg * cc.n;
+    place(cc);
   }
   DiffCursor lc = cc, pc = cc;   // loading rows, loading page entries
 
   const u32 lds0 = uniform(static_cast<u32>(reinterpret_cast<uintptr_t>(smem)));
   const u32 ring_lds = lds0 + wave * kDiffRing;
   const char* ring = smem + wave * kDiffRing;
-  const u32 page_lds = lds0 + S::kPageOff + wave * S::kPageSlots * kWave * 4;
-  const int* page_mem = reinterpret_cast<const int*>(smem + S::kPageOff) + wave * S::kPageSlots * kWave;
+  const u32 page_lds = lds0 + S::kPageOff + wave * S::kPageSlots * 64;
+  const int* page_mem = reinterpret_cast<const int*>(smem + S::kPageOff) + wave * S::kPageSlots * 16;
+  const u32 query_lds = lds0 + S::kQueryOff + wave * S::kQueryBytes, lambda_lds = lds0 + S::kLambdaOff + wave * kWave * 4;
+  const char* query_mem = smem + S::kQueryOff + wave * S::kQueryBytes;
+  const float* lambda_mem = reinterpret_cast<const float*>(smem + S::kLambdaOff) + wave * kWave;
 
   // token (lane & 15) of a stage; what lies outside the attended range repeats its first or last token, so that every
   // row in LDS is one that the sequence owns (a probability of zero times a stale NaN would be NaN)
@@ -295,7 +383,7 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
   auto fetch_pages = [&]() {
     int col, off;
     split(token_of(pc), col, off);
-    diff_dma4(a.block_table + pc.b * a.table_stride + col, page_lds + (px % S::kPageSlots) * (kWave * 4));
+    if (lane < 16) diff_dma4(a.block_table + pc.b * a.table_stride + col, page_lds + (px % S::kPageSlots) * 64);
     ++px;
     if (px < N) advance(pc);
   };
@@ -307,15 +395,14 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
     const int t = token_of(lc);
     int col, off;
     split(t, col, off);
-    const int page = max(0, min(page_mem[(lx % S::kPageSlots) * kWave + lane], a.num_blocks - 1));
+    const int page = max(0, min(page_mem[(lx % S::kPageSlots) * 16 + c16], a.num_blocks - 1));
     const int slot = page * a.block_size + off;
-    const int pair = lc.hb / a.hb_per_pair;
     const u32 base = ring_lds + (lx % NS) * (2 * S::kTile);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int row = i * S::kRowsPerLoad + dr;
       const int s = __shfl(slot, row, kWave);
-      row_off[i] = s * a.row_bytes + pair * S::kRow;
+      row_off[i] = s * a.row_bytes + lc.pair * S::kRow;
       diff_dma16(a.k_cache + row_off[i] + ((dc ^ row) & (S::kChunks - 1)) * 16, uniform(base + i * 1024));
     }
   };
@@ -330,9 +417,23 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
     if (lx < N) advance(lc);
   };
 
+  // Query rows [heads][2 maps][D] and lambdas of the context at cursor c.
+  auto heads_of = [&](const DiffCursor& c) { return min(S::kHeads, (c.pair + 1) * a.group - c.head0); };
+  auto fetch_query = [&](const DiffCursor& c) {
+    const int heads = heads_of(c);
+    const char* row = a.q + c.b * a.q_stride_bytes + static_cast<int64_t>(c.head0) * S::kRow;
+#pragma unroll
+    for (int i = 0; i < S::kQueryLoads; ++i)   // (what lies behind the block's heads repeats its last chunk)
+      diff_dma16(row + min(i * kWave + lane, heads * S::kChunks - 1) * 16, uniform(query_lds + i * 1024));
+    const int head = c.head0 + min(lane, heads - 1);
+    diff_dma4(reinterpret_cast<const int32_t*>(a.lambda + c.b * a.lambda_batch_stride + head * a.lambda_head_stride),
+              uniform(lambda_lds));
+  };
+
   // ---- prologue: the first ring of stages in flight, the next ring's page entries with them
 #pragma unroll 1
   for (int i = 0; i < NS; ++i) fetch_pages();
+  fetch_query(cc);
   diff_wait_vm<0>();
 #pragma unroll 1
   for (int i = 0; i < NS && i < N; ++i) {
@@ -345,31 +446,52 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
   u32x4 q[2 * KS];
   f32x4 o[NB][MB];
   float m[NB], l[NB];
-  bool fresh = true;         // a context begins: its query rows are still to be fetched
+  float lam = 0.0f;
+  bool fresh = true;         // a context begins: its query rows are still to be read
   bool first_run = true;     // the first context of the range
   bool from_start = false;   // the context's first stage was this worker's
   const int k_read = c16 * S::kRow;
   const int v_row = 4 * g + (c16 >> 2);
   const int v_read = v_row * S::kRow + (c16 & 1) * 8;
   const int v_chunk = ((c16 & 3) >> 1) ^ ((v_row & 7) << 1);
+  const int head = NB == 1 ? c16 & 7 : c16;   // the lane's head in its block
 
 #pragma unroll 1
   for (int s = 0; s < N; ++s) {
-    const int pair = cc.hb / a.hb_per_pair;
-    const int head0 = pair * a.group + (cc.hb - pair * a.hb_per_pair) * S::kHeads;   // first head of the block
-    const int heads = min(S::kHeads, (pair + 1) * a.group - head0);
+    const int head0 = cc.head0, heads = heads_of(cc);
+    const bool more = s + NS < N;
+    const bool last = cc.st == cc.n - 1;
+    DiffCursor nc = cc;
+    if (s + 1 < N) advance(nc);
+    const char* st = ring + (s % NS) * (2 * S::kTile);
+
+    // ---- keys: wait for them (and for the query rows of a new context, asked for one stage ago)
+    if (s + NS > N) diff_wait_vm<0>();
+    else if (fresh && s > 0) diff_wait_vm<kStageOps>();
+    else diff_wait_vm<NL + (NS - 1) * kStageOps>();
     if (fresh) {
       fresh = false;
       from_start = cc.st == 0;
-      const int head = NB == 1 ? c16 & 7 : c16;
-      const char* row = a.q + cc.b * a.q_stride_bytes + static_cast<int64_t>(head0 + (head < heads ? head : 0)) * (4 * D) + g * 16;
+      lam = lambda_mem[head < heads ? head : 0];
 #pragma unroll
-      for (int mp = 0; mp < 2; ++mp) {
-        const bool on = head < heads && (NB == 2 || (c16 >> 3) == mp);
-#pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-          const u32x4 x = ldg16(row + mp * (2 * D) + kk * 64);
-          q[mp * KS + kk] = on ? x : u32x4{0, 0, 0, 0};
+      for (int kk = 0; kk < KS; ++kk) {
+        if constexpr (S::kQueryLds) {
+          const char* row = query_mem + head * S::kRow + g * 16 + kk * 64;
+          if constexpr (NB == 1) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(row + (c16 >> 3) * (2 * D));
+            q[kk] = head < heads && c16 < 8 ? x : u32x4{0, 0, 0, 0};
+            q[KS + kk] = head < heads && c16 >= 8 ? x : u32x4{0, 0, 0, 0};
+          } else {
+            const u32x4 x0 = *reinterpret_cast<const u32x4*>(row), x1 = *reinterpret_cast<const u32x4*>(row + 2 * D);
+            q[kk] = head < heads ? x0 : u32x4{0, 0, 0, 0};
+            q[KS + kk] = head < heads ? x1 : u32x4{0, 0, 0, 0};
+          }
+        } else {
+          const char* row = a.q + cc.b * a.q_stride_bytes + static_cast<int64_t>(head0 + (head < heads ? head : 0)) * S::kRow +
+                            g * 16 + kk * 64;
+          const u32x4 x0 = ldg16(row), x1 = ldg16(row + 2 * D);
+          q[kk] = head < heads ? x0 : u32x4{0, 0, 0, 0};
+          q[KS + kk] = head < heads ? x1 : u32x4{0, 0, 0, 0};
         }
       }
 #pragma unroll
@@ -379,13 +501,11 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) o[nb][mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
+      diff_wait_lds();   // (the next context's rows may take the place of these)
     }
-    const bool more = s + NS < N;
-    const char* st = ring + (s % NS) * (2 * S::kTile);
+    if (last && s + 1 < N) fetch_query(nc);
 
-    // ---- keys: wait for them, read them, and fill their place again
-    if (s + NS <= N) diff_wait_vm<NL + (NS - 1) * kStageOps>();
-    else diff_wait_vm<0>();
+    // ---- read the keys and fill their place again
     u32x4 kr[2 * KS];
 #pragma unroll
     for (int i = 0; i < 2 * KS; ++i)
@@ -413,7 +533,7 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
       }
     }
     const int tok0 = (cc.lo / kDiffTokens + cc.st) * kDiffTokens + 4 * g;
-    u32x2 p_hi[NB], p_lo[NB];
+    u32x4 p[NB];   // the lane's four probabilities: their 16-bit values, then what those leave over
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       float sv[4];
@@ -433,44 +553,47 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
           for (int mb = 0; mb < MB; ++mb) o[nb][mb] *= alpha;
         }
       }
-      float p[4];
+      float e[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        p[r] = fast_exp2(sv[r] - m[nb]);
-        l[nb] += p[r];
+        e[r] = fast_exp2(sv[r] - m[nb]);
+        l[nb] += e[r];
       }
-      p_hi[nb] = u32x2{QT::pack(p[0], p[1]), QT::pack(p[2], p[3])};
-      p_lo[nb] = u32x2{QT::pack(p[0] - QT::lo(p_hi[nb][0]), p[1] - QT::hi(p_hi[nb][0])),
-                       QT::pack(p[2] - QT::lo(p_hi[nb][1]), p[3] - QT::hi(p_hi[nb][1]))};
+      const u32 h0 = QT::pack(e[0], e[1]), h1 = QT::pack(e[2], e[3]);
+      p[nb] = u32x4{h0, h1, QT::pack(e[0] - QT::lo(h0), e[1] - QT::hi(h0)), QT::pack(e[2] - QT::lo(h1), e[3] - QT::hi(h1))};
     }
 
     // ---- values: the same, by the transposing read (lane c16 of 16 supplies 4 dims of token 4 g + c16 / 4 and receives
     // the 4 tokens 4 g .. of dim 16 mb + c16)
     if (more) diff_wait_vm<(NS - 1) * kStageOps + 1 + NL>();
     else diff_wait_vm<0>();
-    s16x4 vt[MB];
+    // (two blocks of columns leave registers for half of the values at a time)
+    constexpr int VB = MB / NB;
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
-      vt[mb] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((diff_lds_s16x4*)(st + S::kTile + v_read + ((v_chunk ^ (2 * mb)) * 16)));
-    diff_wait_lds();
-    if (more) load_values();
+    for (int h = 0; h < NB; ++h) {
+      s16x4 vt[VB];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+      for (int i = 0; i < VB; ++i)
+        vt[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (diff_lds_s16x4*)(st + S::kTile + v_read + ((v_chunk ^ (2 * (h * VB + i))) * 16)));
+      diff_wait_lds();
+      if (h == NB - 1 && more) load_values();
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        o[nb][mb] = Mfma<QT>::k16(vt[mb], p_hi[nb], o[nb][mb]);
-        o[nb][mb] = Mfma<QT>::k16(vt[mb], p_lo[nb], o[nb][mb]);
-      }
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < VB; ++i) {
+          const int mb = h * VB + i;
+          const u32x2 v = __builtin_bit_cast(u32x2, vt[i]);
+          o[nb][mb] = Mfma<QT>::k32(u32x4{v[0], v[1], v[0], v[1]}, p[nb], o[nb][mb]);
+        }
+    }
 
     // ---- the end of the context, or of the range
-    const bool last = cc.st == cc.n - 1;
     if (last || s == N - 1) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) l[nb] = diff_rows_sum(l[nb]);
       if (last && from_start) {
-        const int head = NB == 1 ? c16 & 7 : c16;
         const bool on = head < heads && (NB == 2 || c16 < 8);
-        const float lam = a.lambda[cc.b * a.lambda_batch_stride + (head0 + (head < heads ? head : 0)) * a.lambda_head_stride];
         f32x4 d[MB];
         const float inv0 = 1.0f / l[0], inv1 = 1.0f / l[NB - 1];
 #pragma unroll
@@ -482,12 +605,11 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
             const float v1 = NB == 1 ? dpp<0x128>(v0) : o[NB - 1][mb][r] * inv1;
             d[mb][r] = diff_of(v0, lam, v1);
           }
-        diff_store_row<QT, MB>(a, d, cc.b, head0 + (head < heads ? head : 0), on, g);
+        diff_store_row<QT, MB>(a, smem + S::kNormOff, d, cc.b, head0 + (head < heads ? head : 0), on, g);
       } else {
-        const int64_t slot = 2 * static_cast<int64_t>(worker) + (first_run ? 0 : 1);
+        const int64_t slot = 2 * ((static_cast<int64_t>(team) << a.team_shift) + member) + (first_run ? 0 : 1);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          const int head = NB == 1 ? c16 & 7 : c16;
           const int64_t col = slot * S::kCols + nb * 16 + c16;
           if (head < heads) {
 #pragma unroll
@@ -499,49 +621,45 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
       first_run = false;
       fresh = true;
     }
-    if (s + 1 < N) advance(cc);
+    cc = nc;
   }
 }
 
-// Joins the parts of the contexts that several workers hold, and writes zeros for empty contexts.  One workgroup per
-// (head, sequence); the parts are dealt to its wavefronts, a lane holds 2 D / 64 dims of both maps.  The parts are read
-// and added in the order of the list, whatever order they were written in.
-template <typename QT, int D, int NB>
-__global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(DiffArgs a) {
+// Joins the parts of the contexts that several teams hold, and writes zeros for empty contexts.  A lane holds 2 D / 64 dims
+// of both maps.  SPLIT: one workgroup per (head, sequence), whose WAVES wavefronts share the parts; else one wavefront per
+// head, WAVES heads to a workgroup.  The parts are added in an order that only their number sets.
+template <typename QT, int D, int NB, int WAVES, bool SPLIT>
+__global__ __launch_bounds__(WAVES * kWave) void diff_merge_kernel(DiffArgs a) {
   using S = DiffShape<D, NB>;
   constexpr int E = 2 * D / kWave;   // dims per lane
   typedef __attribute__((ext_vector_type(E))) float fvec;
-  __shared__ float acc[kDiffWaves][2][2 * D];
-  __shared__ float sums[kDiffWaves][2][2];   // maximum, sum
-  const int head = blockIdx.x, b = blockIdx.y;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-  const int pair = head / a.group;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = SPLIT ? blockIdx.x : blockIdx.x * WAVES + wave, b = blockIdx.y;
+  if (!SPLIT && head >= a.n_heads) return;
+  const int pair = a.group == 1 ? head : static_cast<int>(static_cast<u32>(head) / static_cast<u32>(a.group));
   const int in_pair = head - pair * a.group;
-  const int hb = pair * a.hb_per_pair + in_pair / S::kHeads;
-  const int h = in_pair % S::kHeads;
-  const int n_hb = a.n_pairs * a.hb_per_pair;
+  const int hb = pair * a.hb_per_pair + static_cast<int>(static_cast<u32>(in_pair) / S::kHeads);
+  const int h = static_cast<int>(static_cast<u32>(in_pair) % S::kHeads);
+  const int n_hg = (a.n_pairs * a.hb_per_pair) >> a.team_shift;
+  const int hg = hb >> a.team_shift, member = hb & ((1 << a.team_shift) - 1);
+  // (asked for before the parts, whose loads hang off the prefix: the launch is a chain of such trips)
+  const float lam = a.lambda[b * a.lambda_batch_stride + head * a.lambda_head_stride];
+  u32 weight[E / 2];
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) weight[i] = a.norm_w != nullptr ? reinterpret_cast<const u32*>(a.norm_w)[lane * (E / 2) + i] : 0;
   const int p0 = a.ws_prefix[b], n = a.ws_prefix[b + 1] - p0;
   char* row = a.out + b * a.out_stride_bytes + static_cast<int64_t>(head) * (4 * D);
   if (n == 0) {
-    if (wave == 0)
+    if (!SPLIT || wave == 0)
       for (int i = 0; i < E / 2; ++i) reinterpret_cast<u32*>(row)[lane * (E / 2) + i] = 0;
     return;
   }
-  const int64_t total = static_cast<int64_t>(a.ws_prefix[a.batch]) * n_hb;
-  const int used = diff_used(a, total);
-  const int64_t s0 = static_cast<int64_t>(p0) * n_hb + static_cast<int64_t>(hb) * n, s1 = s0 + n - 1;
-  auto worker_of = [&](int64_t id) {
-    int w = static_cast<int>(id * used / total);
-    while (w + 1 < used && diff_start(w + 1, total, used) <= id) ++w;
-    return w;
-  };
-  const int wf = worker_of(s0), wl = worker_of(s1);
-  if (wf == wl) return;   // one worker held it whole and wrote the row
-  const int first_slot = diff_start(wf, total, used) < s0 ? 1 : 0;
-  auto column = [&](int w, int mp) {
-    const int64_t slot = 2 * static_cast<int64_t>(w) + (w == wf ? first_slot : 0);
-    return slot * S::kCols + (NB == 1 ? mp * 8 : mp * 16) + h;
-  };
+  const DiffDeal deal = diff_deal(a, static_cast<int64_t>(a.ws_prefix[a.batch]) * n_hg);
+  const int64_t s0 = static_cast<int64_t>(p0) * n_hg + static_cast<int64_t>(hg) * n;
+  int64_t begin, unused;
+  const int wf = diff_team_of(deal, s0, begin), wl = diff_team_of(deal, s0 + n - 1, unused);
+  if (wf == wl) return;   // one team held it whole and wrote the rows
+  const int first_slot = begin < s0 ? 1 : 0;
   fvec o[2];
   float m[2], l[2];
 #pragma unroll
@@ -551,10 +669,11 @@ __global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(DiffArgs a) {
     l[mp] = 0.0f;
   }
 #pragma unroll 4
-  for (int w = wf + wave; w <= wl; w += kDiffWaves) {
+  for (int w = wf + (SPLIT ? wave : 0); w <= wl; w += SPLIT ? WAVES : 1) {
+    const int64_t slot = 2 * ((static_cast<int64_t>(w) << a.team_shift) + member) + (w == wf ? first_slot : 0);
 #pragma unroll
     for (int mp = 0; mp < 2; ++mp) {
-      const int64_t col = column(w, mp);
+      const int64_t col = slot * S::kCols + (NB == 1 ? mp * 8 : mp * 16) + h;
       const f32x2 ml = *reinterpret_cast<const f32x2*>(a.ws_ml + col * 2);
       const fvec x = *reinterpret_cast<const fvec*>(a.ws_o + col * (2 * D) + lane * E);
       const float mx = fmaxf(m[mp], ml[0]);
@@ -564,32 +683,38 @@ __global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(DiffArgs a) {
       m[mp] = mx;
     }
   }
+  if constexpr (SPLIT) {
+    __shared__ float acc[WAVES][2][2 * D];
+    __shared__ float sums[WAVES][2][2];   // maximum, sum
 #pragma unroll
-  for (int mp = 0; mp < 2; ++mp) {
-    *reinterpret_cast<fvec*>(&acc[wave][mp][lane * E]) = o[mp];
-    if (lane == 0) {
-      sums[wave][mp][0] = m[mp];
-      sums[wave][mp][1] = l[mp];
+    for (int mp = 0; mp < 2; ++mp) {
+      *reinterpret_cast<fvec*>(&acc[wave][mp][lane * E]) = o[mp];
+      if (lane == 0) {
+        sums[wave][mp][0] = m[mp];
+        sums[wave][mp][1] = l[mp];
+      }
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int mp = 0; mp < 2; ++mp) {
+      float mx = m[mp];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) mx = fmaxf(mx, sums[w][mp][0]);
+      fvec t = fvec(0.0f);
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float f = fast_exp2(sums[w][mp][0] - mx);
+        t += *reinterpret_cast<const fvec*>(&acc[w][mp][lane * E]) * f;
+        sum += sums[w][mp][1] * f;
+      }
+      o[mp] = t;
+      l[mp] = sum;
     }
   }
-  __syncthreads();
-  if (wave != 0) return;
 #pragma unroll
-  for (int mp = 0; mp < 2; ++mp) {
-    float mx = m[mp];
-#pragma unroll
-    for (int w = 1; w < kDiffWaves; ++w) mx = fmaxf(mx, sums[w][mp][0]);
-    fvec t = fvec(0.0f);
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kDiffWaves; ++w) {
-      const float f = fast_exp2(sums[w][mp][0] - mx);
-      t += *reinterpret_cast<const fvec*>(&acc[w][mp][lane * E]) * f;
-      sum += sums[w][mp][1] * f;
-    }
-    o[mp] = t * (1.0f / sum);
-  }
-  const float lam = a.lambda[b * a.lambda_batch_stride + head * a.lambda_head_stride];
+  for (int mp = 0; mp < 2; ++mp) o[mp] *= 1.0f / l[mp];
   fvec d;
   float ss = 0.0f;
 #pragma unroll
@@ -604,9 +729,8 @@ __global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(DiffArgs a) {
   for (int i = 0; i < E; i += 2) {
     float w0 = 1.0f, w1 = 1.0f;
     if (a.norm_w != nullptr) {
-      const u32 x = reinterpret_cast<const u32*>(a.norm_w)[(lane * E + i) / 2];
-      w0 = QT::lo(x);
-      w1 = QT::hi(x);
+      w0 = QT::lo(weight[i / 2]);
+      w1 = QT::hi(weight[i / 2]);
     }
     reinterpret_cast<u32*>(row)[(lane * E + i) / 2] = QT::pack(d[i] * f * w0, d[i + 1] * f * w1);
   }
@@ -626,8 +750,15 @@ int launch_diff(const DiffArgs& a, hipStream_t stream) {
                S::lds_bytes(a.batch), stream, a);
   int rc = static_cast<int>(hipGetLastError());
   if (rc != 0) return rc;
-  launch_timed(diff_merge_kernel<QT, D, NB>, dim3(static_cast<unsigned>(a.n_heads), static_cast<unsigned>(a.batch)),
-               dim3(kDiffThreads), 0, stream, a);
+  // few rows: their contexts may be in many parts, which the wavefronts of a workgroup share; many rows: a wavefront each
+  const unsigned batch = static_cast<unsigned>(a.batch), heads = static_cast<unsigned>(a.n_heads);
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.n_heads;
+  if (rows <= kDiffSplit16)
+    launch_timed(diff_merge_kernel<QT, D, NB, 16, true>, dim3(heads, batch), dim3(16 * kWave), 0, stream, a);
+  else if (rows <= kDiffSplit4)
+    launch_timed(diff_merge_kernel<QT, D, NB, 4, true>, dim3(heads, batch), dim3(4 * kWave), 0, stream, a);
+  else
+    launch_timed(diff_merge_kernel<QT, D, NB, 4, false>, dim3((heads + 3) / 4, batch), dim3(4 * kWave), 0, stream, a);
   return static_cast<int>(hipGetLastError());
 }
 
@@ -701,6 +832,9 @@ int paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, v
   a.max_len = long_table ? 0x7fffffff - 16 : static_cast<int>(table_width * block_size);
   a.window_left = window_left < 0 ? -1 : static_cast<int>(window_left < 0x7fffffffLL ? window_left : 0x7fffffffLL);
   a.n_workers = device_cu_count() * kDiffWaves;
+  a.pools = device_cu_count() == 256 ? 1 : 0;
+  const int64_t head_blocks = n_kv_pairs * a.hb_per_pair;
+  a.team_shift = head_blocks % 4 == 0 ? 2 : head_blocks % 2 == 0 ? 1 : 0;
   a.scale_log2 = sm_scale * kLog2e;
   a.eps = eps;
   a.out_scale = out_scale;
