@@ -145,6 +145,20 @@ def test_sharp_and_cancelling_maps():
     check(close, 4, 2, 128, 16, torch.full((1,), 0.9, device=DEV), weight=w)
 
 
+def test_infinite_keys_of_one_map_leave_the_other_alone():
+    """A key of the second map whose scores are -inf has no weight there and its ordinary one in the first map."""
+    lens = [70, 200]
+    p = problem(lens, 2, 1, 64, 16, BF16, seed=12)
+    p["q"] = p["q"].abs()   # (so that every product with the infinite key is -inf)
+    plain = dict(p, k=p["k"].clone())
+    for b, t in ((0, 5), (0, 69), (1, 100)):
+        page, row = int(p["table"][b, t // 16]), t % 16
+        p["k"][page, row, 1] = float("-inf")
+        plain["k"][page, row, 1] = -1000.0   # (scores of some -6000: no weight either)
+    assert torch.equal(run(p, 2, 64, lam_of(2)), run(plain, 2, 64, lam_of(2)))
+    check(plain, 2, 1, 64, 16, lam_of(2))
+
+
 def test_lambda_shapes_and_strides():
     lens, H = [90, 700, 33], 6
     p = problem(lens, H, 2, 64, 16, BF16, seed=4)

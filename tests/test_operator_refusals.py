@@ -84,7 +84,7 @@ def test_mla_prologue():
 def test_differential_decode():
     lib = capi.lib()
     size = lib.xllm_mi355_paged_decode_diff_workspace_bytes
-    assert size(16, 4, 128) > 0 and size(16, 4, 64) < size(16, 4, 128) < size(64, 4, 128)
+    assert size(16, 4, 64) > 0 and 0 < size(16, 4, 128) < size(64, 4, 128)
     assert size(0, 1, 128) == 0 and size(5, 2, 128) == 0 and size(4, 2, 96) == 0
     fn = lib.xllm_mi355_paged_decode_diff
     base = dict(q=FAKE, k=FAKE, v=FAKE, out=FAKE, table=FAKE, stride=8, width=8, lens=FAKE, lam=FAKE, lb=0, lh=1, w=None,

@@ -220,7 +220,7 @@ struct Span {
   uintptr_t lo = 0, hi = 0;
   Span() = default;
   Span(const void* p, int64_t bytes) : lo(reinterpret_cast<uintptr_t>(p)), hi(p == nullptr ? 0 : lo + static_cast<uintptr_t>(bytes)) {}
-  bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
+  bool meets(const Span& o) const { return lo < hi && o.lo < o.hi && lo < o.hi && o.lo < hi; }
 };
 // [n0, n1, inner] elements with strides s0, s1 and a contiguous last dim.
 inline Span span_of(const void* p, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t inner, int64_t elem_bytes) {

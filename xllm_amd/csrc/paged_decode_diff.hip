@@ -10,7 +10,7 @@
 // to keep bytes in flight; both maps are taken in the one pass over the rows (two ordinary decodes would read V twice).
 //
 // Schedule.  The context of every (sequence, head block) is cut into stages of 16 tokens.  A worker is one wavefront, four
-// to a workgroup, one workgroup per CU; a team is the 4, 2 or 1 workers of a workgroup (as the head blocks divide) that
+// or eight to a workgroup, one workgroup per CU; a team is the 4, 2 or 1 workers of a workgroup (as the head blocks divide) that
 // walk the same stages of adjacent head blocks side by side, so that what they ask for at a time is one run of memory: a
 // token's pairs lie next to each other.  The stages of the batch form one list ordered (sequence, group of head blocks,
 // stage); every team streams an equal range of it, whatever the mix of lengths, and its workers meet neither each other
@@ -24,8 +24,8 @@
 //   S^T[token, column] = K[token, dims] . Q^T        v_mfma_f32_16x16x32, K read from LDS, Q^T in registers
 //   O^T[dim, column]  += V^T[dim, token] . P^T       v_mfma_f32_16x16x32, V^T by the transposing LDS read, P^T straight
 //                                                    from the accumulators of S^T
-// The 16 columns hold both maps of up to eight heads (map 0 in columns 0-7, map 1 in 8-15: each map's query rows are
-// zero in the other's columns, so the two products add into one accumulator).  Groups of more than eight heads take two
+// The 16 columns hold both maps of up to eight heads (map 0 in columns 0-7, map 1 in 8-15); both maps' keys are multiplied
+// with all of them, and a column keeps the scores of its own.  Groups of more than eight heads take two
 // blocks of 16 columns, one per map, so that rows are still read once for sixteen heads.
 // P is rounded to the 16-bit type in two parts, p = hi + lo, and both go through the matrix cores: the difference of the
 // maps can cancel most of o, which would leave the rounding of a single 16-bit P as the error of what remains (the norm
@@ -39,17 +39,15 @@ namespace xllm_mi355 {
 
 namespace {
 
-// One worker per SIMD.  (Two, each with half the ring, measured the same: 97 and 96 us for 64 sequences, 775 and 774 us for
-// 256; the loop waits for memory, not for its own instructions: without its P.V products it took 2 % less.)
-constexpr int kDiffWaves = 4;
-constexpr int kDiffThreads = kDiffWaves * kWave;
 constexpr int kDiffTokens = 16;               // tokens of a stage
-constexpr int kDiffRing = 32768;              // ring bytes of a worker
+constexpr int kDiffRings = 131072;            // ring bytes of a workgroup
 constexpr int kDiffMaxBatch = 1024;           // sequences per launch (their prefix and lengths lie in LDS)
-// A worker takes at least this many stages: with fewer, short batches would be cut into pieces whose partial rows cost
-// more than their keys and values.
+// A team takes at least this many stages.  One is faster for a few short contexts (4 of up to 512 tokens: 11.4 us for one
+// stage, 12.5 for two, 14.9 for four) and slower where one context is then in 250 parts (4000 tokens: 24.4, 20.3, 21.7 us).
 constexpr int kDiffMinStages = 2;
 // Output rows up to which the parts of a row are joined by a workgroup of 16 wavefronts, and of 4 (one wavefront beyond).
+// 16 rows of 250 parts: 12 us with 16, 30 us with 4; 1024 rows of 5 parts: 6 us with 4 and with one; 8192 rows of 2 parts:
+// 34 us with 4, 14 us with one.
 constexpr int64_t kDiffSplit16 = 256, kDiffSplit4 = 2048;
 constexpr float kDiffSlack = 8.0f;            // a maximum moves when a score exceeds it by this much (log2 units)
 
@@ -197,26 +195,33 @@ struct DiffCursor {
 
 template <int D, int NB>
 struct DiffShape {
+  // One worker per SIMD for rows of 512 bytes, two for rows of 256, which bring half the bytes for the same instructions.
+  // 64 sequences of 1k to 8k tokens over 4 pairs of 64-dim maps: 99 us with two and 102 with one for 16 heads, 111 and 124
+  // for 64 heads; of 128-dim maps and 16 heads: 97 and 96 us (0.5k to 4k tokens), where the loop waits for memory and not
+  // for its instructions (without its P.V products it takes 2 % less).
+  static constexpr int kWaves = D == 64 ? 8 : 4;
+  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kRing = kDiffRings / kWaves;         // ring bytes of a worker
   static constexpr int kRow = 4 * D;                       // bytes of a pair's row
   static constexpr int kChunks = kRow / 16;                // 16-byte chunks of a row
   static constexpr int kRowsPerLoad = kWave / kChunks;
   static constexpr int kLoads = kDiffTokens / kRowsPerLoad; // load instructions of a stage's keys, and of its values
   static constexpr int kTile = kDiffTokens * kRow;         // bytes of a stage's keys
-  static constexpr int kStages = kDiffRing / (2 * kTile);  // ring length
+  static constexpr int kStages = kRing / (2 * kTile);  // ring length
   static constexpr int kPageSlots = 2 * kStages;           // page-table entries are fetched two ring lengths ahead
   static constexpr int kCols = 16 * NB;
   static constexpr int kHeads = NB == 1 ? 8 : 16;          // heads of a head block
-  // Query rows and lambdas of a context take the LDS path too, but for the one shape whose queries do not fit beside the
-  // rings: there they are fetched into registers, which waits for all rows in flight at every change of context.
-  static constexpr bool kQueryLds = !(D == 128 && NB == 2);
+  // Query rows and lambdas of a context take the LDS path too.  Those of sixteen heads do not fit beside the rings: they
+  // are fetched into registers, which waits for all rows in flight at every change of context.
+  static constexpr bool kQueryLds = NB == 1;
   static constexpr int kQueryBytes = kQueryLds ? kHeads * kRow : 0;
   static constexpr int kQueryLoads = kQueryBytes / (kWave * 16);
   // LDS: rings | page entries [waves][kPageSlots][16] | queries [waves] | lambdas [waves][64] | norm weights | scan scratch
   //      [8] | lengths [batch] | prefix [batch + 1]
-  static constexpr int kPageOff = kDiffWaves * kDiffRing;
-  static constexpr int kQueryOff = kPageOff + kDiffWaves * kPageSlots * 64;
-  static constexpr int kLambdaOff = kQueryOff + kDiffWaves * kQueryBytes;
-  static constexpr int kNormOff = kLambdaOff + kDiffWaves * kWave * 4;
+  static constexpr int kPageOff = kDiffRings;
+  static constexpr int kQueryOff = kPageOff + kWaves * kPageSlots * 64;
+  static constexpr int kLambdaOff = kQueryOff + kWaves * kQueryBytes;
+  static constexpr int kNormOff = kLambdaOff + kWaves * kWave * 4;
   static constexpr int kTmpOff = kNormOff + 4 * D;
   static constexpr int kLensOff = kTmpOff + 32;
   static constexpr size_t lds_bytes(int batch) { return kLensOff + static_cast<size_t>(2 * batch + 1) * 4; }
@@ -250,8 +255,9 @@ __device__ __forceinline__ void diff_store_row(const DiffArgs& a, const char* no
 }
 
 template <typename QT, int D, int NB>
-__global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a) {
+__global__ __launch_bounds__((DiffShape<D, NB>::kThreads), 1) void diff_decode_kernel(DiffArgs a) {
   using S = DiffShape<D, NB>;
+  constexpr int kThreads = S::kThreads;
   constexpr int KS = D / 32;       // k-steps of a map's scores
   constexpr int MB = 2 * D / 16;   // dim blocks of the output
   constexpr int NS = S::kStages;
@@ -271,10 +277,10 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
 
   // ---- norm weights, lengths and the exclusive prefix sum of the stages
   if (a.norm_w != nullptr)
-    for (int i = tid; i < D; i += kDiffThreads)
+    for (int i = tid; i < D; i += kThreads)
       reinterpret_cast<u32*>(smem + S::kNormOff)[i] = reinterpret_cast<const u32*>(a.norm_w)[i];
   {
-    const int per = (a.batch + kDiffThreads - 1) / kDiffThreads;
+    const int per = (a.batch + kThreads - 1) / kThreads;
     const int lo = min(a.batch, tid * per), hi = min(a.batch, lo + per);
     int local = 0;
     for (int b = lo; b < hi; ++b) {
@@ -296,11 +302,11 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
       prefix[b] = excl;
       excl += diff_stages(a, lens[b]);
     }
-    if (tid == kDiffThreads - 1) prefix[a.batch] = excl;   // (an empty slice leaves the total as it came in)
+    if (tid == kThreads - 1) prefix[a.batch] = excl;   // (an empty slice leaves the total as it came in)
     __syncthreads();
   }
   if (blockIdx.x == 0)
-    for (int b = tid; b <= a.batch; b += kDiffThreads) a.ws_prefix[b] = prefix[b];
+    for (int b = tid; b <= a.batch; b += kThreads) a.ws_prefix[b] = prefix[b];
 
   const int64_t total = static_cast<int64_t>(prefix[a.batch]) * n_hg;
   if (total == 0) return;
@@ -354,8 +360,8 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
   DiffCursor lc = cc, pc = cc;   // loading rows, loading page entries
 
   const u32 lds0 = uniform(static_cast<u32>(reinterpret_cast<uintptr_t>(smem)));
-  const u32 ring_lds = lds0 + wave * kDiffRing;
-  const char* ring = smem + wave * kDiffRing;
+  const u32 ring_lds = lds0 + wave * S::kRing;
+  const char* ring = smem + wave * S::kRing;
   const u32 page_lds = lds0 + S::kPageOff + wave * S::kPageSlots * 64;
   const int* page_mem = reinterpret_cast<const int*>(smem + S::kPageOff) + wave * S::kPageSlots * 16;
   const u32 query_lds = lds0 + S::kQueryOff + wave * S::kQueryBytes, lambda_lds = lds0 + S::kLambdaOff + wave * kWave * 4;
@@ -443,7 +449,7 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
   }
 
   // ---- the range
-  u32x4 q[2 * KS];
+  u32x4 q[NB * KS];
   f32x4 o[NB][MB];
   float m[NB], l[NB];
   float lam = 0.0f;
@@ -475,23 +481,16 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
       lam = lambda_mem[head < heads ? head : 0];
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
-        if constexpr (S::kQueryLds) {
-          const char* row = query_mem + head * S::kRow + g * 16 + kk * 64;
-          if constexpr (NB == 1) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(row + (c16 >> 3) * (2 * D));
-            q[kk] = head < heads && c16 < 8 ? x : u32x4{0, 0, 0, 0};
-            q[KS + kk] = head < heads && c16 >= 8 ? x : u32x4{0, 0, 0, 0};
-          } else {
-            const u32x4 x0 = *reinterpret_cast<const u32x4*>(row), x1 = *reinterpret_cast<const u32x4*>(row + 2 * D);
-            q[kk] = head < heads ? x0 : u32x4{0, 0, 0, 0};
-            q[KS + kk] = head < heads ? x1 : u32x4{0, 0, 0, 0};
-          }
+        if constexpr (S::kQueryLds) {   // (the lane's column belongs to map c16 / 8)
+          q[kk] = *reinterpret_cast<const u32x4*>(query_mem + head * S::kRow + (c16 >> 3) * (2 * D) + g * 16 + kk * 64);
         } else {
           const char* row = a.q + cc.b * a.q_stride_bytes + static_cast<int64_t>(head0 + (head < heads ? head : 0)) * S::kRow +
                             g * 16 + kk * 64;
+          // (columns without a head hold zeros; with the loads' registers used as they are the compiler moves them to
+          // and from accumulation registers in the loop: 142 instead of 128 us for 64 sequences and 64 heads of 128 dims)
           const u32x4 x0 = ldg16(row), x1 = ldg16(row + 2 * D);
           q[kk] = head < heads ? x0 : u32x4{0, 0, 0, 0};
-          q[KS + kk] = head < heads ? x1 : u32x4{0, 0, 0, 0};
+          q[(NB - 1) * KS + kk] = head < heads ? x1 : u32x4{0, 0, 0, 0};
         }
       }
 #pragma unroll
@@ -523,10 +522,12 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_decode_kernel(DiffArgs a
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
         s0 = Mfma<QT>::k32(kr[kk], q[kk], s0);
-        s1 = Mfma<QT>::k32(kr[KS + kk], q[KS + kk], s1);
+        s1 = Mfma<QT>::k32(kr[KS + kk], q[(NB - 1) * KS + kk], s1);
       }
       if constexpr (NB == 1) {
-        sc[0] = s0 + s1;   // (each is zero in the other's columns)
+        // (both maps' keys met every column's queries: a column keeps its own map's scores)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[0][r] = c16 < 8 ? s0[r] : s1[r];
       } else {
         sc[0] = s0;
         sc[NB - 1] = s1;
@@ -746,7 +747,7 @@ int launch_diff(const DiffArgs& a, hipStream_t stream) {
                                              static_cast<int>(S::lds_bytes(kDiffMaxBatch)));
     if (e != hipSuccess) return static_cast<int>(e);
   }
-  launch_timed(diff_decode_kernel<QT, D, NB>, dim3(static_cast<unsigned>(a.n_workers / kDiffWaves)), dim3(kDiffThreads),
+  launch_timed(diff_decode_kernel<QT, D, NB>, dim3(static_cast<unsigned>(a.n_workers / S::kWaves)), dim3(S::kThreads),
                S::lds_bytes(a.batch), stream, a);
   int rc = static_cast<int>(hipGetLastError());
   if (rc != 0) return rc;
@@ -770,13 +771,18 @@ int dispatch_diff(const DiffArgs& a, int64_t head_dim, hipStream_t stream) {
 
 size_t diff_prefix_bytes() { return (static_cast<size_t>(kDiffMaxBatch + 1) * 4 + 255) / 256 * 256; }
 int64_t diff_columns(int64_t group) { return group <= 8 ? 16 : 32; }
+int64_t diff_workers(int64_t head_dim, int64_t group) {
+  const int waves = head_dim == 64 ? (group <= 8 ? DiffShape<64, 1>::kWaves : DiffShape<64, 2>::kWaves)
+                                   : (group <= 8 ? DiffShape<128, 1>::kWaves : DiffShape<128, 2>::kWaves);
+  return static_cast<int64_t>(device_cu_count()) * waves;
+}
 
 }  // namespace
 
 // prefix | maxima and sums | partial rows, two slots per worker
 size_t diff_workspace_bytes(int64_t n_heads, int64_t n_pairs, int64_t head_dim) {
   if (n_heads <= 0 || n_pairs <= 0 || n_heads % n_pairs != 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  const size_t cols = static_cast<size_t>(device_cu_count()) * kDiffWaves * 2 * diff_columns(n_heads / n_pairs);
+  const size_t cols = static_cast<size_t>(diff_workers(head_dim, n_heads / n_pairs) * 2 * diff_columns(n_heads / n_pairs));
   return diff_prefix_bytes() + cols * 2 * 4 + cols * 2 * head_dim * 4;
 }
 
@@ -831,7 +837,7 @@ int paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, v
   const bool long_table = table_width > (0x7fffffffLL - 16) / block_size;
   a.max_len = long_table ? 0x7fffffff - 16 : static_cast<int>(table_width * block_size);
   a.window_left = window_left < 0 ? -1 : static_cast<int>(window_left < 0x7fffffffLL ? window_left : 0x7fffffffLL);
-  a.n_workers = device_cu_count() * kDiffWaves;
+  a.n_workers = static_cast<int>(diff_workers(head_dim, a.group));
   a.pools = device_cu_count() == 256 ? 1 : 0;
   const int64_t head_blocks = n_kv_pairs * a.hb_per_pair;
   a.team_shift = head_blocks % 4 == 0 ? 2 : head_blocks % 2 == 0 ? 1 : 0;

@@ -65,17 +65,18 @@ def _check_plan(plan):
 
 
 def _require_cuda(*tensors):
-    dev = None
+    index = first = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError("this path runs on the GPU only: every tensor must be a device tensor")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError("all tensors must live on the same device")
-    return dev
+        i = t.get_device()   # (-1 on the host)
+        if i != index:
+            if i < 0:
+                raise ValueError("this path runs on the GPU only: every tensor must be a device tensor")
+            if index is not None:
+                raise ValueError("all tensors must live on the same device")
+            index, first = i, t
+    return None if first is None else first.device
 
 
 # ------------------------------------------------------------------------------------------
@@ -819,7 +820,7 @@ def absorbed_bmm(x, w, out=None):
 def _launch(dev, name, *args):
     """The entry point `name` of the library on dev's current stream, with dev as the current device."""
     fn = getattr(capi.lib(), name)
-    if torch.cuda.current_device() == dev.index:
+    if torch._C._cuda_getDevice() == dev.index:
         return fn(*args, _stream(dev))
     with torch.cuda.device(dev):
         return fn(*args, _stream(dev))
