@@ -1,0 +1,105 @@
+"""The operators of a step through the C++ host side (torch.ops.xllm_ops.*): the same bits as xllm_amd.ops, and refusals."""
+import pytest
+import torch
+
+from xllm_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def xops():
+    from xllm_amd import torch_ops
+    return torch_ops.load()
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def test_step_tables(xops):
+    kv, new, free, head = i32([5, 0, 33, 16]), i32([1, 20, 1, 0]), torch.arange(50, 90, dtype=torch.int32, device=DEV), i32([3])
+    table = torch.randint(0, 50, (4, 6), device=DEV).to(torch.int32)
+    want = ops.build_step_tables(kv, new, table, free, 16, 24, head)
+    names = list(ops.StepTables.__dataclass_fields__)
+    got = xops.build_step_tables(kv, new, table, free, 16, 24, head)
+    for name, g in zip(names, got):
+        assert torch.equal(g, getattr(want, name)), name
+    outs = [torch.empty_like(g) for g in got]
+    outs[0].copy_(table)
+    xops.build_step_tables_out(kv, new, outs[0], free, 16, 24, head, *outs)   # the table in place
+    for name, g in zip(names, outs):
+        assert torch.equal(g, getattr(want, name)), name
+    for bad in ((kv.long(), new, table, free, 16, 24), (kv, new[:3], table, free, 16, 24), (kv, new, table, free, 0, 24),
+                (kv, new, table[:3], free, 16, 24), (kv, new, table, free.cpu(), 16, 24)):
+        with pytest.raises((ValueError, TypeError)):
+            xops.build_step_tables(*bad)
+
+
+def test_rows_and_rotation(xops):
+    inv, factor = ops.rope_frequencies(64, scaling=ops.RopeScaling("yarn", factor=4.0, original_max_position=64), device=DEV)
+    pos = torch.randint(0, 300, (21,), device=DEV)
+    rows = xops.build_cos_sin_cache(inv, None, 300, 0, factor, torch.float32)
+    assert torch.equal(rows, ops.build_cos_sin_cache(inv, 300, attention_factor=factor))
+    assert torch.equal(xops.build_cos_sin_cache(inv, pos, 0, 0, factor, torch.float32), rows[pos])
+    q, k = torch.randn(21, 6, 96, device=DEV).to(BF16), torch.randn(21, 2, 64, device=DEV).to(BF16)
+    for interleave in (False, True):
+        for inverse in (False, True):
+            want = ops.rotary_embedding(pos, q, k, rows, interleave=interleave, rotary_offset=32, key_rotary_offset=0,
+                                        inverse=inverse, out_query=torch.empty_like(q), out_key=torch.empty_like(k))
+            oq, ok, iq, ik = torch.empty_like(q), torch.empty_like(k), q.clone(), k.clone()
+            xops.rotary_embedding(pos, q, k, rows, interleave, 32, 0, inverse, oq, ok)
+            xops.rotary_embedding(pos, iq, ik, rows, interleave, 32, 0, inverse)
+            for a, b in ((oq, want[0]), (ok, want[1]), (iq, want[0]), (ik, want[1])):
+                assert torch.equal(a, b)
+    alone = q.clone()
+    xops.rotary_embedding(pos, alone, None, rows)
+    assert torch.equal(alone, ops.rotary_embedding(pos, q.clone(), None, rows)[0])
+    for bad in ((pos.int(), q, k, rows), (pos, q, k.float(), rows), (pos, q, k[:3], rows), (pos, q, k, rows.double()),
+                (pos, q, q, rows), (pos, q.transpose(1, 2), None, rows)):
+        with pytest.raises((ValueError, TypeError)):
+            xops.rotary_embedding(*bad)
+    with pytest.raises((ValueError, TypeError)):
+        xops.build_cos_sin_cache(inv.float(), None, 10, 0, 1.0, torch.float32)
+    with pytest.raises((ValueError, TypeError)):
+        xops.build_cos_sin_cache(inv, None, 0, 0, 1.0, torch.float32)
+
+
+def test_mla_prologue(xops):
+    T, H = 9, 5
+    q, kv, w = torch.randn(T, H, 192, device=DEV).to(BF16), torch.randn(T, 576, device=DEV).to(BF16), torch.ones(512, dtype=BF16, device=DEV)
+    inv, _ = ops.rope_frequencies(64, device=DEV)
+    rows, pos = ops.build_cos_sin_cache(inv, 50), torch.randint(0, 50, (T,), device=DEV)
+    slots = torch.randperm(32, device=DEV)[:T].to(torch.int32)
+    caches = [torch.zeros(2, 16, 1, 576, dtype=BF16, device=DEV) for _ in range(2)]
+    oq = [torch.empty(T, H, 64, dtype=BF16, device=DEV) for _ in range(2)]
+    okv = [torch.empty_like(kv) for _ in range(2)]
+    ops.mla_norm_rope_and_cache(q[..., 128:], kv, w, 1e-6, rows, True, pos, k_cache=caches[0], slot_mapping=slots,
+                                out_q_pe=oq[0], out_kv=okv[0])
+    xops.mla_norm_rope_and_cache(q[..., 128:], kv, w, 1e-6, rows, True, pos, caches[1], slots, oq[1], okv[1])
+    assert torch.equal(*caches) and torch.equal(*oq) and torch.equal(*okv)
+    for change in (dict(slot_mapping=None), dict(k_cache=None), dict(kv=kv[:, :575]), dict(position_ids=pos.int()), dict(kv=kv.float())):
+        args = dict(q_pe=q[..., 128:], kv=kv, kv_norm_weight=w, eps=1e-6, cos_sin_cache=rows, interleave=True, position_ids=pos,
+                    k_cache=caches[0], slot_mapping=slots)
+        args.update(change)
+        with pytest.raises((ValueError, TypeError)):
+            xops.mla_norm_rope_and_cache(**args)
+
+
+def test_differential_decode(xops):
+    B, H, pairs, D, bs, P = 3, 4, 2, 64, 16, 20
+    q = torch.randn(B, 2 * H, D, device=DEV).to(BF16)
+    k, v = torch.randn(P, bs, 2 * pairs, D, device=DEV).to(BF16), torch.randn(P, bs, pairs, 2 * D, device=DEV).to(BF16)
+    table, lens = torch.randperm(P, device=DEV)[:18].view(3, 6).to(torch.int32), i32([90, 0, 17])
+    lam, w = torch.rand(B, H, device=DEV), torch.ones(2 * D, dtype=BF16, device=DEV)
+    want, got = torch.empty(B, H, 2 * D, dtype=BF16, device=DEV), torch.empty(B, H, 2 * D, dtype=BF16, device=DEV)
+    for weight, window, lm in ((w, -1, lam), (None, 20, lam[0].contiguous()), (w, -1, lam[:1, :1])):
+        ops.batch_decode_diff(q, k, v, want, table, lens, lm, scale=0.2, norm_weight=weight, eps=1e-6, out_scale=0.5, window_left=window)
+        xops.batch_decode_diff(q, k, v, got, table, lens, lm, 0.2, weight, 1e-6, 0.5, window)
+        assert torch.equal(got, want)
+    for bad in ((q[:, :7], k, v, got, table, lens, lam, 0.2), (q, k, k, got, table, lens, lam, 0.2), (q, k, v, got, table, lens.long(), lam, 0.2),
+                (q, k, v, got, table, lens, lam.double(), 0.2), (q, k, v, got.float(), table, lens, lam, 0.2), (q, k, v, got, table, lens, lam, -1.0)):
+        with pytest.raises((ValueError, TypeError)):
+            xops.batch_decode_diff(*bad)

@@ -112,8 +112,8 @@ SHIM_LIB = os.path.join(HERE, "libxllm_mi355_torch.so")
 
 def build_shim(force=True, verbose=True):
     """The C++ host side (torch::Tensor interface + torch op registration) over the C ABI."""
-    src = os.path.join(CSRC, "shim", "ops_api.cpp")
-    deps = [src, os.path.join(CSRC, "shim", "ops_api.h"), os.path.join(HERE, "..", "include", "xllm_mi355.h")]
+    srcs = [os.path.join(CSRC, "shim", f) for f in ("ops_api.cpp", "step_ops.cpp")]
+    deps = [*srcs, os.path.join(CSRC, "shim", "ops_api.h"), os.path.join(HERE, "..", "include", "xllm_mi355.h")]
     if not force and not _stale(SHIM_LIB, deps):
         return SHIM_LIB
     import torch
@@ -125,7 +125,7 @@ def build_shim(force=True, verbose=True):
     libdir = os.path.join(os.path.dirname(torch.__file__), "lib")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", *incs, "-o", SHIM_LIB, src,
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", *incs, "-o", SHIM_LIB, *srcs,
            f"-L{HERE}", "-lxllm_mi355", "-Wl,-rpath,$ORIGIN", f"-L{libdir}", f"-Wl,-rpath,{libdir}",
            "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"]
     if verbose:

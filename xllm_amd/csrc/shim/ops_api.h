@@ -164,6 +164,49 @@ struct LlmDecodeMetadataUpdateParams {
 };
 void update_llm_decode_metadata(const LlmDecodeMetadataUpdateParams& params, void* stream);
 
+// ---- operators around the path (step_ops.cpp); layouts and meaning as in include/xllm_mi355.h --------------------------
+
+// The tables of a step from the requests' lengths, on the device (the host's part of
+// xllm/core/framework/batch/batch_input_builder.cpp).  kv_lens, new_lens [B] and free_pages [F] int32, block_table [B, W]
+// int32.  Tensors of `out` that are defined are written into (block_table may be the input itself), the others allocated.
+struct StepTables {
+  torch::Tensor block_table;       // [B, W] int32
+  torch::Tensor seq_lens;          // [B] int32
+  torch::Tensor q_cu_seq_lens;     // [B + 1] int32
+  torch::Tensor position_ids;      // [max_new_tokens] int64
+  torch::Tensor slot_mapping;      // [max_new_tokens] int32
+  torch::Tensor new_page_indptr;   // [B + 1] int32
+  torch::Tensor counters;          // [3] int32: tokens of the step, free head of the next step, tokens without a page
+};
+void build_step_tables(const torch::Tensor& kv_lens, const torch::Tensor& new_lens, const torch::Tensor& block_table,
+                       const torch::Tensor& free_pages, int64_t block_size, int64_t max_new_tokens,
+                       const std::optional<torch::Tensor>& free_head, StepTables& out);
+
+// cos | sin rows [rows, 2 * inv_freq.numel()] of position_ids, or of num_positions positions from first_position on.
+torch::Tensor build_cos_sin_cache(const torch::Tensor& inv_freq, const std::optional<torch::Tensor>& position_ids,
+                                  int64_t num_positions, int64_t first_position, double attention_factor,
+                                  torch::ScalarType dtype, const std::optional<torch::Tensor>& out = std::nullopt);
+
+// Rotation of query [T, Hq, D] and key [T, Hk, D'] (may be undefined), into out_query / out_key or in place.
+void rotary_embedding(const torch::Tensor& position_ids, const torch::Tensor& query, const std::optional<torch::Tensor>& key,
+                      const torch::Tensor& cos_sin_cache, bool interleave, int64_t rotary_offset,
+                      std::optional<int64_t> key_rotary_offset, bool inverse, const std::optional<torch::Tensor>& out_query,
+                      const std::optional<torch::Tensor>& out_key);
+
+// The MLA prologue: latent norm, rotation of rope key and query part, latent store.
+void mla_norm_rope_and_cache(const torch::Tensor& q_pe, const torch::Tensor& kv, const torch::Tensor& kv_norm_weight,
+                             double eps, const torch::Tensor& cos_sin_cache, bool interleave,
+                             const torch::Tensor& position_ids, const std::optional<torch::Tensor>& k_cache,
+                             const std::optional<torch::Tensor>& slot_mapping, const std::optional<torch::Tensor>& out_q_pe,
+                             const std::optional<torch::Tensor>& out_kv);
+
+// Differential attention of one new token per sequence: query [B, 2 H, D], k_cache [P, bs, 2 pairs, D], v_cache
+// [P, bs, pairs, 2 D], output [B, H, 2 D], lambda one value, [H] or [B, H] fp32.
+void batch_decode_diff(const torch::Tensor& query, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                       torch::Tensor& output, const torch::Tensor& block_table, const torch::Tensor& seq_lens,
+                       const torch::Tensor& lambda, double scale, const std::optional<torch::Tensor>& norm_weight,
+                       double eps, double out_scale, int64_t window_left = -1);
+
 }  // namespace mi355
 
 // The reference's own namespace, types and signature (xllm/core/kernels/dcu/flash_mla_adapter.h:29-53): a caller

@@ -26,7 +26,6 @@ Operators around the path that the reference does on the host, in its layers or 
 
 Errors: the reference CHECK-aborts; here every violated precondition raises.
 """
-import ctypes
 import functools
 import math
 from dataclasses import dataclass
@@ -817,24 +816,11 @@ def absorbed_bmm(x, w, out=None):
 # ------------------------------------------------------------------------------------------
 # the tables of a step
 
-def _launch(dev, name, *args):
-    """The entry point `name` of the library on dev's current stream, with dev as the current device."""
-    fn = getattr(capi.lib(), name)
-    if torch._C._cuda_getDevice() == dev.index:
-        return fn(*args, _stream(dev))
-    with torch.cuda.device(dev):
-        return fn(*args, _stream(dev))
-
-
-_EINVAL = -1
-
-
-def _check_launch(rc, name, what):
-    """The library refuses operands that overlap; `what` says so in the words of the Python call, whose other arguments
-    were found good before."""
-    if rc == _EINVAL:
-        raise ValueError(what)
-    capi.check(rc, name)
+@functools.lru_cache(maxsize=None)
+def _host_side(name):
+    """The dispatcher's entry of the C++ host side: it checks the arguments (ValueError, TypeError) and launches."""
+    from . import torch_ops
+    return getattr(torch_ops.load(), name).default
 
 
 @dataclass
@@ -852,9 +838,6 @@ class StepTables:
     counters: torch.Tensor
 
 
-_I32_FIELDS = ("block_table", "seq_lens", "q_cu_seq_lens", "slot_mapping", "new_page_indptr", "counters")
-
-
 def build_step_tables(kv_lens, new_lens, block_table, free_pages, block_size, max_new_tokens, free_head=None, out=None):
     """The tables of a step on the GPU, from the requests' lengths: no host loop, no copy, capturable.
     kv_lens [B] int32: tokens in the cache; new_lens [B] int32: tokens this step brings (1 for a decode, a chunk for a
@@ -866,58 +849,12 @@ def build_step_tables(kv_lens, new_lens, block_table, free_pages, block_size, ma
     attend before its tokens are stored.
     out: StepTables to write into (the persistent buffers of a captured step); its block_table may be block_table itself.
     Returns StepTables."""
-    dev = _require_cuda(kv_lens, new_lens, block_table, free_pages, free_head)
-    i32 = torch.int32
-    for name, t in (("kv_lens", kv_lens), ("new_lens", new_lens), ("free_pages", free_pages)):
-        if t.dtype != i32 or t.dim() != 1 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 vector")
-    B, F, T, block_size = kv_lens.numel(), free_pages.numel(), int(max_new_tokens), int(block_size)
-    if new_lens.numel() != B:
-        raise ValueError("kv_lens and new_lens must have one entry per request")
-    if block_table.dtype != i32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] == 0 or \
-            block_table.stride(1) != 1:
-        raise ValueError("block_table must be int32 [B, W] with unit column stride, one row per request")
-    if free_head is not None and (free_head.dtype != i32 or free_head.numel() != 1):
-        raise ValueError("free_head must be int32 [1]")
-    if block_size <= 0 or T < 0:
-        raise ValueError("block_size must be positive and max_new_tokens not negative")
-    W = block_table.shape[1]
-    in_stride = block_table.stride(0) if B > 1 else W
-    if in_stride < W:
-        raise ValueError("block_table: rows must not overlap")
     if out is None:
-        seq_lens, cu, indptr, counters, slots = torch.empty(3 * B + 5 + T, dtype=i32, device=dev).split(
-            (B, B + 1, B + 1, 3, T))
-        out = StepTables(torch.empty((B, W), dtype=i32, device=dev), seq_lens, cu,
-                         torch.empty(T, dtype=torch.int64, device=dev), slots, indptr, counters)
-        out_stride = W
-    else:
-        fields = [getattr(out, f) for f in _I32_FIELDS]
-        _require_cuda(kv_lens, out.position_ids, *fields)
-        sizes = dict(seq_lens=B, q_cu_seq_lens=B + 1, slot_mapping=T, new_page_indptr=B + 1, counters=3)
-        for f, t in zip(_I32_FIELDS, fields):
-            if t.dtype != i32 or (f in sizes and (tuple(t.shape) != (sizes[f],) or not t.is_contiguous())):
-                raise ValueError(f"out.{f} must be contiguous int32 of its documented size")
-        if out.position_ids.dtype != torch.int64 or tuple(out.position_ids.shape) != (T,) or \
-                not out.position_ids.is_contiguous():
-            raise ValueError("out.position_ids must be contiguous int64 [max_new_tokens]")
-        tab = out.block_table
-        out_stride = tab.stride(0) if B > 1 else W
-        if tuple(tab.shape) != (B, W) or tab.stride(1) != 1 or out_stride < W:
-            raise ValueError("out.block_table must be [B, W] with unit column stride")
-    if B == 0:
-        for t in (out.q_cu_seq_lens, out.new_page_indptr, out.counters, out.position_ids):
-            t.zero_()
-        if free_head is not None:
-            out.counters[1:2].copy_(free_head.view(1).clamp(0, F))
-        out.slot_mapping.fill_(-1)
-        return out
-    rc = _launch(dev, "xllm_mi355_build_step_tables", kv_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
-                 in_stride, out.block_table.data_ptr(), out_stride, W, free_pages.data_ptr(), F, _ptr(free_head),
-                 out.seq_lens.data_ptr(), out.q_cu_seq_lens.data_ptr(), out.position_ids.data_ptr(),
-                 out.slot_mapping.data_ptr(), out.new_page_indptr.data_ptr(), out.counters.data_ptr(), B, block_size, T)
-    _check_launch(rc, "xllm_mi355_build_step_tables",
-                  "an output of build_step_tables overlaps an input or another output (in place means block_table itself)")
+        return StepTables(*_host_side("build_step_tables")(kv_lens, new_lens, block_table, free_pages, int(block_size),
+                                                           int(max_new_tokens), free_head))
+    _host_side("build_step_tables_out")(kv_lens, new_lens, block_table, free_pages, int(block_size), int(max_new_tokens),
+                                        free_head, out.block_table, out.seq_lens, out.q_cu_seq_lens, out.position_ids,
+                                        out.slot_mapping, out.new_page_indptr, out.counters)
     return out
 
 
@@ -1002,64 +939,8 @@ def build_cos_sin_cache(inv_freq, num_positions=0, position_ids=None, first_posi
     bits, rounded once to dtype (float32, bfloat16 or float16).  Rows of position_ids [rows] int64 -- one step's rows,
     shared by all layers, which then index them by 0 .. rows - 1 -- or of first_position .. first_position + num_positions - 1.
     inv_freq, attention_factor: from rope_frequencies.  Returns the rows (out, if given)."""
-    dev = _require_cuda(inv_freq, position_ids, out)
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.numel() == 0:
-        raise ValueError("inv_freq must be a contiguous float64 vector (rope_frequencies)")
-    if position_ids is not None:
-        if position_ids.dtype != torch.int64 or position_ids.dim() != 1 or not position_ids.is_contiguous():
-            raise ValueError("position_ids must be a contiguous int64 vector")
-        if first_position != 0 or num_positions not in (0, position_ids.numel()):
-            raise ValueError("give position_ids or a range of positions, not both")
-        rows = position_ids.numel()
-    else:
-        rows = int(num_positions)
-        if rows <= 0 or first_position < 0:
-            raise ValueError("num_positions must be positive and first_position not negative")
-    shape = (rows, 2 * inv_freq.numel())
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
-    elif tuple(out.shape) != shape or not out.is_contiguous():
-        raise ValueError("out must be contiguous [rows, rotary_dim]")
-    if out.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError("cos_sin rows are float32, bfloat16 or float16")
-    if rows == 0:
-        return out
-    rc = _launch(dev, "xllm_mi355_rope_cos_sin", inv_freq.data_ptr(), _ptr(position_ids), int(first_position), rows,
-                 inv_freq.numel(), float(attention_factor), out.data_ptr(), _dtype_code(out))
-    _check_launch(rc, "xllm_mi355_rope_cos_sin", "out overlaps an input")
-    return out
-
-
-_Strides = ctypes.c_int64 * 2
-
-
-def _check_cos_sin(cos_sin_cache, position_ids, n_tokens):
-    if position_ids.dtype != torch.int64 or not position_ids.is_contiguous() or position_ids.numel() != n_tokens:
-        raise ValueError("position_ids must be a contiguous int64 tensor [tokens]")
-    if cos_sin_cache.dim() != 2 or not cos_sin_cache.is_contiguous() or cos_sin_cache.shape[0] == 0:
-        raise ValueError("cos_sin_cache must be [max_position, rotary_dim], contiguous")
-    if cos_sin_cache.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError("cos_sin_cache must be float32, bfloat16 or float16")
-
-
-def _check_rotated(name, x, out):
-    """x [T, H, D] and where its result goes: their shape, and {token, head} strides for the library (0 where there is only
-    one of them: its stride then means nothing)."""
-    if x.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim]")
-    T, H, D = x.shape
-    ts, hs, es = x.stride()
-    if H == 0 or D == 0 or (es != 1 and T > 0):
-        raise ValueError(f"{name} must be [tokens, heads, head_dim], contiguous in its last dim")
-    strides = _Strides(ts if T > 1 else 0, hs if H > 1 else 0)
-    if out is x:
-        return T, H, D, strides, strides
-    if out.shape != x.shape or out.dtype != x.dtype:
-        raise ValueError(f"out_{name} must have {name}'s shape and dtype")
-    ts, hs, es = out.stride()
-    if es != 1 and T > 0:
-        raise ValueError(f"out_{name} must be contiguous in its last dim")
-    return T, H, D, strides, _Strides(ts if T > 1 else 0, hs if H > 1 else 0)
+    return _host_side("build_cos_sin_cache")(inv_freq, position_ids, int(num_positions), int(first_position),
+                                             float(attention_factor), dtype, out)
 
 
 def rotary_embedding(position_ids, query, key, cos_sin_cache, interleave=False, rotary_offset=0, key_rotary_offset=None,
@@ -1071,36 +952,9 @@ def rotary_embedding(position_ids, query, key, cos_sin_cache, interleave=False, 
     interleave: pairs (2i, 2i + 1), else (i, i + rotary_dim / 2).  inverse: the transposed map, which undoes a rotation by
     unscaled rows and turns the gradient of the result into the gradient of the input.
     Works in place, or into out_query / out_key.  Returns (query's result, key's result or None)."""
-    dev = _require_cuda(position_ids, query, key, cos_sin_cache, out_query, out_key)
-    oq = query if out_query is None else out_query
-    ok = key if out_key is None else out_key
-    if key is None and out_key is not None:
-        raise ValueError("out_key without a key")
-    code = _dtype_code(query)
-    if code == capi.FP8_E4M3:
-        raise TypeError("query must be bfloat16, float16 or float32")
-    T, Hq, D, q_st, oq_st = _check_rotated("query", query, oq)
-    _check_cos_sin(cos_sin_cache, position_ids, T)
-    rows, R = cos_sin_cache.shape
-    k_off = rotary_offset if key_rotary_offset is None else key_rotary_offset
-    Hk = Dk = 0
-    k_st = ok_st = None
-    if key is not None:
-        Tk, Hk, Dk, k_st, ok_st = _check_rotated("key", key, ok)
-        if Tk != T or key.dtype != query.dtype:
-            raise ValueError("key must have query's tokens and dtype")
-    if R % 2 != 0 or R == 0:
-        raise ValueError("the rotary dim must be even")
-    if rotary_offset < 0 or rotary_offset + R > D or (Hk and (k_off < 0 or k_off + R > Dk)):
-        raise ValueError("the rotated part must lie inside the head")
-    if T == 0:
-        return oq, ok
-    rc = _launch(dev, "xllm_mi355_rotary_embedding", position_ids.data_ptr(), cos_sin_cache.data_ptr(), rows,
-                 query.data_ptr(), oq.data_ptr(), _ptr(key), _ptr(ok), T, Hq, Hk, D, Dk, rotary_offset, k_off if Hk else 0, R,
-                 q_st, oq_st, k_st, ok_st, 1 if interleave else 0, 1 if inverse else 0, code, _dtype_code(cos_sin_cache))
-    _check_launch(rc, "xllm_mi355_rotary_embedding",
-                  "a result of rotary_embedding overlaps itself, the other one or an input (in place means the operand itself)")
-    return oq, ok
+    _host_side("rotary_embedding")(position_ids, query, key, cos_sin_cache, bool(interleave), rotary_offset,
+                                   key_rotary_offset, bool(inverse), out_query, out_key)
+    return query if out_query is None else out_query, key if out_key is None else out_key
 
 
 def mla_norm_rope_and_cache(q_pe, kv, kv_norm_weight, eps, cos_sin_cache, interleave, position_ids, k_cache=None,
@@ -1111,66 +965,13 @@ def mla_norm_rope_and_cache(q_pe, kv, kv_norm_weight, eps, cos_sin_cache, interl
     (negative slots and slots beyond the cache are skipped) and / or to out_kv [T, 576] (kv itself: in place).
     out_q_pe [T, H, 64]: contiguous is what dense_decode reads; None: in place.  bfloat16 or float16.
     Returns (q_pe's result, out_kv)."""
-    dev = _require_cuda(q_pe, kv, kv_norm_weight, cos_sin_cache, position_ids, k_cache, slot_mapping, out_q_pe, out_kv)
-    oq = q_pe if out_q_pe is None else out_q_pe
-    dtype = q_pe.dtype
-    if dtype != torch.bfloat16 and dtype != torch.float16:
-        raise TypeError("q_pe must be bfloat16 or float16")
-    T, H, d_rope, q_st, oq_st = _check_rotated("q_pe", q_pe, oq)
-    d_latent = kv_norm_weight.numel()
-    row = d_latent + d_rope
-    if kv.dim() != 2 or kv.shape[0] != T or kv.shape[1] != row or (T > 0 and kv.stride(1) != 1):
-        raise ValueError("kv must be [tokens, latent + rope dims] with contiguous rows")
-    if kv.dtype != dtype or kv_norm_weight.dtype != dtype or not kv_norm_weight.is_contiguous():
-        raise TypeError("kv and kv_norm_weight must have q_pe's dtype, the weight contiguous")
-    _check_cos_sin(cos_sin_cache, position_ids, T)
-    if cos_sin_cache.shape[1] != d_rope:
-        raise ValueError("cos_sin_cache must have the rope dims")
-    if (k_cache is None) != (slot_mapping is None):
-        raise ValueError("k_cache and slot_mapping come together")
-    if k_cache is None and out_kv is None:
-        raise ValueError("the latent rows need a place: k_cache or out_kv")
-    out_row = blocks = block_size = 0
-    if out_kv is not None:
-        if out_kv.shape != kv.shape or out_kv.dtype != dtype or (T > 0 and out_kv.stride(1) != 1):
-            raise ValueError("out_kv must have kv's shape and dtype, with contiguous rows")
-        out_row = out_kv.stride(0) if T > 1 else row
-        if out_row < row:
-            raise ValueError("out_kv: rows must not overlap")
-    if k_cache is not None:
-        if k_cache.dim() != 4 or k_cache.shape[2] != 1 or k_cache.shape[3] != row or k_cache.dtype != dtype or \
-                not k_cache.is_contiguous():
-            raise ValueError("k_cache must be contiguous [P, bs, 1, latent + rope dims] of kv's dtype")
-        if slot_mapping.dtype != torch.int32 or not slot_mapping.is_contiguous() or slot_mapping.numel() != T:
-            raise ValueError("slot_mapping must be contiguous int32 [tokens]")
-        blocks, block_size = k_cache.shape[0], k_cache.shape[1]
-        if blocks == 0 or block_size == 0:
-            raise ValueError("k_cache is empty")
-    if T == 0:
-        return oq, out_kv
-    kv_row = kv.stride(0) if T > 1 else row
-    if kv_row < row:
-        raise ValueError("kv: rows must not overlap")
-    if eps < 0:
-        raise ValueError("eps must not be negative")
-    rc = _launch(dev, "xllm_mi355_mla_norm_rope_and_cache", q_pe.data_ptr(), oq.data_ptr(), kv.data_ptr(), _ptr(out_kv),
-                 kv_norm_weight.data_ptr(), float(eps), cos_sin_cache.data_ptr(), cos_sin_cache.shape[0],
-                 position_ids.data_ptr(), _ptr(k_cache), _ptr(slot_mapping), T, H, d_latent, d_rope, q_st[0], q_st[1],
-                 oq_st[0], oq_st[1], kv_row, out_row, block_size, blocks, 1 if interleave else 0, _dtype_code(q_pe),
-                 _dtype_code(cos_sin_cache))
-    _check_launch(rc, "xllm_mi355_mla_norm_rope_and_cache",
-                  "a result of mla_norm_rope_and_cache overlaps itself, another one or an input (in place means the operand itself)")
-    return oq, out_kv
+    _host_side("mla_norm_rope_and_cache")(q_pe, kv, kv_norm_weight, float(eps), cos_sin_cache, bool(interleave), position_ids,
+                                          k_cache, slot_mapping, out_q_pe, out_kv)
+    return q_pe if out_q_pe is None else out_q_pe, out_kv
 
 
 # ------------------------------------------------------------------------------------------
 # differential attention
-
-@functools.lru_cache(maxsize=256)
-def _diff_workspace_bytes(dev, n_heads, n_pairs, head_dim):
-    with torch.cuda.device(dev):   # (the size goes by the device's compute units)
-        return int(capi.lib().xllm_mi355_paged_decode_diff_workspace_bytes(n_heads, n_pairs, head_dim))
-
 
 def batch_decode_diff(query, k_cache, v_cache, output, block_table, seq_lens, lambda_, scale=None, norm_weight=None,
                       eps=1e-5, out_scale=1.0, window_left=-1):
@@ -1183,67 +984,7 @@ def batch_decode_diff(query, k_cache, v_cache, output, block_table, seq_lens, la
     batch_decode: an empty sequence gets zeros, a context beyond the table is cut there.  lambda_: the layer's learned
     weight as float32, one value, [H], or [B, H].  norm_weight [2 D] of query's dtype; out_scale: usually 1 - lambda_init.
     window_left >= 0: the last window_left + 1 tokens only.  bfloat16 or float16; D 64 or 128.  Returns output."""
-    dev = _require_cuda(query, k_cache, v_cache, output, block_table, seq_lens, lambda_, norm_weight)
-    dtype = query.dtype
-    if query.dim() != 3 or query.shape[1] % 2 != 0 or query.shape[1] == 0:
-        raise ValueError("query must be [B, 2 H, D]")
-    if dtype != torch.bfloat16 and dtype != torch.float16:
-        raise TypeError("query must be bfloat16 or float16")
-    B, H2, D = query.shape
-    H = H2 // 2
-    q_row, q_head, q_elem = query.stride()
-    if q_elem != 1 or q_head != D:
-        raise ValueError("query: last two dims must be contiguous")
-    if output.dim() != 3 or output.dtype != dtype or tuple(output.shape) != (B, H, 2 * D):
-        raise ValueError("output must be [B, H, 2 D] of query's dtype")
-    o_row, o_head, o_elem = output.stride()
-    if o_elem != 1 or (H > 1 and o_head != 2 * D) or (B > 1 and o_row < H2 * D):
-        raise ValueError("output: last two dims must be contiguous and rows apart")
-    if k_cache.dim() != 4 or not k_cache.is_contiguous():
-        raise ValueError("k_cache must be contiguous [P, bs, 2 pairs, D]")
-    P, bs, k_heads, k_dim = k_cache.shape
-    pairs = k_heads // 2
-    if k_heads % 2 != 0 or k_dim != D or P == 0 or bs == 0 or pairs == 0:
-        raise ValueError("k_cache must be contiguous [P, bs, 2 pairs, D]")
-    if tuple(v_cache.shape) != (P, bs, pairs, 2 * D) or not v_cache.is_contiguous():
-        raise ValueError("v_cache must be contiguous [P, bs, pairs, 2 D]")
-    if k_cache.dtype != dtype or v_cache.dtype != dtype:
-        raise TypeError("the caches must have query's dtype")
-    if H % pairs != 0:
-        raise ValueError("the heads must be a multiple of the KV pairs")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or \
-            block_table.shape[1] == 0 or block_table.stride(1) != 1:
-        raise ValueError("block_table must be int32 [B, W] with unit column stride, one row per sequence")
-    W = block_table.shape[1]
-    t_row = block_table.stride(0) if B > 1 else W
-    if seq_lens.dtype != torch.int32 or seq_lens.numel() != B or not seq_lens.is_contiguous():
-        raise ValueError("seq_lens must be contiguous int32 [B]")
-    if lambda_.dtype != torch.float32:
-        raise TypeError("lambda_ must be float32")
-    if lambda_.numel() == 1:
-        lam_b = lam_h = 0
-    elif tuple(lambda_.shape) == (H,):
-        lam_b, lam_h = 0, lambda_.stride(0)
-    elif tuple(lambda_.shape) == (B, H):
-        lam_b, lam_h = lambda_.stride()
-    else:
-        raise ValueError("lambda_ must hold one value, or be [H] or [B, H]")
-    if norm_weight is not None and (norm_weight.dtype != dtype or norm_weight.numel() != 2 * D or
-                                    not norm_weight.is_contiguous()):
-        raise ValueError("norm_weight must be contiguous [2 D] of query's dtype")
     if scale is None:
-        scale = D ** -0.5
-    if not scale > 0 or not eps >= 0:
-        raise ValueError("scale must be positive and eps not negative")
-    if t_row < W or (B > 1 and q_row < H2 * D):
-        raise ValueError("block_table and query: rows must not overlap")
-    if B == 0:
-        return output
-    # (a workspace of the call's own: calls on other streams and captured graphs never meet in it)
-    ws = torch.empty(_diff_workspace_bytes(dev, H, pairs, D), dtype=torch.uint8, device=dev)
-    rc = _launch(dev, "xllm_mi355_paged_decode_diff", query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                 output.data_ptr(), block_table.data_ptr(), t_row, W, seq_lens.data_ptr(), lambda_.data_ptr(), lam_b, lam_h,
-                 _ptr(norm_weight), float(eps), float(out_scale), B, H, pairs, D, bs, P, q_row if B > 1 else H2 * D,
-                 o_row if B > 1 else H2 * D, int(window_left), float(scale), ws.data_ptr(), ws.numel(), _dtype_code(query))
-    _check_launch(rc, "xllm_mi355_paged_decode_diff", "output overlaps an input")
-    return output
+        scale = query.shape[-1] ** -0.5
+    return _host_side("batch_decode_diff")(query, k_cache, v_cache, output, block_table, seq_lens, lambda_, float(scale),
+                                           norm_weight, float(eps), float(out_scale), int(window_left))

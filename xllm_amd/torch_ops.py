@@ -19,6 +19,9 @@ over the C ABI, registered with the torch dispatcher as torch.ops.xllm_ops.*.
         num_kv_heads, scale, sliding_window, is_causal, return_lse, plan=None, layer_id=-1)
         -> (output [T, Hq * D], lse or None)
       -- AttentionImpl::forward of the reference (xllm/core/layers/dcu/attention.cpp:55-112) end to end
+  torch.ops.xllm_ops.build_step_tables / build_step_tables_out / build_cos_sin_cache / rotary_embedding /
+  mla_norm_rope_and_cache / batch_decode_diff
+      -- the operators of a step around the decode, arguments as in xllm_amd.ops
 """
 import os
 
