@@ -644,7 +644,8 @@ int xllm_mi355_mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const v
  * lambda: fp32 with strides in elements (0 where a sequence or a head shares it).  norm_weight [2 head_dim] of `dtype`.
  * block_table [batch, table_stride], of which table_width entries are valid: longer contexts are cut there.  window_left
  * as in xllm_mi355_paged_decode_gqa.  A sequence with seq_lens[b] <= 0 gets out = 0.  Page ids are clamped into the cache.
- * dtype (queries, caches, output): bf16 or fp16.  head_dim 64 or 128; any block size.
+ * dtype (queries, caches, output): bf16 or fp16.  head_dim 64 or 128; any block size.  The attended tokens that a table
+ * row can hold (table_width * block_size, or the window) times the KV pairs stay below 2^35.
  * The workspace needs no initialisation; two calls that overlap in time need one each.
  */
 size_t xllm_mi355_paged_decode_diff_workspace_bytes(int64_t n_heads, int64_t n_kv_pairs, int64_t head_dim);

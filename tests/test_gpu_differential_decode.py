@@ -120,6 +120,27 @@ def test_many_sequences_in_slices():
     check(p, 2, 1, 64, 16, lam_of(2))
 
 
+def test_tables_of_vast_capacity():
+    """Each sequence's table could hold 2^31 tokens, so that a few sequences are all that one launch's counters take."""
+    lens = [5000, 1, 0, 300, 4097, 16, 17, 4096, 2, 900, 33, 0, 4, 5, 6, 8000, 1, 70, 4095, 40]
+    p = problem(lens, 2, 1, 64, 4096, BF16, seed=9, garbage=float("nan"))
+    wide = torch.full((len(lens), 2 ** 31 // 4096), 2 ** 30, dtype=torch.int32, device=DEV)
+    wide[:, :p["table"].shape[1]] = p["table"]
+    check(dict(p, table=wide), 2, 1, 64, 4096, lam_of(2))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D,H,pairs", [(128, 16, 4), (128, 24, 2), (64, 16, 4)])
+def test_many_rows_in_parts(dtype, D, H, pairs):
+    """Thousands of output rows, most contexts held by one worker and some by several."""
+    gen = torch.Generator().manual_seed(8)
+    lens = torch.randint(1, 100, (300,), generator=gen).tolist()
+    lens[7], lens[150], lens[299] = 3000, 1500, 700
+    p = problem(lens, H, pairs, D, 16, dtype, seed=8, garbage=float("nan"))
+    w = (1 + 0.1 * torch.randn(2 * D, generator=torch.Generator().manual_seed(3))).to(dtype).to(DEV)
+    check(p, H, pairs, D, 16, lam_of(H), weight=w, out_scale=0.2)
+
+
 @pytest.mark.parametrize("window", [0, 1, 15, 16, 100, 511, 5000])
 def test_sliding_window(window):
     lens = [1, 16, 17, 130, 600, 0, 2500]

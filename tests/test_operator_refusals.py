@@ -98,6 +98,10 @@ def test_differential_decode():
         assert call(fn, base, **change) == EINVAL, change
     for change in (dict(D=96), dict(D=256), dict(P=1 << 28)):
         assert call(fn, base, **change) == ESHAPE, change
+    # tables that could hold more stages of one sequence than 32 bits count; a window bounds them
+    vast = dict(H=256, pairs=256, qs=65536, os=65536, bs=1 << 20, P=1, width=2048, stride=2048)
+    assert call(fn, base, **vast) == ESHAPE
+    assert call(fn, base, **vast, window=100, ws=None) == EWORKSPACE
     for dtype in (FP32, FP8):
         assert call(fn, base, dtype=dtype) == EDTYPE
     for change in (dict(q=FAKE + 8), dict(k=FAKE + 2), dict(v=FAKE + 8), dict(out=FAKE + 4), dict(w=FAKE + 4), dict(qs=4100),

@@ -42,13 +42,19 @@ namespace {
 constexpr int kDiffTokens = 16;               // tokens of a stage
 constexpr int kDiffRings = 131072;            // ring bytes of a workgroup
 constexpr int kDiffMaxBatch = 1024;           // sequences per launch (their prefix and lengths lie in LDS)
-// A team takes at least this many stages.  One is faster for a few short contexts (4 of up to 512 tokens: 11.4 us for one
-// stage, 12.5 for two, 14.9 for four) and slower where one context is then in 250 parts (4000 tokens: 24.4, 20.3, 21.7 us).
+// A team takes at least two stages once a quarter of the teams are busy; below that one, since a short list is all latency.
+// (One, two, four at least: 4 contexts of up to 512 tokens 11.4, 12.5, 14.9 us; one of 100 tokens 13.0, 15.9, 21.6 us; one
+// of 4000 tokens, which is then in 250, 125 or 62 parts, 24.4, 20.3, 21.7 us.)
 constexpr int kDiffMinStages = 2;
 // Output rows up to which the parts of a row are joined by a workgroup of 16 wavefronts, and of 4 (one wavefront beyond).
 // 16 rows of 250 parts: 12 us with 16, 30 us with 4; 1024 rows of 5 parts: 6 us with 4 and with one; 8192 rows of 2 parts:
 // 34 us with 4, 14 us with one.
 constexpr int64_t kDiffSplit16 = 256, kDiffSplit4 = 2048;
+// Output rows from which the parts of 256-dim rows are stored past the caches (up to eight heads per pair).  In a row of
+// launches, the merge reading them right behind: 256 sequences x 16 heads of 1k to 8k tokens 695 us and 715 through the
+// caches, 128 x 32 heads 364 and 373, 512 x 16 heads of 0.5k to 2k 407 and 419; but 64 x 16 heads 98.5 and 97, 1 x 8 heads of
+// 32k 41.4 and 39.2, groups of sixteen (64 x 64 heads) 142 and 137, rows of 128 dims (512 x 32 heads) 246 and 243.
+constexpr int64_t kDiffStreamRows = 4096;
 constexpr float kDiffSlack = 8.0f;            // a maximum moves when a score exceeds it by this much (log2 units)
 
 typedef __attribute__((address_space(3))) s16x4 diff_lds_s16x4;
@@ -87,6 +93,7 @@ struct DiffArgs {
   // chip (256 CUs, workgroup i on XCD i % 8) the odd XCDs stream slower with equal shares: 9 : 8 takes 4 % off the launch
   // (256 sequences: 771 -> 742 us; 16 : 15 740, 16 : 17 769).  A tuned share and no more: every device computes the same.
   int pools;
+  int stream_parts;     // 1: partial rows are stored past the caches
   float scale_log2;
   float eps;
   float out_scale;
@@ -124,8 +131,9 @@ __device__ __forceinline__ DiffDeal diff_deal(const DiffArgs& a, int64_t total) 
   DiffDeal d;
   d.total = total;
   const int most = a.n_workers >> a.team_shift;
-  const int64_t n = total / kDiffMinStages;
-  d.used = static_cast<int>(n < 1 ? 1 : (n < most ? n : most));
+  int64_t n = total / kDiffMinStages;
+  if (n < most / 4) n = total < most / 4 ? total : most / 4;
+  d.used = static_cast<int>(n < most ? n : most);
   const bool pools = a.pools != 0 && d.used == most;
   d.half = pools ? most / 2 : 0;
   d.cut = pools ? total * kPoolEven / (kPoolEven + kPoolOdd) : 0;
@@ -200,6 +208,10 @@ struct DiffShape {
   // for 64 heads; of 128-dim maps and 16 heads: 97 and 96 us (0.5k to 4k tokens), where the loop waits for memory and not
   // for its instructions (without its P.V products it takes 2 % less).
   static constexpr int kWaves = D == 64 ? 8 : 4;
+  // Registers as if two wavefronts shared a SIMD, which they do or could, but for the shape whose accumulators alone are
+  // 128: with all 512 the compiler keeps accumulators in accumulation registers and copies them to ordinary ones and back
+  // around every product, a third of the loop's instructions.
+  static constexpr int kPerSimd = D == 128 && NB == 2 ? 1 : 2;
   static constexpr int kThreads = kWaves * kWave;
   static constexpr int kRing = kDiffRings / kWaves;         // ring bytes of a worker
   static constexpr int kRow = 4 * D;                       // bytes of a pair's row
@@ -255,7 +267,7 @@ __device__ __forceinline__ void diff_store_row(const DiffArgs& a, const char* no
 }
 
 template <typename QT, int D, int NB>
-__global__ __launch_bounds__((DiffShape<D, NB>::kThreads), 1) void diff_decode_kernel(DiffArgs a) {
+__global__ __launch_bounds__((DiffShape<D, NB>::kThreads), (DiffShape<D, NB>::kPerSimd)) void diff_decode_kernel(DiffArgs a) {
   using S = DiffShape<D, NB>;
   constexpr int kThreads = S::kThreads;
   constexpr int KS = D / 32;       // k-steps of a map's scores
@@ -471,8 +483,9 @@ __global__ __launch_bounds__((DiffShape<D, NB>::kThreads), 1) void diff_decode_k
     if (s + 1 < N) advance(nc);
     const char* st = ring + (s % NS) * (2 * S::kTile);
 
-    // ---- keys: wait for them (and for the query rows of a new context, asked for one stage ago)
+    // ---- wait for the stage (and for the query rows of a new context, asked for one stage ago)
     if (s + NS > N) diff_wait_vm<0>();
+    else if (NB == 1 && !(fresh && s > 0)) diff_wait_vm<(NS - 1) * kStageOps>();
     else if (fresh && s > 0) diff_wait_vm<kStageOps>();
     else diff_wait_vm<NL + (NS - 1) * kStageOps>();
     if (fresh) {
@@ -504,15 +517,26 @@ __global__ __launch_bounds__((DiffShape<D, NB>::kThreads), 1) void diff_decode_k
     }
     if (last && s + 1 < N) fetch_query(nc);
 
-    // ---- read the keys and fill their place again
+    // ---- read the keys (and the values, where the registers hold both) and fill their place again
     u32x4 kr[2 * KS];
 #pragma unroll
     for (int i = 0; i < 2 * KS; ++i)
       kr[i] = *reinterpret_cast<const u32x4*>(st + k_read + (((i * 4 + g) ^ c16) & (S::kChunks - 1)) * 16);
-    diff_wait_lds();
+    constexpr int VB = MB / NB;
+    s16x4 vt[VB];
+    auto read_values = [&](int h) {
+#pragma unroll
+      for (int i = 0; i < VB; ++i)
+        vt[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (diff_lds_s16x4*)(st + S::kTile + v_read + ((v_chunk ^ (2 * (h * VB + i))) * 16)));
+      diff_wait_lds();
+    };
+    if constexpr (NB == 1) read_values(0);
+    else diff_wait_lds();
     if (more) {
       fetch_pages();
       load_keys();
+      if constexpr (NB == 1) load_values();
     }
 
     // ---- scores: lane (column c16, tokens 4 g .. 4 g + 3)
@@ -564,21 +588,18 @@ __global__ __launch_bounds__((DiffShape<D, NB>::kThreads), 1) void diff_decode_k
       p[nb] = u32x4{h0, h1, QT::pack(e[0] - QT::lo(h0), e[1] - QT::hi(h0)), QT::pack(e[2] - QT::lo(h1), e[3] - QT::hi(h1))};
     }
 
-    // ---- values: the same, by the transposing read (lane c16 of 16 supplies 4 dims of token 4 g + c16 / 4 and receives
-    // the 4 tokens 4 g .. of dim 16 mb + c16)
-    if (more) diff_wait_vm<(NS - 1) * kStageOps + 1 + NL>();
-    else diff_wait_vm<0>();
-    // (two blocks of columns leave registers for half of the values at a time)
-    constexpr int VB = MB / NB;
+    // ---- values by the transposing read (lane c16 of 16 supplies 4 dims of token 4 g + c16 / 4 and receives the 4 tokens
+    // 4 g .. of dim 16 mb + c16); two blocks of columns leave registers for half of them at a time
+    if constexpr (NB == 2) {
+      if (more) diff_wait_vm<(NS - 1) * kStageOps + 1 + NL>();
+      else diff_wait_vm<0>();
+    }
 #pragma unroll
     for (int h = 0; h < NB; ++h) {
-      s16x4 vt[VB];
-#pragma unroll
-      for (int i = 0; i < VB; ++i)
-        vt[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (diff_lds_s16x4*)(st + S::kTile + v_read + ((v_chunk ^ (2 * (h * VB + i))) * 16)));
-      diff_wait_lds();
-      if (h == NB - 1 && more) load_values();
+      if constexpr (NB == 2) {
+        read_values(h);
+        if (h == NB - 1 && more) load_values();
+      }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -613,8 +634,18 @@ __global__ __launch_bounds__((DiffShape<D, NB>::kThreads), 1) void diff_decode_k
         for (int nb = 0; nb < NB; ++nb) {
           const int64_t col = slot * S::kCols + nb * 16 + c16;
           if (head < heads) {
+            float* part = a.ws_o + col * (2 * D) + 4 * g;
+            if (D == 128 && NB == 1 && a.stream_parts != 0) {
+              int zero = 0;   // (an offset the compiler cannot see through: it folds the two branches' stores otherwise)
 #pragma unroll
-            for (int mb = 0; mb < MB; ++mb) *reinterpret_cast<f32x4*>(a.ws_o + col * (2 * D) + mb * 16 + 4 * g) = o[nb][mb];
+              for (int mb = 0; mb < MB; ++mb) {
+                asm volatile("" : "+s"(zero));
+                __builtin_nontemporal_store(o[nb][mb], reinterpret_cast<f32x4*>(part + zero + mb * 16));
+              }
+            } else {
+#pragma unroll
+              for (int mb = 0; mb < MB; ++mb) *reinterpret_cast<f32x4*>(part + mb * 16) = o[nb][mb];
+            }
             if (g == 0) *reinterpret_cast<f32x2*>(a.ws_ml + col * 2) = f32x2{m[nb], l[nb]};
           }
         }
@@ -810,6 +841,13 @@ int paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, v
   if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || (q_token_stride & 7) != 0 || !aligned(out, 8) ||
       (out_token_stride & 3) != 0 || !aligned(norm_weight, 8))
     return XLLM_MI355_EALIGN;
+  const int64_t group = n_heads / n_kv_pairs, hb_per_pair = group <= 8 ? 1 : (group + 15) / 16, head_blocks = n_kv_pairs * hb_per_pair;
+  const int team_shift = head_blocks % 4 == 0 ? 2 : head_blocks % 2 == 0 ? 1 : 0;
+  const int64_t max_len = table_width > (0x7fffffffLL - 16) / block_size ? 0x7fffffffLL - 16 : table_width * block_size;
+  const int64_t attended = window_left >= 0 && window_left < max_len ? window_left + 1 : max_len;
+  // stages of one sequence, at most (attended tokens that do not begin at a stage reach into one more)
+  const int64_t most_stages = (attended / kDiffTokens + 2) * (head_blocks >> team_shift);
+  if (most_stages > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
   const size_t need = diff_workspace_bytes(n_heads, n_kv_pairs, head_dim);
   if (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < need) return XLLM_MI355_EWORKSPACE;
 
@@ -826,21 +864,18 @@ int paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, v
   DiffArgs a = {};
   a.n_heads = static_cast<int>(n_heads);
   a.n_pairs = static_cast<int>(n_kv_pairs);
-  a.group = static_cast<int>(n_heads / n_kv_pairs);
-  const int per_block = a.group <= 8 ? 8 : 16;
-  a.hb_per_pair = (a.group + per_block - 1) / per_block;
+  a.group = static_cast<int>(group);
+  a.hb_per_pair = static_cast<int>(hb_per_pair);
   a.block_size = static_cast<int>(block_size);
   a.bs_shift = -1;
   for (int s = 0; s < 31; ++s)
     if ((1LL << s) == block_size) a.bs_shift = s;
   a.num_blocks = static_cast<int>(num_blocks);
-  const bool long_table = table_width > (0x7fffffffLL - 16) / block_size;
-  a.max_len = long_table ? 0x7fffffff - 16 : static_cast<int>(table_width * block_size);
+  a.max_len = static_cast<int>(max_len);
   a.window_left = window_left < 0 ? -1 : static_cast<int>(window_left < 0x7fffffffLL ? window_left : 0x7fffffffLL);
   a.n_workers = static_cast<int>(diff_workers(head_dim, a.group));
   a.pools = device_cu_count() == 256 ? 1 : 0;
-  const int64_t head_blocks = n_kv_pairs * a.hb_per_pair;
-  a.team_shift = head_blocks % 4 == 0 ? 2 : head_blocks % 2 == 0 ? 1 : 0;
+  a.team_shift = team_shift;
   a.scale_log2 = sm_scale * kLog2e;
   a.eps = eps;
   a.out_scale = out_scale;
@@ -858,14 +893,17 @@ int paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, v
   a.ws_prefix = reinterpret_cast<int*>(ws);
   a.ws_ml = reinterpret_cast<float*>(ws + diff_prefix_bytes());
   a.ws_o = a.ws_ml + cols * 2;
-  // batches beyond the LDS prefix are decoded in slices, one launch pair after the other
-  for (int64_t b0 = 0; b0 < batch; b0 += kDiffMaxBatch) {
-    a.batch = static_cast<int>(batch - b0 < kDiffMaxBatch ? batch - b0 : kDiffMaxBatch);
+  // batches beyond the LDS prefix, or whose tables could hold more stages than 32 bits count, are decoded in slices, one
+  // launch pair after the other
+  const int64_t fit = 0x7fffffffLL / most_stages, slice = fit < kDiffMaxBatch ? fit : kDiffMaxBatch;
+  for (int64_t b0 = 0; b0 < batch; b0 += slice) {
+    a.batch = static_cast<int>(batch - b0 < slice ? batch - b0 : slice);
     a.q = static_cast<const char*>(q) + b0 * a.q_stride_bytes;
     a.out = static_cast<char*>(out) + b0 * a.out_stride_bytes;
     a.block_table = block_table + b0 * table_stride;
     a.seq_lens = seq_lens + b0;
     a.lambda = lambda + b0 * lambda_batch_stride;
+    a.stream_parts = a.batch * n_heads >= kDiffStreamRows ? 1 : 0;
     const int rc = dtype == XLLM_MI355_BF16 ? dispatch_diff<BF16>(a, head_dim, stream) : dispatch_diff<FP16>(a, head_dim, stream);
     if (rc != 0) return rc;
   }
