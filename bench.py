@@ -260,6 +260,51 @@ def neighbours(ops, workloads, torch, dev, steps, lib=None, capi=None):
     tab, cu = lay.block_table.to(dev), cu.to(dev)
     row("gather_mla_latent_cache", "gather_paged_rows_kernel", f"{total} rows of 1152 bytes from pages of {cfg.block_size}",
         timed(lambda: ops.gather_mla_latent_cache(lat, tab, cu, total)), 2 * total * 1152)
+    # the tables of a mixed step: kept entries and lengths read, pages taken, table, positions and slots written
+    B, W, budget = 2048, 1030, 65536
+    kv_lens = torch.randint(0, 16384, (B,), generator=g).to(torch.int32).to(dev)
+    new_lens = torch.randint(0, 64, (B,), generator=g).to(torch.int32).to(dev)
+    btab = torch.randint(0, 1 << 20, (B, W), generator=g).to(torch.int32).to(dev)
+    free = torch.arange(1 << 14, dtype=torch.int32, device=dev)
+    kept, taken = int(((kv_lens + 15) // 16).sum()), int(new_lens.sum()) // 16
+    row("build_step_tables", "step_tables_kernel", f"{B} requests, table of {W}, {budget} new tokens",
+        timed(lambda: ops.build_step_tables(kv_lens, new_lens, btab, free, 16, budget)),
+        B * 20 + (kept + taken + B * W) * 4 + budget * 12)
+    # cos | sin rows of 128k positions (writes only)
+    inv, factor = ops.rope_frequencies(128, base=500000.0, device=dev, scaling=ops.RopeScaling(
+        "llama3", factor=8.0, original_max_position=8192))
+    rows128 = torch.empty(131072, 128, device=dev)
+    row("build_cos_sin_cache", "rope_cos_sin_kernel", "131072 positions x 128, fp32",
+        timed(lambda: ops.build_cos_sin_cache(inv, 131072, attention_factor=factor, out=rows128)), rows128.numel() * 4)
+    # rotation of q and k of a prefill chunk in tensors of their own, in place
+    q, k = qkv[:, :nq * D].view(T, nq, D), qkv[:, nq * D:(nq + nk) * D].view(T, nk, D)
+    row("rotary_embedding", "rotary_kernel", f"{T} tokens, {nq}/{nk} heads x {D}, in place",
+        timed(lambda: ops.rotary_embedding(pos, q, k, cs)), T * (nq + nk) * D * 2 * 2)
+    # MLA prologue of a prefill chunk
+    T, H = 4096, 128
+    qm = torch.randn(T, H, 192, generator=g).to(torch.bfloat16).to(dev)
+    latent = torch.randn(T, 576, generator=g).to(torch.bfloat16).to(dev)
+    lw, cs64 = torch.ones(512, dtype=torch.bfloat16, device=dev), torch.cat([ang[:, :32].cos(), ang[:, :32].sin()], 1).to(dev)
+    q_pe, pos = torch.empty(T, H, 64, dtype=torch.bfloat16, device=dev), pos[:T].contiguous()
+    lslots = torch.randperm(T + 64, generator=g)[:T].to(torch.int32).to(dev)
+    row("mla_norm_rope_and_cache", "mla_prologue_kernel", f"{T} tokens, {H} heads x 64 and latent rows of 576",
+        timed(lambda: ops.mla_norm_rope_and_cache(qm[..., 128:], latent, lw, 1e-6, cs64, True, pos, k_cache=lat[:65],
+                                                  slot_mapping=lslots, out_q_pe=q_pe)), T * (H * 64 + 576) * 2 * 2)
+    # differential decode over the pages of configuration 2, its heads taken in pairs (one wide value head per pair)
+    cfg = workloads.CONFIGS["llama3_8b"]
+    lay = workloads.make_layout(cfg, 1)
+    gd = torch.Generator(device=dev).manual_seed(1)
+    pairs = cfg.n_kv_heads // 2
+    dk = workloads.randn_16bit((lay.num_blocks, cfg.block_size, 2 * pairs, cfg.head_dim), 1.0, gd, dev)
+    dv = workloads.randn_16bit((lay.num_blocks, cfg.block_size, pairs, 2 * cfg.head_dim), 1.0, gd, dev)
+    dq = workloads.randn_16bit((cfg.batch, cfg.n_q_heads, cfg.head_dim), 1.0, gd, dev)
+    dout = torch.empty(cfg.batch, cfg.n_q_heads // 2, 2 * cfg.head_dim, dtype=torch.bfloat16, device=dev)
+    lam, dw = torch.full((cfg.n_q_heads // 2,), 0.5, device=dev), torch.ones(2 * cfg.head_dim, dtype=torch.bfloat16, device=dev)
+    tab, lens = lay.block_table.to(dev), lay.seq_lens.to(dev)
+    row("batch_decode_diff", "diff_decode_kernel + diff_merge_kernel",
+        f"{cfg.batch} sequences, {cfg.n_q_heads // 2} heads over {pairs} pairs of {cfg.head_dim}, contexts {cfg.len_lo} to {cfg.len_hi}",
+        timed(lambda: ops.batch_decode_diff(dq, dk, dv, dout, tab, lens, lam, norm_weight=dw, out_scale=0.5)),
+        workloads.gqa_bytes(cfg, lay.seq_lens, 2))
     return {"neighbour_ops": rows, "steps": steps, "peak_gbs": HBM_PEAK_GBS,
             "note": "torch events around the loop of calls (launch gaps included)"}
 

@@ -23,6 +23,7 @@ over the C ABI, registered with the torch dispatcher as torch.ops.xllm_ops.*.
   mla_norm_rope_and_cache / batch_decode_diff
       -- the operators of a step around the decode, arguments as in xllm_amd.ops
 """
+import ctypes
 import os
 
 import torch
@@ -37,6 +38,8 @@ def load():
     if not _loaded:
         if not os.path.exists(SHIM_PATH):
             raise RuntimeError(f"{SHIM_PATH} is missing: build it with `python -m xllm_amd.build`")
+        if os.environ.get("XLLM_MI355_LIBRARY"):   # another build of the library (see capi.py): the host side binds to it too
+            ctypes.CDLL(os.environ["XLLM_MI355_LIBRARY"], mode=ctypes.RTLD_GLOBAL)
         torch.ops.load_library(SHIM_PATH)
         _loaded = True
     return torch.ops.xllm_ops
