@@ -581,7 +581,7 @@ int xllm_mi355_build_step_tables(const int32_t* kv_lens, const int32_t* new_lens
 /*
  * cos | sin rows for the rotary entry points of this library, out[r, i] = factor * cos(angle), out[r, half + i] = factor *
  * sin(angle), angle = position(r) * inv_freq[i], with the angle and its reduction in 64 bits (a 32-bit angle at position
- * 10^5 is off by 4e-3) and one rounding to out_dtype.  position(r) = positions[r], or first_position + r where positions is
+ * 10^5 is off by 4e-3) and one rounding to out_dtype; angles up to 2^50 in magnitude.  position(r) = positions[r], or first_position + r where positions is
  * null.  Frequencies scaled for long contexts (the reference's rotary_embedding files in
  * xllm/core/layers/common/) are the caller's inv_freq and factor; ops.rope_frequencies makes them.
  * inv_freq: [half] fp64; out: [n_rows, 2 * half] contiguous, of out_dtype (fp32, bf16, fp16).  half up to 4096.
@@ -619,8 +619,8 @@ int xllm_mi355_rotary_embedding(const int64_t* positions, const void* cos_sin, i
  * q_pe, q_pe_out [n_tokens, n_heads, 64] with token and head strides (q_pe a slice of the queries; q_pe_out contiguous is
  * what xllm_mi355_paged_decode_mla reads; it may be q_pe itself), kv, kv_out rows of 576 with a row stride (kv_out null or
  * kv itself or apart), cache [num_blocks, block_size, 1, 576] or null (one of kv_out and cache is needed).  Slots outside
- * the cache are skipped; a position outside [0, n_positions) is not rotated.  Arithmetic in fp32, rounded once to dtype
- * (bf16, fp16).  Pointers and strides multiples of 16 bytes.
+ * the cache are skipped, the others are distinct; a position outside [0, n_positions) is not rotated.  Arithmetic in fp32,
+ * rounded once to dtype (bf16, fp16).  Pointers and strides multiples of 16 bytes.
  */
 int xllm_mi355_mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const void* kv, void* kv_out,
                                        const void* kv_weight, float eps,

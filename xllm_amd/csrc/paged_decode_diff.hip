@@ -32,6 +32,12 @@
 // scales it up).  It is free: a stage's 16 tokens fill half the depth of a 16x16x32 MFMA, and the other half takes the same
 // values against lo.
 // Softmax statistics, sums and the norm are in fp32.
+//
+// Measured (bf16, 128-dim maps, 16-bit caches): 64 sequences of 0.5k to 4k tokens, 4 pairs, 16 heads (568 MB) 89 us and 6 us
+// of merge, 6.4 TB/s in the decode kernel; 256 sequences of 1k to 8k tokens, 32 heads (4.66 GB) 700 us and 11 us, 6.65 TB/s,
+// where a plain read of as many bytes runs at 7.05 TB/s.  4 sequences of up to 512 tokens: 5.9 us and 5.8 us, all latency (the
+// chain lengths -> page entries -> rows, then the merge's prefix -> parts).  Groups of sixteen heads (64 sequences, 64 heads):
+// 5.0 TB/s, bound by the moves between accumulation and ordinary registers around their 128 accumulators.
 #include "common.cuh"
 #include "launch.h"
 
@@ -841,7 +847,8 @@ int paged_decode_diff(const void* q, const void* k_cache, const void* v_cache, v
   if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || (q_token_stride & 7) != 0 || !aligned(out, 8) ||
       (out_token_stride & 3) != 0 || !aligned(norm_weight, 8))
     return XLLM_MI355_EALIGN;
-  const int64_t group = n_heads / n_kv_pairs, hb_per_pair = group <= 8 ? 1 : (group + 15) / 16, head_blocks = n_kv_pairs * hb_per_pair;
+  const int64_t group = n_heads / n_kv_pairs, hb_per_pair = group <= 8 ? 1 : (group + 15) / 16;
+  const int64_t head_blocks = n_kv_pairs * hb_per_pair;
   const int team_shift = head_blocks % 4 == 0 ? 2 : head_blocks % 2 == 0 ? 1 : 0;
   const int64_t max_len = table_width > (0x7fffffffLL - 16) / block_size ? 0x7fffffffLL - 16 : table_width * block_size;
   const int64_t attended = window_left >= 0 && window_left < max_len ? window_left + 1 : max_len;

@@ -9,6 +9,8 @@
 //   (a, b) -> (a c_i - b s_i, b c_i + a s_i)
 // in fp32 between one load and one store.  All three are bound by the bytes they move (a few operations per element) or,
 // at decode sizes, by the launch: the kernels read and write 16 bytes per lane and instruction and keep several in flight.
+// 64 rows of 128 values take 2.2 us, the rotation of 64 tokens of 40 heads and the MLA prologue of 64 tokens of 128 heads
+// 3.0 us each, which is a launch with one or two trips to memory in it (position, then its cos | sin row).
 #include "common.cuh"
 #include "launch.h"
 
@@ -228,7 +230,9 @@ __device__ __forceinline__ void turn_words(Pack<DT, P>& x, Pack<DT, P>& y, const
 // words when interleaved).  Lanes behind the rotated part copy the rest of the head when the result goes elsewhere, two
 // words each, at neighbouring words in neighbouring lanes.  One head per lane: with four (one set of cosines and sines for
 // all of them, four times the bytes in flight per lane) 8192 tokens of 40 heads took the same 27 us, 4097 tokens of 20
-// heads with a copied rest 28 instead of 19 us, for want of wavefronts.
+// heads with a copied rest 28 instead of 19 us, for want of wavefronts.  Bound by the bytes: 8192 tokens of 40 heads of 128
+// bf16 values in place (172 MB with the table's rows) 27.2 us = 6.3 TB/s, 4097 tokens of 20 heads of 256 fp16 values to
+// another place, 64 of them rotated (84 MB), 17.2 us = 4.9 TB/s; a large copy runs at 5.2 TB/s.
 // VEC = false takes one pair (or two elements to copy) per lane, for operands that are not aligned to 16 bytes.
 template <int DT, int CT, bool INTERLEAVE, bool VEC>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a, float sin_sign) {
@@ -359,7 +363,8 @@ struct MlaPrologueArgs {
 
 // The first kv_blocks workgroups take the tokens' latent rows, one wavefront per row: eight latent values per lane (one
 // 16-byte word), their sum of squares over the wavefront, and the rope part in lanes 0-3.  The others rotate the rope
-// part of the query heads, four lanes per head.
+// part of the query heads, four lanes per head.  Bound by the bytes: 4099 tokens of 128 heads (149 MB, nearly all of it
+// the heads' rope parts in rows of 128 bytes) 24.5 us = 6.1 TB/s.
 template <int DT, int CT, bool INTERLEAVE>
 __global__ __launch_bounds__(kRotThreads) void mla_prologue_kernel(MlaPrologueArgs a) {
   constexpr int kUnits = kRopeDim / 16;
