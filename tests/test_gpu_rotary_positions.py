@@ -167,6 +167,35 @@ def test_strides_slices_and_alignment(interleave, shift):
     assert torch.equal(buf[shift + T * (Hq + Hk) * D:], before[shift + T * (Hq + Hk) * D:])
 
 
+@pytest.mark.parametrize("T", [1, 2, 77])
+@pytest.mark.parametrize("layout", ["heads", "grouped", "head major"])
+def test_results_in_slices_of_one_buffer(T, layout):
+    """Results, and operands in place, that interleave in memory without meeting."""
+    Hq, D = 4, 64
+    Hk = 2 if layout == "heads" else 4
+    gen = torch.Generator(device=DEV).manual_seed(T)
+
+    def halves(x):
+        if layout == "heads":      # [T, Hq + Hk, D]
+            return x[:, :Hq], x[:, Hq:]
+        if layout == "grouped":    # [T, H, q | k]
+            return x[..., :D], x[..., D:]
+        return x[:Hq].transpose(0, 1), x[Hq:].transpose(0, 1)   # [Hq + Hk, T, D]
+
+    shape = {"heads": (T, Hq + Hk, D), "grouped": (T, Hq, 2 * D), "head major": (Hq + Hk, T, D)}[layout]
+    x = torch.randn(shape, generator=gen, device=DEV).to(BF16)
+    q, k = halves(x)
+    pos = torch.arange(T, device=DEV) * 3
+    table = ops.build_cos_sin_cache(ops.rope_frequencies(D, device=DEV)[0], 3 * T)
+    want_q, want_k = torch.empty_like(q.contiguous()), torch.empty_like(k.contiguous())
+    ops.rotary_embedding(pos, q, k, table, out_query=want_q, out_key=want_k)
+    oq, ok = halves(torch.full_like(x, 7.0))
+    ops.rotary_embedding(pos, q, k, table, out_query=oq, out_key=ok)
+    assert torch.equal(oq, want_q) and torch.equal(ok, want_k)
+    ops.rotary_embedding(pos, q, k, table)
+    assert torch.equal(q, want_q) and torch.equal(k, want_k)
+
+
 def test_sides_of_their_own_sizes():
     """Queries whose rotated part is the tail of a wide head, keys that are nothing else: the MLA shapes, and out of place
     for one side only."""
@@ -315,6 +344,28 @@ def test_mla_prologue(dtype, T, H, interleave):
     ops.mla_norm_rope_and_cache(q_pe, kv, w, 1e-6, table, interleave, pos, k_cache=only_cache, slot_mapping=slots.to(DEV),
                                 out_q_pe=torch.empty_like(oq))
     assert torch.equal(only_cache.view(-1, 576)[slots[0].item()], out_kv[0])
+
+
+@pytest.mark.parametrize("T", [1, 5])
+def test_mla_prologue_on_slices_of_one_buffer(T):
+    """The latent rows and the queries of one projection's output, both in place."""
+    H, width = 4, 576 + 4 * 192
+    x = torch.randn(T, width, generator=torch.Generator(device=DEV).manual_seed(T), device=DEV).to(BF16)
+    w = torch.ones(512, dtype=BF16, device=DEV)
+    table = ops.build_cos_sin_cache(ops.rope_frequencies(64, device=DEV)[0], 8)
+    pos = torch.arange(T, device=DEV)
+
+    def parts(y):
+        return y[:, 576:].view(T, H, 192)[..., 128:], y[:, :576]
+
+    q, kv = parts(x)
+    oq, okv = torch.empty(T, H, 64, dtype=BF16, device=DEV), torch.empty(T, 576, dtype=BF16, device=DEV)
+    ops.mla_norm_rope_and_cache(q, kv, w, 1e-6, table, False, pos, out_q_pe=oq, out_kv=okv)
+    y = x.clone()
+    q, kv = parts(y)
+    ops.mla_norm_rope_and_cache(q, kv, w, 1e-6, table, False, pos, out_kv=kv)
+    assert torch.equal(q, oq) and torch.equal(kv, okv)
+    assert torch.equal(y[:, 576:].view(T, H, 192)[..., :128], x[:, 576:].view(T, H, 192)[..., :128])
 
 
 def test_mla_prologue_zero_rows_and_positions_outside():

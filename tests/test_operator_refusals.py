@@ -138,6 +138,16 @@ def test_outputs_that_meet_inputs_or_each_other():
     assert call(lib.xllm_mi355_rotary_embedding, rot, qo=at["q"] + 16) == EINVAL
     assert call(lib.xllm_mi355_rotary_embedding, rot, qo=at["q"], sqo=strides(512, 64)) == EINVAL   # heads meet
     assert call(lib.xllm_mi355_rotary_embedding, rot, sqo=strides(256, 128)) == EINVAL              # tokens meet
+    # two operands of one buffer whose rows meet: four heads each of [T, 7, 128], in place; results that meet by one word
+    st = strides(7 * 128, 128)
+    one = dict(rot, qo=at["q"], k=at["q"] + 3 * 256, ko=at["q"] + 3 * 256, sq=st, sqo=st, sk=st, sko=st)
+    assert call(lib.xllm_mi355_rotary_embedding, one) == EINVAL
+    assert call(lib.xllm_mi355_rotary_embedding, dict(one, ko=at["ko"])) == EINVAL   # (k is read where q is written)
+    st = strides(8 * 128 - 8, 128)
+    two = dict(rot, ko=at["qo"] + 4 * 256, sqo=st, sko=st)
+    assert call(lib.xllm_mi355_rotary_embedding, two) == EINVAL
+    for where in ("pos", "table"):
+        assert call(lib.xllm_mi355_rotary_embedding, rot, qo=at[where], q=at[where]) == EINVAL, where
     mla, at = spread(dict(q=0, qo=0, kv=0, kvo=0, w=0, eps=1e-6, table=0, rows=10, pos=0, cache=0, slots=0, T=4, H=8, dl=512,
                           dr=64, qt=1536, qh=192, qot=512, qoh=64, kvs=576, kvos=576, bs=16, P=4, interleave=1, dtype=BF16,
                           ctype=FP32, stream=None),
@@ -148,6 +158,9 @@ def test_outputs_that_meet_inputs_or_each_other():
                 got = call(lib.xllm_mi355_mla_norm_rope_and_cache, mla, **{out: at[other]})
                 assert got == EINVAL, (out, other)
     assert call(lib.xllm_mi355_mla_norm_rope_and_cache, mla, kvo=at["kv"] + 16) == EINVAL
+    # latent rows and rope parts of one buffer of 1936 values a token: the last head meets the next token's latent
+    fused = dict(mla, q=at["kv"] + 1152 + 16, qo=at["kv"] + 1152 + 16, qt=1936, qot=1936, qh=192, qoh=192, kvs=1936, kvos=1936)
+    assert call(lib.xllm_mi355_mla_norm_rope_and_cache, fused, kvo=at["kv"]) == EINVAL
     rows, at = spread(dict(inv=0, pos=0, first=0, rows=4, half=32, factor=1.0, out=0, dtype=FP32, stream=None), ("inv", "pos", "out"))
     for other in ("inv", "pos"):
         assert call(lib.xllm_mi355_rope_cos_sin, rows, out=at[other]) == EINVAL

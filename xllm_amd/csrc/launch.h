@@ -227,6 +227,40 @@ inline Span span_of(const void* p, int64_t n0, int64_t s0, int64_t n1, int64_t s
   return Span(p, ((n0 - 1) * s0 + (n1 - 1) * s1 + inner) * elem_bytes);
 }
 
+// [n0, n1] runs of `len` bytes, strides in bytes: a [tokens, heads, dims] operand, which may be a slice of a wider buffer.
+struct Region {
+  const void* p = nullptr;
+  int64_t n0 = 0, s0 = 0, n1 = 0, s1 = 0, len = 0;
+  Span span() const { return Span(p, (n0 - 1) * s0 + (n1 - 1) * s1 + len); }
+  // Two slices of one buffer interleave without meeting: what lies in one period of the outer stride of both is compared,
+  // and where that overlaps too, one period of the inner stride (both with either dim as the outer one).
+  bool meets(const Region& o) const {
+    if (p == nullptr || o.p == nullptr || !span().meets(o.span())) return false;
+    return !apart(o) && !Region{p, n1, s1, n0, s0, len}.apart(Region{o.p, o.n1, o.s1, o.n0, o.s0, o.len});
+  }
+
+ private:
+  static int64_t floor_mod(int64_t x, int64_t m) { return (x % m + m) % m; }
+  static int64_t period(int64_t n, int64_t s, int64_t on, int64_t os) {   // the stride that both share, 0: none
+    return n == 1 ? os : on == 1 || s == os ? s : 0;
+  }
+  bool apart(const Region& o) const {
+    const int64_t d = static_cast<int64_t>(reinterpret_cast<uintptr_t>(o.p) - reinterpret_cast<uintptr_t>(p));
+    const int64_t mine = (n1 - 1) * s1 + len, its = (o.n1 - 1) * o.s1 + o.len, inner = period(n1, s1, o.n1, o.s1);
+    auto clear = [&](int64_t at) {   // one outer row of each, the other's `at` bytes behind
+      if (at >= mine || at + its <= 0) return true;
+      if (inner <= 0 || (n1 == 1 && o.n1 == 1)) return false;
+      const int64_t m = floor_mod(at, inner);
+      return m >= len && inner - m >= o.len;
+    };
+    if (n0 == 1 && o.n0 == 1) return clear(d);
+    const int64_t outer = period(n0, s0, o.n0, o.s0);
+    if (outer <= 0 || mine > outer || its > outer) return false;
+    const int64_t r = floor_mod(d, outer);
+    return clear(r) && clear(r - outer);
+  }
+};
+
 // Kernel attributes (dynamic LDS size) are set per device.  Returns true the first time it is called with
 // `seen` on the current device (devices 0..63; beyond that always true: setting them again is harmless).
 inline bool first_use_on_current_device(std::atomic<uint64_t>& seen) {

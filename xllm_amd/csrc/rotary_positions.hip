@@ -542,22 +542,24 @@ int rotary_embedding(const int64_t* positions, const void* cos_sin, int64_t n_po
     if (!side(a.k, k, k_out, k_strides, k_out_strides, n_heads_k, head_dim_k, rotary_offset_k)) return XLLM_MI355_EINVAL;
     add(a.k);
   }
-  // A result goes to its own operand, element for element, or apart from everything that is read; its heads do not meet.
-  const Span read[4] = {span_of(q, n_tokens, a.q.in_token, n_heads_q, a.q.in_head, head_dim_q, es),
-                        n_heads_k > 0 ? span_of(k, n_tokens, a.k.in_token, n_heads_k, a.k.in_head, head_dim_k, es) : Span(),
-                        Span(cos_sin, n_positions * rotary_dim * table_size), Span(positions, n_tokens * 8)};
+  // A result goes to its own operand, element for element, or apart from everything that is read, and the two results lie
+  // apart; so do the heads of each.
+  auto region = [&](const RotSide& s, bool out) {
+    if (s.heads == 0) return Region{};
+    return out ? Region{s.out, n_tokens, s.out_token * es, s.heads, s.out_head * es, s.dim * es}
+               : Region{s.in, n_tokens, s.in_token * es, s.heads, s.in_head * es, s.dim * es};
+  };
   for (const RotSide* s : {&a.q, &a.k}) {
     if (s->heads == 0) continue;
+    const RotSide& other = s == &a.q ? a.k : a.q;
     if (!rows_apart(n_tokens, s->out_token, s->heads, s->out_head, s->dim)) return XLLM_MI355_EINVAL;
-    if (s->in == s->out) {
-      if (s->in_token != s->out_token || s->in_head != s->out_head) return XLLM_MI355_EINVAL;
-      continue;
-    }
-    const Span w = span_of(s->out, n_tokens, s->out_token, s->heads, s->out_head, s->dim, es);
-    for (const Span& r : read)
-      if (w.meets(r)) return XLLM_MI355_EINVAL;
+    const Region w = region(*s, true);
+    if (s->in == s->out ? s->in_token != s->out_token || s->in_head != s->out_head : w.meets(region(*s, false)))
+      return XLLM_MI355_EINVAL;
+    if (w.meets(region(other, false)) || w.meets(region(other, true)) || w.span().meets(Span(positions, n_tokens * 8)) ||
+        w.span().meets(Span(cos_sin, n_positions * rotary_dim * table_size)))
+      return XLLM_MI355_EINVAL;
   }
-  if (n_heads_k > 0 && a.q.out == a.k.out) return XLLM_MI355_EINVAL;
   a.positions = positions;
   a.cos_sin = static_cast<const char*>(cos_sin);
   a.n_positions = n_positions;
@@ -600,22 +602,22 @@ int mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const void* kv, vo
     return XLLM_MI355_EALIGN;
   {
     const int64_t table_size = cos_sin_dtype == XLLM_MI355_FP32 ? 4 : 2, row = kLatent + kRopeDim;
-    const Span sq = span_of(q_pe, n_tokens, q_token_stride, n_heads, q_head_stride, kRopeDim, 2);
-    const Span skv = span_of(kv, n_tokens, kv_row_stride, 1, 0, row, 2);
+    const Region sq{q_pe, n_tokens, q_token_stride * 2, n_heads, q_head_stride * 2, kRopeDim * 2};
+    const Region skv{kv, n_tokens, kv_row_stride * 2, 1, 0, row * 2};
     const Span rest[4] = {Span(kv_weight, kLatent * 2), Span(cos_sin, n_positions * kRopeDim * table_size),
                           Span(positions, n_tokens * 8), Span(slots, k_cache != nullptr ? n_tokens * 4 : 0)};
-    const Span wq = span_of(q_pe_out, n_tokens, q_out_token_stride, n_heads, q_out_head_stride, kRopeDim, 2);
-    const Span wkv = kv_out != nullptr ? span_of(kv_out, n_tokens, kv_out_row_stride, 1, 0, row, 2) : Span();
-    const Span wc = Span(k_cache, k_cache != nullptr ? num_blocks * block_size * row * 2 : 0);
+    const Region wq{q_pe_out, n_tokens, q_out_token_stride * 2, n_heads, q_out_head_stride * 2, kRopeDim * 2};
+    const Region wkv = kv_out != nullptr ? Region{kv_out, n_tokens, kv_out_row_stride * 2, 1, 0, row * 2} : Region{};
+    const Region wc = k_cache != nullptr ? Region{k_cache, 1, 0, 1, 0, num_blocks * block_size * row * 2} : Region{};
     if (!rows_apart(n_tokens, q_out_token_stride, n_heads, q_out_head_stride, kRopeDim)) return XLLM_MI355_EINVAL;
-    if (q_pe_out == q_pe ? q_out_token_stride != q_token_stride || q_out_head_stride != q_head_stride
-                         : wq.meets(sq) || wq.meets(skv))
+    if (q_pe_out == q_pe ? q_out_token_stride != q_token_stride || q_out_head_stride != q_head_stride : wq.meets(sq))
       return XLLM_MI355_EINVAL;
-    if (kv_out == kv ? kv_out_row_stride != kv_row_stride : wkv.meets(skv) || wkv.meets(sq)) return XLLM_MI355_EINVAL;
-    if (q_pe_out != q_pe && kv_out != kv && wq.meets(wkv)) return XLLM_MI355_EINVAL;
+    if (kv_out == kv ? kv_out_row_stride != kv_row_stride : wkv.meets(skv)) return XLLM_MI355_EINVAL;
+    if (wq.meets(skv) || wkv.meets(sq) || wq.meets(wkv)) return XLLM_MI355_EINVAL;
     if (wc.meets(sq) || wc.meets(skv) || wc.meets(wq) || wc.meets(wkv)) return XLLM_MI355_EINVAL;
     for (const Span& r : rest)
-      if (wq.meets(r) || wkv.meets(r) || wc.meets(r)) return XLLM_MI355_EINVAL;
+      if (wq.span().meets(r) || (kv_out != nullptr && wkv.span().meets(r)) || (k_cache != nullptr && wc.span().meets(r)))
+        return XLLM_MI355_EINVAL;
   }
   MlaPrologueArgs a = {};
   a.q = static_cast<const uint16_t*>(q_pe);
