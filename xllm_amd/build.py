@@ -134,6 +134,33 @@ def build_shim(force=True, verbose=True):
     return SHIM_LIB
 
 
+PYTHON_LIB = os.path.join(HERE, "_step_ops.so")
+
+
+def build_python(force=True, verbose=True):
+    """The Python module over the C++ host side of the step's operators (xllm_amd._step_ops)."""
+    src = os.path.join(CSRC, "shim", "step_ops_python.cpp")
+    if not force and not _stale(PYTHON_LIB, [src, os.path.join(CSRC, "shim", "ops_api.h")]):
+        return PYTHON_LIB
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    incs = []
+    for p in (*cpp_extension.include_paths(device_type="cuda"), "/opt/rocm/include", sysconfig.get_paths()["include"]):
+        incs += ["-isystem", p]
+    libdir = os.path.join(os.path.dirname(torch.__file__), "lib")
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", *incs, "-o", PYTHON_LIB, src,
+           f"-L{HERE}", "-lxllm_mi355_torch", "-Wl,-rpath,$ORIGIN", f"-L{libdir}", f"-Wl,-rpath,{libdir}",
+           "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10"]
+    if verbose:
+        print("+", " ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    return PYTHON_LIB
+
+
 if __name__ == "__main__":
     build(force="--if-stale" not in sys.argv)
     build_shim(force="--if-stale" not in sys.argv)
+    build_python(force="--if-stale" not in sys.argv)

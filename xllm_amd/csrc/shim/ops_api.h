@@ -182,6 +182,9 @@ void build_step_tables(const torch::Tensor& kv_lens, const torch::Tensor& new_le
                        const torch::Tensor& free_pages, int64_t block_size, int64_t max_new_tokens,
                        const std::optional<torch::Tensor>& free_head, StepTables& out);
 
+// The small int32 results of `out` as parts of one allocation (two microseconds less than five of them).
+StepTables step_tables_memory(const torch::Tensor& kv_lens, int64_t max_new_tokens);
+
 // cos | sin rows [rows, 2 * inv_freq.numel()] of position_ids, or of num_positions positions from first_position on.
 torch::Tensor build_cos_sin_cache(const torch::Tensor& inv_freq, const std::optional<torch::Tensor>& position_ids,
                                   int64_t num_positions, int64_t first_position, double attention_factor,

@@ -1,7 +1,7 @@
 // The operators around the decode path on the host side: torch::Tensor arguments checked, unpacked and handed to the C ABI
-// on the current HIP stream of the tensors' device.  Registered with the dispatcher as torch.ops.xllm_ops.*, which is also
-// what the Python functions of the same names call: the checks cost a microsecond here and five there (rotary_embedding of
-// 64 tokens: 7.3 us per call instead of 11.7 us over ctypes).  A violated precondition is a ValueError or a TypeError.
+// on the current HIP stream of the tensors' device.  Registered with the dispatcher as torch.ops.xllm_ops.*; the Python
+// functions of the same names call the same code through step_ops_python.cpp.  The checks cost a microsecond here and five
+// in Python.  A violated precondition is a ValueError or a TypeError.
 #include <ATen/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -127,6 +127,20 @@ void build_step_tables(const Tensor& kv_lens, const Tensor& new_lens, const Tens
                B, block_size, T, stream_of(kv_lens)),
            "xllm_mi355_build_step_tables",
            "an output of build_step_tables overlaps an input or another output (in place means block_table itself)");
+}
+
+StepTables step_tables_memory(const Tensor& kv_lens, int64_t max_new_tokens) {
+  StepTables t;
+  const int64_t B = kv_lens.numel();
+  if (max_new_tokens < 0) return t;   // (refused by the call)
+  const std::vector<Tensor> part = torch::empty({3 * B + 5 + max_new_tokens}, kv_lens.options().dtype(torch::kInt32))
+                                       .unsafe_split_with_sizes({B, B + 1, B + 1, 3, max_new_tokens});
+  t.seq_lens = part[0];
+  t.q_cu_seq_lens = part[1];
+  t.new_page_indptr = part[2];
+  t.counters = part[3];
+  t.slot_mapping = part[4];
+  return t;
 }
 
 Tensor build_cos_sin_cache(const Tensor& inv_freq, const OptTensor& position_ids, int64_t num_positions,
@@ -297,18 +311,7 @@ using Tables = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor
 
 Tables op_build_step_tables(Tensor kv_lens, Tensor new_lens, Tensor block_table, Tensor free_pages, int64_t block_size,
                             int64_t max_new_tokens, OptTensor free_head) {
-  k::StepTables t;
-  // (the five small results in one allocation: two microseconds less than five)
-  const int64_t B = kv_lens.numel();
-  if (max_new_tokens >= 0) {
-    std::vector<Tensor> part = torch::empty({3 * B + 5 + max_new_tokens}, kv_lens.options().dtype(torch::kInt32))
-                                   .unsafe_split_with_sizes({B, B + 1, B + 1, 3, max_new_tokens});
-    t.seq_lens = part[0];
-    t.q_cu_seq_lens = part[1];
-    t.new_page_indptr = part[2];
-    t.counters = part[3];
-    t.slot_mapping = part[4];
-  }
+  k::StepTables t = k::step_tables_memory(kv_lens, max_new_tokens);
   k::build_step_tables(kv_lens, new_lens, block_table, free_pages, block_size, max_new_tokens, free_head, t);
   return {t.block_table, t.seq_lens, t.q_cu_seq_lens, t.position_ids, t.slot_mapping, t.new_page_indptr, t.counters};
 }

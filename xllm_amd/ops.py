@@ -817,10 +817,10 @@ def absorbed_bmm(x, w, out=None):
 # the tables of a step
 
 @functools.lru_cache(maxsize=None)
-def _host_side(name):
-    """The dispatcher's entry of the C++ host side: it checks the arguments (ValueError, TypeError) and launches."""
+def _host_side():
+    """The C++ host side of the functions below: it checks the arguments (ValueError, TypeError) and launches."""
     from . import torch_ops
-    return getattr(torch_ops.load(), name).default
+    return torch_ops.load_step_ops()
 
 
 @dataclass
@@ -849,13 +849,13 @@ def build_step_tables(kv_lens, new_lens, block_table, free_pages, block_size, ma
     attend before its tokens are stored.
     out: StepTables to write into (the persistent buffers of a captured step); its block_table may be block_table itself.
     Returns StepTables."""
-    if out is None:
-        return StepTables(*_host_side("build_step_tables")(kv_lens, new_lens, block_table, free_pages, int(block_size),
-                                                           int(max_new_tokens), free_head))
-    _host_side("build_step_tables_out")(kv_lens, new_lens, block_table, free_pages, int(block_size), int(max_new_tokens),
-                                        free_head, out.block_table, out.seq_lens, out.q_cu_seq_lens, out.position_ids,
-                                        out.slot_mapping, out.new_page_indptr, out.counters)
-    return out
+    given = None
+    if out is not None:
+        given = (out.block_table, out.seq_lens, out.q_cu_seq_lens, out.position_ids, out.slot_mapping, out.new_page_indptr,
+                 out.counters)
+    made = _host_side().build_step_tables(kv_lens, new_lens, block_table, free_pages, block_size, max_new_tokens, free_head,
+                                          given)
+    return StepTables(*made) if out is None else out
 
 
 # ------------------------------------------------------------------------------------------
@@ -939,8 +939,7 @@ def build_cos_sin_cache(inv_freq, num_positions=0, position_ids=None, first_posi
     bits, rounded once to dtype (float32, bfloat16 or float16).  Rows of position_ids [rows] int64 -- one step's rows,
     shared by all layers, which then index them by 0 .. rows - 1 -- or of first_position .. first_position + num_positions - 1.
     inv_freq, attention_factor: from rope_frequencies.  Returns the rows (out, if given)."""
-    return _host_side("build_cos_sin_cache")(inv_freq, position_ids, int(num_positions), int(first_position),
-                                             float(attention_factor), dtype, out)
+    return _host_side().build_cos_sin_cache(inv_freq, position_ids, num_positions, first_position, attention_factor, dtype, out)
 
 
 def rotary_embedding(position_ids, query, key, cos_sin_cache, interleave=False, rotary_offset=0, key_rotary_offset=None,
@@ -952,8 +951,8 @@ def rotary_embedding(position_ids, query, key, cos_sin_cache, interleave=False, 
     interleave: pairs (2i, 2i + 1), else (i, i + rotary_dim / 2).  inverse: the transposed map, which undoes a rotation by
     unscaled rows and turns the gradient of the result into the gradient of the input.
     Works in place, or into out_query / out_key.  Returns (query's result, key's result or None)."""
-    _host_side("rotary_embedding")(position_ids, query, key, cos_sin_cache, bool(interleave), rotary_offset,
-                                   key_rotary_offset, bool(inverse), out_query, out_key)
+    _host_side().rotary_embedding(position_ids, query, key, cos_sin_cache, bool(interleave), rotary_offset,
+                                  key_rotary_offset, bool(inverse), out_query, out_key)
     return query if out_query is None else out_query, key if out_key is None else out_key
 
 
@@ -965,8 +964,8 @@ def mla_norm_rope_and_cache(q_pe, kv, kv_norm_weight, eps, cos_sin_cache, interl
     (negative slots and slots beyond the cache are skipped) and / or to out_kv [T, 576] (kv itself: in place).
     out_q_pe [T, H, 64]: contiguous is what dense_decode reads; None: in place.  bfloat16 or float16.
     Returns (q_pe's result, out_kv)."""
-    _host_side("mla_norm_rope_and_cache")(q_pe, kv, kv_norm_weight, float(eps), cos_sin_cache, bool(interleave), position_ids,
-                                          k_cache, slot_mapping, out_q_pe, out_kv)
+    _host_side().mla_norm_rope_and_cache(q_pe, kv, kv_norm_weight, eps, cos_sin_cache, bool(interleave), position_ids,
+                                         k_cache, slot_mapping, out_q_pe, out_kv)
     return q_pe if out_q_pe is None else out_q_pe, out_kv
 
 
@@ -986,5 +985,6 @@ def batch_decode_diff(query, k_cache, v_cache, output, block_table, seq_lens, la
     window_left >= 0: the last window_left + 1 tokens only.  bfloat16 or float16; D 64 or 128.  Returns output."""
     if scale is None:
         scale = query.shape[-1] ** -0.5
-    return _host_side("batch_decode_diff")(query, k_cache, v_cache, output, block_table, seq_lens, lambda_, float(scale),
-                                           norm_weight, float(eps), float(out_scale), int(window_left))
+    _host_side().batch_decode_diff(query, k_cache, v_cache, output, block_table, seq_lens, lambda_, scale, norm_weight, eps,
+                                   out_scale, window_left)
+    return output

@@ -30,6 +30,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 SHIM_PATH = os.path.join(_HERE, "libxllm_mi355_torch.so")
+PYTHON_PATH = os.path.join(_HERE, "_step_ops.so")
 _loaded = False
 
 
@@ -43,3 +44,12 @@ def load():
         torch.ops.load_library(SHIM_PATH)
         _loaded = True
     return torch.ops.xllm_ops
+
+
+def load_step_ops():
+    """xllm_amd._step_ops: the operators of a step around the decode as plain Python calls, past the dispatcher."""
+    load()
+    if not os.path.exists(PYTHON_PATH):
+        raise RuntimeError(f"{PYTHON_PATH} is missing: build it with `python -m xllm_amd.build`")
+    from . import _step_ops
+    return _step_ops
