@@ -78,6 +78,18 @@ def test_against_the_loop(B, bs, kv_hi, new_hi, budget):
     assert_tables_equal(got, loop_reference(kv, new, table, free.tolist(), bs, budget, 0))
 
 
+@pytest.mark.parametrize("B", [255, 256, 258, 511, 512, 513, 1023, 1024, 1026, 2047, 2048, 2050, 4095, 4096])
+@pytest.mark.parametrize("short", [False, True])
+def test_batches_around_the_ends_of_a_workgroup(B, short):
+    """Where a thread takes one request more, and token counts around whole workgroups; short: budget and pages run out."""
+    kv, new, table, free = make(B, 16, 60, 3, seed=B, extra=1)
+    budget = sum(new) - 257 if short else sum(new) + 255
+    if short:
+        free = free[:B // 4].contiguous()
+    got = call(kv, new, table, free, 16, budget)
+    assert_tables_equal(got, loop_reference(kv, new, table, free.tolist(), 16, budget, 0))
+
+
 @pytest.mark.parametrize("case", ["budget", "no budget", "free list", "empty free list", "width", "head", "head beyond",
                                   "negative lengths", "hole", "wide"])
 def test_what_runs_out(case):

@@ -22,14 +22,13 @@ namespace xllm_mi355 {
 
 namespace {
 
-// Requests of the one-launch forms: a thread holds a run of them in registers.  Workgroups of 256 threads up to 256
-// requests, whose barriers are cheaper (64 decode rows: 3.3 us, with 1024 threads 5.8 us; 256 rows: 3.8 and 6.0 us); of
-// 1024 threads beyond; two launches where the sums no longer fit LDS (1024 rows: 6.2 us in one launch, 15 us in two; 4096
-// rows: 9.2 and 21 us).
-constexpr int kSmallThreads = 256, kSmallRun = 1;
-constexpr int kLargeThreads = 1024, kLargeRun = 4;
-constexpr int kFusedBatch = kLargeThreads * kLargeRun;   // 3 arrays of up to 16 KB in LDS
-constexpr int kStepCells = 1024;         // tokens of a piece
+// Requests of the one-launch forms: a thread holds a run of one, two or four in registers, and the workgroups are as small
+// as that allows, since the barriers of the sums are cheaper (64 decode rows: 3.4 us with 256 threads, 5.8 with 1024; 300
+// rows: 3.9 with 256 threads and runs of two, 6.0 with 1024; 1024 rows: 4.3 with 512 and runs of two, 4.9 with 256 and runs
+// of four, 6.2 with 1024 and runs of four; 2048 rows: 5.9 with runs of two and 6.7 with runs of four).  Two launches where
+// the sums no longer fit LDS (1024 rows: 15 us in two; 4096 rows: 9.2 us in one, 21 in two).
+constexpr int kFusedBatch = 4096;        // 3 arrays of up to 16 KB in LDS
+constexpr int kSumsThreads = 256;        // of the second of two launches
 constexpr int kStepCols = 8;             // table entries of a lane, their loads in flight together
 
 struct StepArgs {
@@ -47,7 +46,6 @@ struct StepArgs {
   int32_t* counters;
   int64_t in_stride, out_stride;
   int batch, width, block_size, bs_shift, budget, n_free;
-  int token_pieces;           // pieces of the tokens, the first ones; then those of the table
   int segments;               // of a table row; a wavefront takes one
   int segment_cols;           // at most kWave * kStepCols
 };
@@ -225,10 +223,16 @@ __global__ __launch_bounds__(1024) void step_sums_kernel(StepArgs a) {
   step_outputs<1024>(a, a.cu, a.indptr, false, tmp);
 }
 
+// Pieces of the tokens, a token per thread (with four per thread 22077 tokens of 134 requests took 5.9 us, now 3.6), then
+// those of the table.
+template <int THREADS>
+__host__ __device__ __forceinline__ int token_pieces(const StepArgs& a) {
+  return static_cast<int>((static_cast<int64_t>(a.budget) + THREADS - 1) / THREADS);
+}
 template <int THREADS>
 __host__ __device__ __forceinline__ int64_t step_pieces(const StepArgs& a) {
   const int64_t units = static_cast<int64_t>(a.batch) * a.segments;
-  return a.token_pieces + (units + THREADS / kWave - 1) / (THREADS / kWave);
+  return token_pieces<THREADS>(a) + (units + THREADS / kWave - 1) / (THREADS / kWave);
 }
 
 // One piece of the tokens, or of the table.  OLD: the pages that the requests keep are in `old`.
@@ -237,29 +241,26 @@ __device__ __forceinline__ void step_piece(const StepArgs& a, int64_t piece, con
                                            const int32_t* old, int head) {
   const int tid = threadIdx.x;
   auto kept = [&](int b) { return OLD ? old[b] : step_pages(a, step_kv(a, b)); };
-  if (piece < a.token_pieces) {
-    const int n_tokens = cu[a.batch];
-#pragma unroll
-    for (int k = 0; k < kStepCells / THREADS; ++k) {
-      const int i = static_cast<int>(piece) * kStepCells + k * THREADS + tid;
-      if (i >= a.budget) continue;
-      int64_t pos = 0;
-      int slot = -1;
-      if (i < n_tokens) {
-        const int b = request_of(cu, a.batch, i);
-        const u32 kv = step_kv(a, b);
-        pos = kv + static_cast<u32>(i - cu[b]);
-        const u32 col = step_column(a, static_cast<u32>(pos));
-        if (col < static_cast<u32>(a.width)) {
-          const int32_t* src = step_source(a, cu, indptr, b, static_cast<int>(col), kept(b), head);
-          const int64_t page = src != nullptr ? *src : -1;
-          const int64_t s = page * a.block_size + (pos - static_cast<int64_t>(col) * a.block_size);
-          if (page >= 0 && s <= 0x7fffffffLL) slot = static_cast<int>(s);
-        }
+  const int of_tokens = token_pieces<THREADS>(a);
+  if (piece < of_tokens) {
+    const int64_t i = piece * THREADS + tid;
+    if (i >= a.budget) return;
+    int64_t pos = 0;
+    int slot = -1;
+    if (i < cu[a.batch]) {
+      const int token = static_cast<int>(i), b = request_of(cu, a.batch, token);
+      const u32 kv = step_kv(a, b);
+      pos = kv + static_cast<u32>(token - cu[b]);
+      const u32 col = step_column(a, static_cast<u32>(pos));
+      if (col < static_cast<u32>(a.width)) {
+        const int32_t* src = step_source(a, cu, indptr, b, static_cast<int>(col), kept(b), head);
+        const int64_t page = src != nullptr ? *src : -1;
+        const int64_t s = page * a.block_size + (pos - static_cast<int64_t>(col) * a.block_size);
+        if (page >= 0 && s <= 0x7fffffffLL) slot = static_cast<int>(s);
       }
-      a.positions[i] = pos;
-      a.slots[i] = slot;
     }
+    a.positions[i] = pos;
+    a.slots[i] = slot;
     return;
   }
   // A wavefront per segment of a row: the request and its pages are the same in all lanes, which leaves a comparison and
@@ -267,7 +268,7 @@ __device__ __forceinline__ void step_piece(const StepArgs& a, int64_t piece, con
   // for 2 M entries).  The lanes' loads are issued before the first is used: an entry without a source reads the row's
   // first one, so that no load hangs off a branch.
   const bool in_place = a.table_in == a.table_out;
-  const int64_t unit = (piece - a.token_pieces) * (THREADS / kWave) + __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int64_t unit = (piece - of_tokens) * (THREADS / kWave) + __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lane = tid & (kWave - 1);
   const int64_t row_of = unit <= 0x7fffffffLL ? static_cast<u32>(unit) / static_cast<u32>(a.segments) : unit / a.segments;
   if (row_of >= a.batch) return;
@@ -312,11 +313,18 @@ __global__ __launch_bounds__(THREADS) void step_tables_kernel(StepArgs a) {
   for (int64_t p = blockIdx.x - 1; p < n; p += gridDim.x - 1) step_piece<THREADS, true>(a, p, cu, indptr, old, head);
 }
 
-__global__ __launch_bounds__(kSmallThreads) void step_tables_from_sums_kernel(StepArgs a) {
+template <int THREADS, int RUN>
+void launch_step_tables(const StepArgs& a, int64_t most, hipStream_t stream) {
+  const int64_t n = step_pieces<THREADS>(a) + 1;
+  step_tables_kernel<THREADS, RUN><<<dim3(static_cast<unsigned>(n < most ? n : most)), THREADS,
+                                     static_cast<size_t>(3 * a.batch + 2) * 4, stream>>>(a);
+}
+
+__global__ __launch_bounds__(kSumsThreads) void step_tables_from_sums_kernel(StepArgs a) {
   const int head = step_head(a);
-  const int64_t n = step_pieces<kSmallThreads>(a);
+  const int64_t n = step_pieces<kSumsThreads>(a);
   for (int64_t p = blockIdx.x; p < n; p += gridDim.x)
-    step_piece<kSmallThreads, false>(a, p, a.cu, a.indptr, nullptr, head);
+    step_piece<kSumsThreads, false>(a, p, a.cu, a.indptr, nullptr, head);
 }
 
 }  // namespace
@@ -377,27 +385,25 @@ int build_step_tables(const int32_t* kv_lens, const int32_t* new_lens, const int
     if ((1LL << s) == block_size) a.bs_shift = s;
   a.budget = static_cast<int>(max_new_tokens);
   a.n_free = static_cast<int>(n_free);
-  a.token_pieces = static_cast<int>((max_new_tokens + kStepCells - 1) / kStepCells);
   a.segments = static_cast<int>((table_width + kWave * kStepCols - 1) / (kWave * kStepCols));
   a.segment_cols = static_cast<int>((table_width + a.segments - 1) / a.segments);
-  // Every workgroup of the one-launch forms makes the sums for itself, so there are no more of them than run at once: one
-  // per CU of 1024 threads (2048 requests, 2 M table entries, 65536 tokens: 9.8 us, of which the sums are 5; with two per
-  // CU 13 us; with one per piece of work 91 us).
-  const int cus = device_cu_count();
-  const size_t lds = static_cast<size_t>(3 * batch + 2) * 4;
-  auto grid = [](int64_t groups, int64_t most) { return dim3(static_cast<unsigned>(groups < most ? groups : most)); };
-  if (batch <= kSmallThreads * kSmallRun) {
-    step_tables_kernel<kSmallThreads, kSmallRun><<<grid(step_pieces<kSmallThreads>(a) + 1, 8LL * cus), kSmallThreads, lds, stream>>>(a);
-    return static_cast<int>(hipGetLastError());
-  }
+  // Every workgroup of the one-launch forms makes the sums for itself, so there are no more of them than run at once: 2048
+  // threads per CU, and one workgroup per CU of 1024 (2048 requests, 2 M table entries, 65536 tokens: 8.7 us; with two per
+  // CU 11 us; with one per piece of work 91 us).
+  const int64_t cus = device_cu_count();
   if (batch <= kFusedBatch) {
-    step_tables_kernel<kLargeThreads, kLargeRun><<<grid(step_pieces<kLargeThreads>(a) + 1, 1LL * cus), kLargeThreads, lds, stream>>>(a);
+    if (batch <= 256) launch_step_tables<256, 1>(a, 8 * cus, stream);
+    else if (batch <= 512) launch_step_tables<256, 2>(a, 8 * cus, stream);
+    else if (batch <= 1024) launch_step_tables<512, 2>(a, 4 * cus, stream);
+    else if (batch <= 2048) launch_step_tables<1024, 2>(a, cus, stream);
+    else launch_step_tables<1024, 4>(a, cus, stream);
     return static_cast<int>(hipGetLastError());
   }
   step_sums_kernel<<<1, 1024, 0, stream>>>(a);
   const int rc = static_cast<int>(hipGetLastError());
   if (rc != 0) return rc;
-  step_tables_from_sums_kernel<<<grid(step_pieces<kSmallThreads>(a), 16LL * cus), kSmallThreads, 0, stream>>>(a);
+  const int64_t pieces = step_pieces<kSumsThreads>(a), most = 16 * cus;
+  step_tables_from_sums_kernel<<<dim3(static_cast<unsigned>(pieces < most ? pieces : most)), kSumsThreads, 0, stream>>>(a);
   return static_cast<int>(hipGetLastError());
 }
 
