@@ -48,7 +48,8 @@ namespace {
 constexpr int kDiffTokens = 16;               // tokens of a stage
 constexpr int kDiffRings = 131072;            // ring bytes of a workgroup
 constexpr int kDiffMaxBatch = 1024;           // sequences per launch (their prefix and lengths lie in LDS)
-// A team takes at least two stages once a quarter of the teams are busy; below that one, since a short list is all latency.
+// A team takes at least two stages once a quarter of the teams are busy and no team has to take two contexts for it; below
+// that one, since a short list is all latency (117 sequences of 10 tokens, 8 pairs: 9.1 us, with two contexts a team 12.3).
 // (One, two, four at least: 4 contexts of up to 512 tokens 11.4, 12.5, 14.9 us; one of 100 tokens 13.0, 15.9, 21.6 us; one
 // of 4000 tokens, which is then in 250, 125 or 62 parts, 24.4, 20.3, 21.7 us.)
 constexpr int kDiffMinStages = 2;
@@ -137,8 +138,9 @@ __device__ __forceinline__ DiffDeal diff_deal(const DiffArgs& a, int64_t total) 
   DiffDeal d;
   d.total = total;
   const int most = a.n_workers >> a.team_shift;
-  int64_t n = total / kDiffMinStages;
-  if (n < most / 4) n = total < most / 4 ? total : most / 4;
+  int64_t n = total / kDiffMinStages, floor = static_cast<int64_t>(a.batch) * ((a.n_pairs * a.hb_per_pair) >> a.team_shift);
+  if (floor < most / 4) floor = most / 4;
+  if (n < floor) n = total < floor ? total : floor;
   d.used = static_cast<int>(n < most ? n : most);
   const bool pools = a.pools != 0 && d.used == most;
   d.half = pools ? most / 2 : 0;
