@@ -70,6 +70,18 @@ def test_rows_of_positions_and_of_a_range(dtype, dim):
         check_rows(got, inv, torch.arange(first, first + n), factor)
 
 
+@pytest.mark.parametrize("dtype,dim,n", [(FP32, 96, 21901), (FP32, 256, 9001), (FP32, 64, 33000), (BF16, 96, 50001),
+                                         (FP16, 128, 33001), (BF16, 32, 131101), (FP32, 2048, 1101), (FP32, 4096, 600)])
+def test_long_ranges(dtype, dim, n):
+    """Ranges whose rows are made from one another: the same bound; the row count leaves lines of the last pass over."""
+    inv, factor = ops.rope_frequencies(dim, scaling=ops.RopeScaling("yarn", factor=4.0, original_max_position=2048), device=DEV)
+    for first in (0, 4_000_000):
+        buf = torch.full((n + 2, dim), 7.0, dtype=dtype, device=DEV)
+        got = ops.build_cos_sin_cache(inv, n, first_position=first, attention_factor=factor, dtype=dtype, out=buf[1:n + 1])
+        check_rows(got, inv, torch.arange(first, first + n), factor)
+        assert (buf[0] == 7).all() and (buf[n + 1] == 7).all()
+
+
 def test_rows_into_a_given_tensor_and_far_positions():
     inv, _ = ops.rope_frequencies(64, device=DEV)
     buf = torch.full((12, 64), 7.0, device=DEV)
