@@ -141,6 +141,17 @@ def test_many_rows_in_parts(dtype, D, H, pairs):
     check(p, H, pairs, D, 16, lam_of(H), weight=w, out_scale=0.2)
 
 
+@pytest.mark.parametrize("n", [127, 128, 129, 254, 255, 256, 257, 264, 272])
+def test_about_as_many_stages_as_workers(n):
+    """One stage of 16 tokens a sequence, some of two or three, so that ranges of one stage and of none occur."""
+    gen = torch.Generator().manual_seed(n)
+    lens = torch.randint(1, 17, (n - 6,), generator=gen).tolist()
+    for at, extra in ((0, 20), (n // 2, 33), (n - 8, 40)):
+        lens[at] = extra
+    p = problem(lens, 4, 4, 128, 16, BF16, seed=n, garbage=float("nan"))
+    check(p, 4, 4, 128, 16, lam_of(4))
+
+
 @pytest.mark.parametrize("window", [0, 1, 15, 16, 100, 511, 5000])
 def test_sliding_window(window):
     lens = [1, 16, 17, 130, 600, 0, 2500]
