@@ -358,6 +358,15 @@ def test_mla_prologue(dtype, T, H, interleave):
     assert torch.equal(only_cache.view(-1, 576)[slots[0].item()], out_kv[0])
 
 
+def test_mla_prologue_of_no_tokens():
+    table = ops.build_cos_sin_cache(ops.rope_frequencies(64, device=DEV)[0], 8)
+    cache = torch.full((2, 16, 1, 576), 3.0, dtype=BF16, device=DEV)
+    q, kv = torch.empty(0, 4, 64, dtype=BF16, device=DEV), torch.empty(0, 576, dtype=BF16, device=DEV)
+    none = torch.empty(0, dtype=torch.int64, device=DEV)
+    got = ops.mla_norm_rope_and_cache(q, kv, torch.ones(512, dtype=BF16, device=DEV), 1e-6, table, True, none, cache, none.int())
+    assert got[0] is q and got[1] is None and (cache == 3).all()
+
+
 @pytest.mark.parametrize("T", [1, 5])
 def test_mla_prologue_on_slices_of_one_buffer(T):
     """The latent rows and the queries of one projection's output, both in place."""

@@ -35,7 +35,7 @@
 //
 // Measured (bf16, 128-dim maps, 16-bit caches): 64 sequences of 0.5k to 4k tokens, 4 pairs, 16 heads (568 MB) 89 us and 6 us
 // of merge, 6.4 TB/s in the decode kernel; 256 sequences of 1k to 8k tokens, 32 heads (4.66 GB) 700 us and 11 us, 6.65 TB/s,
-// where a plain read of as many bytes runs at 7.05 TB/s.  4 sequences of up to 512 tokens: 5.9 us and 5.8 us, all latency (the
+// where a plain read of as many bytes runs at 7.05 TB/s.  4 sequences of up to 512 tokens: 5.8 us and 4.7 us, all latency (the
 // chain lengths -> page entries -> rows, then the merge's prefix -> parts).  Groups of sixteen heads (64 sequences, 64 heads):
 // 5.0 TB/s, bound by the moves between accumulation and ordinary registers around their 128 accumulators.
 #include "common.cuh"
@@ -53,10 +53,11 @@ constexpr int kDiffMaxBatch = 1024;           // sequences per launch (their pre
 // (One, two, four at least: 4 contexts of up to 512 tokens 11.4, 12.5, 14.9 us; one of 100 tokens 13.0, 15.9, 21.6 us; one
 // of 4000 tokens, which is then in 250, 125 or 62 parts, 24.4, 20.3, 21.7 us.)
 constexpr int kDiffMinStages = 2;
-// Output rows up to which the parts of a row are joined by a workgroup of 16 wavefronts, and of 4 (one wavefront beyond).
-// 16 rows of 250 parts: 12 us with 16, 30 us with 4; 1024 rows of 5 parts: 6 us with 4 and with one; 8192 rows of 2 parts:
-// 34 us with 4, 14 us with one.
-constexpr int64_t kDiffSplit16 = 256, kDiffSplit4 = 2048;
+// Output rows up to which the parts of a row are joined by a workgroup of 16 or 8 wavefronts, and of 4 (one wavefront beyond).
+// 1024 rows of 5 parts: 6 us with 4 and with one; 8192 rows of 2 parts: 34 us with 4, 14 us with one.  Up to 256 rows: 16
+// wavefronts where a row may have more than kDiffManyParts parts (16 rows of 250 parts: 12.5 us with 16, 15 with 8, 30 with
+// 4), 8 otherwise (32 rows of up to 16 parts: 4.4 us with 8 and 5.0 with 16; 256 rows of some 10: 5.2 and 6.0).
+constexpr int64_t kDiffSplit8 = 256, kDiffSplit4 = 2048, kDiffManyParts = 64;
 // Output rows from which the parts of 256-dim rows are stored past the caches (up to eight heads per pair).  In a row of
 // launches, the merge reading them right behind: 256 sequences x 16 heads of 1k to 8k tokens 695 us and 715 through the
 // caches, 128 x 32 heads 364 and 373, 512 x 16 heads of 0.5k to 2k 407 and 419; but 64 x 16 heads 98.5 and 97, 1 x 8 heads of
@@ -793,8 +794,13 @@ int launch_diff(const DiffArgs& a, hipStream_t stream) {
   // few rows: their contexts may be in many parts, which the wavefronts of a workgroup share; many rows: a wavefront each
   const unsigned batch = static_cast<unsigned>(a.batch), heads = static_cast<unsigned>(a.n_heads);
   const int64_t rows = static_cast<int64_t>(a.batch) * a.n_heads;
-  if (rows <= kDiffSplit16)
+  // (parts of a row: the teams by the contexts that share them, or what the table or the window leaves to split)
+  const int64_t shared = (a.n_workers >> a.team_shift) / (static_cast<int64_t>(a.batch) * ((a.n_pairs * a.hb_per_pair) >> a.team_shift));
+  const int64_t stages = (a.window_left >= 0 && a.window_left < a.max_len ? a.window_left : a.max_len) / kDiffTokens;
+  if (rows <= kDiffSplit8 && shared > kDiffManyParts && stages > kDiffManyParts)
     launch_timed(diff_merge_kernel<QT, D, NB, 16, true>, dim3(heads, batch), dim3(16 * kWave), 0, stream, a);
+  else if (rows <= kDiffSplit8)
+    launch_timed(diff_merge_kernel<QT, D, NB, 8, true>, dim3(heads, batch), dim3(8 * kWave), 0, stream, a);
   else if (rows <= kDiffSplit4)
     launch_timed(diff_merge_kernel<QT, D, NB, 4, true>, dim3(heads, batch), dim3(4 * kWave), 0, stream, a);
   else
