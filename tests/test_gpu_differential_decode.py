@@ -296,6 +296,96 @@ def test_refusals():
 
 
 # ------------------------------------------------------------------------------------------
+# tokens that take nearly all of the weight and bring no value: what is left are the small probabilities
+
+def sink_problem(lens, H, pairs, D, bs, dtype, nats, seed):
+    """A token in every 48 whose scores lie `nats` above 0 in both maps, where the others' are N(0, 1), and whose values are
+    zero.  (Every worker's share of a context holds one.)  The values of the others are positive, so that they add up."""
+    p = problem(lens, H, pairs, D, bs, dtype, seed=seed, garbage=float("nan"))
+    p["q"][..., 0], p["k"][..., 0] = 8.0, 0.0
+    p["v"].abs_()
+    for b, L in enumerate(lens):
+        t = torch.arange(L)[5::48]
+        slot = (p["table"][b].cpu()[t // bs].long() * bs + t % bs).to(DEV)
+        k, v = p["k"].view(-1, 2 * pairs, D), p["v"].view(-1, pairs, 2 * D)
+        k[slot], v[slot] = 0.0, 0.0
+        k[slot, :, 0] = nats * D ** 0.5 / 8.0
+    return p
+
+
+def sink_reference(p, H, pairs, D, bs, lam, weight, eps, out_scale):
+    """(result, bound) in 64 bits.  A score is a sum of D products in fp32 and one product more: (D + 2) 2^-24 of the sum of
+    their magnitudes, which is the relative error of its probability; exp2 adds 2^-22.  The weights are summed in fp32 by
+    fewer additions than there are tokens n, the values by at most 32 for every 16 tokens: 4 n 2^-24 together.  An error of
+    the weights counts twice, in o and in the sum that divides it.  Of two 16-bit parts bf16 leaves 2^-16 of a probability,
+    fp16 2^-22, and 2^-25 where the largest is at least 2^14: 2^-39 of the largest, for every token."""
+    half = torch.finfo(p["q"].dtype).eps / 2
+    fp16 = p["q"].dtype == FP16
+    B, g = p["q"].shape[0], H // pairs
+    out, bound = (torch.zeros(B, H, 2 * D, dtype=torch.float64, device=DEV) for _ in range(2))
+    for b, L in enumerate(p["lens"].tolist()):
+        t = torch.arange(L, device=DEV)
+        slot = p["table"][b, t // bs].long() * bs + t % bs
+        k = p["k"].view(-1, pairs, 2, D)[slot].double().repeat_interleave(g, 1)
+        v = p["v"].view(-1, pairs, 2 * D)[slot].double().repeat_interleave(g, 1).transpose(0, 1).contiguous()   # [H, t, 2 D]
+        q = p["q"][b].double().view(H, 2, D)
+        a = torch.softmax((q[None] * k).sum(-1).permute(1, 2, 0) * D ** -0.5, -1).contiguous()                  # [H, 2, t]
+        mag = (q.abs()[None] * k.abs()).sum(-1).amax(0) * D ** -0.5                                             # [H, 2]
+        part = 2.0 ** -22 if fp16 else 2.0 ** -16
+        rel = 2 * ((D + 2) * 2.0 ** -24 * mag + 2.0 ** -22) + 4 * L * 2.0 ** -24 + part
+        o = torch.matmul(a, v)                                                                                  # [H, 2, 2 D]
+        err = rel[..., None] * o
+        if fp16:
+            err = err + 2.0 ** -39 * a.amax(-1)[..., None] * v.sum(1)[:, None]
+        o, err = o[:, 0] - lam * o[:, 1], err[:, 0] + lam * err[:, 1]
+        f = torch.full((H, 1), out_scale, dtype=torch.float64, device=DEV)
+        if weight is not None:
+            rms = (o.square().mean(-1, keepdim=True) + eps).sqrt()
+            err = err + o.abs() * (err.square().mean(-1, keepdim=True).sqrt() / rms + 2.0 ** -21)
+            f = f * weight.double() / rms
+        out[b] = o * f
+        bound[b] = err * f.abs() * 1.01 + half * (out[b].abs() + err * f.abs())
+    return out, bound + torch.finfo(p["q"].dtype).smallest_normal * torch.finfo(p["q"].dtype).eps / 2
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("nats", [12, 15, 18])
+@pytest.mark.parametrize("D,H,pairs", [(64, 2, 1), (128, 4, 4), (128, 11, 1), (64, 20, 2)])
+def test_small_probabilities_beside_a_sink(dtype, nats, D, H, pairs):
+    """Contexts in parts and contexts that one worker holds, with the norm (which scales up what is left) and without (then
+    out_scale does)."""
+    w = (1 + 0.1 * torch.randn(2 * D, generator=torch.Generator().manual_seed(3))).to(dtype).to(DEV)
+    for lens in ([700, 60, 1], [90] * 600):
+        p = sink_problem(lens, H, pairs, D, 16, dtype, nats, seed=nats + D)
+        some = p if len(lens) < 9 else dict(p, q=p["q"][::97].contiguous(), table=p["table"][::97], lens=p["lens"][::97])
+        for lam, weight, eps, scale in ((0.5, w, 1e-16, 0.2), (1.0, w, 1e-16, 1.0), (0.25, None, 0.0, 2.0 ** 11)):
+            got = run(p, H, D, torch.tensor(lam, device=DEV), weight=weight, eps=eps, out_scale=scale)
+            if some is not p:
+                got = got[::97]
+            want, bound = sink_reference(some, H, pairs, D, 16, lam, weight, eps, scale)
+            worst = ((got.double() - want).abs() / bound).max().item()
+            assert worst <= 1.0, f"{len(lens)} contexts, lambda {lam}: error is {worst:.2f} of its bound"
+
+
+@pytest.mark.parametrize("D,H,pairs", [(128, 4, 2), (64, 12, 1)])
+def test_sharp_and_cancelling_maps_fp16(D, H, pairs):
+    """The same maps as in the bfloat16 test above, in fp16, whose probabilities are held otherwise."""
+    lens = [200, 1500]
+    p = problem(lens, H, pairs, D, 16, FP16, seed=9, spread=30.0)
+    w = torch.ones(2 * D, dtype=FP16, device=DEV)
+    check(p, H, pairs, D, 16, lam_of(H), weight=w, out_scale=0.5)
+    check(p, H, pairs, D, 16, torch.zeros(1, device=DEV))
+    same = dict(p)
+    same["q"] = p["q"].view(2, H, 2, D)[:, :, :1].expand(2, H, 2, D).reshape(2, 2 * H, D).contiguous()
+    same["k"] = p["k"].view(-1, 16, pairs, 2, D)[:, :, :, :1].expand(-1, 16, pairs, 2, D).reshape(p["k"].shape).contiguous()
+    assert (run(same, H, D, torch.ones(1, device=DEV)) == 0).all()
+    close = dict(same)
+    close["k"] = same["k"].clone()
+    close["k"][:, 3, 1::2] = p["k"][:, 3, 1::2]
+    check(close, H, pairs, D, 16, torch.full((1,), 0.9, device=DEV), weight=w)
+
+
+# ------------------------------------------------------------------------------------------
 # the operators of a step, together
 
 def rotate_rows64(x, pos, inv, interleave=False):

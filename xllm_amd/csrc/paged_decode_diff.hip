@@ -30,7 +30,11 @@
 // P is rounded to the 16-bit type in two parts, p = hi + lo, and both go through the matrix cores: the difference of the
 // maps can cancel most of o, which would leave the rounding of a single 16-bit P as the error of what remains (the norm
 // scales it up).  It is free: a stage's 16 tokens fill half the depth of a 16x16x32 MFMA, and the other half takes the same
-// values against lo.
+// values against lo.  What the parts leave over: of bf16 2^-16 of p.  Of fp16, whose values end at 2^-25, 2^-22 of p and
+// 2^-25 absolute; so its probabilities are held against a maximum 14 powers of two lower and reach 2^14 to 2^15
+// (DiffProbs), which leaves 2^-39 of the largest: a token 27 nats below the first one is lost from o, one 18 below keeps
+// 12 bits.  (Held against the maximum itself, where fp16's upper half lies idle, a context whose first token has no value
+// of its own -- a sink -- lost 42 % of its result at 18 nats.)
 // Softmax statistics, sums and the norm are in fp32.
 //
 // Measured (bf16, 128-dim maps, 16-bit caches): 64 sequences of 0.5k to 4k tokens, 4 pairs, 16 heads (568 MB) 89 us and 6 us
@@ -63,7 +67,17 @@ constexpr int64_t kDiffSplit8 = 256, kDiffSplit4 = 2048, kDiffManyParts = 64;
 // caches, 128 x 32 heads 364 and 373, 512 x 16 heads of 0.5k to 2k 407 and 419; but 64 x 16 heads 98.5 and 97, 1 x 8 heads of
 // 32k 41.4 and 39.2, groups of sixteen (64 x 64 heads) 142 and 137, rows of 128 dims (512 x 32 heads) 246 and 243.
 constexpr int64_t kDiffStreamRows = 4096;
-constexpr float kDiffSlack = 8.0f;            // a maximum moves when a score exceeds it by this much (log2 units)
+
+// The running maximum against which a worker holds its probabilities (log2 units): it is set kLift below the largest score
+// and moves when a score passes it by more than kLift + kSlack, so that e = exp2(s - m) stays below 2^(kLift + kSlack).
+// bf16 has fp32's range, and a wide slack keeps the moves rare.  fp16 ends at 2^16: the slack is what it can be with the
+// probabilities at the top of its range.  The moves that this adds (some two a context) are not seen in the times but for the
+// shape with the most accumulators (64 sequences, 64 heads of 128 dims, groups of sixteen: 132.3 us, 128.8 with bf16's values).
+template <typename QT>
+struct DiffProbs {
+  static constexpr float kLift = QT::kIsBf16 ? 0.0f : 14.0f;
+  static constexpr float kSlack = QT::kIsBf16 ? 8.0f : 1.0f;
+};
 
 typedef __attribute__((address_space(3))) s16x4 diff_lds_s16x4;
 
@@ -78,7 +92,7 @@ struct DiffArgs {
   const char* norm_w;
   int* ws_prefix;       // [batch + 1], written by workgroup 0 for the merge
   float* ws_o;          // [2 * workers][columns][2 D]
-  float* ws_ml;         // [2 * workers][columns][2]: maximum (log2 units), sum
+  float* ws_ml;         // [2 * workers][columns][2]: running maximum (log2 units, see DiffProbs), sum
   int64_t table_stride;
   int64_t q_stride_bytes;
   int64_t out_stride_bytes;
@@ -283,6 +297,7 @@ __global__ __launch_bounds__((DiffShape<D, NB>::kThreads), (DiffShape<D, NB>::kP
   constexpr int MB = 2 * D / 16;   // dim blocks of the output
   constexpr int NS = S::kStages;
   constexpr int NL = S::kLoads;
+  constexpr float kTop = DiffProbs<QT>::kLift + DiffProbs<QT>::kSlack;
   constexpr int kStageOps = 1 + 2 * NL;   // vector memory operations of a stage: page entries, keys, values
   static_assert(NS >= 2, "the wait for query rows leaves one younger stage in flight");
 
@@ -575,13 +590,14 @@ __global__ __launch_bounds__((DiffShape<D, NB>::kThreads), (DiffShape<D, NB>::kP
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         sv[r] = tok0 + r < cc.L && tok0 + r >= cc.lo ? sc[nb][r] * a.scale_log2 : -INFINITY;
-        over |= sv[r] > m[nb] + kDiffSlack;
+        over |= sv[r] > m[nb] + kTop;
       }
       if (__builtin_amdgcn_ballot_w64(over) != 0) {   // rare once the maxima have settled
         const float mx = diff_rows_max(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])));
-        if (mx > m[nb] + kDiffSlack) {
-          const float alpha = fast_exp2(m[nb] - mx);
-          m[nb] = mx;
+        if (mx > m[nb] + kTop) {
+          const float top = mx - DiffProbs<QT>::kLift;
+          const float alpha = fast_exp2(m[nb] - top);
+          m[nb] = top;
           l[nb] *= alpha;
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb) o[nb][mb] *= alpha;
