@@ -274,7 +274,7 @@ def neighbours(ops, workloads, torch, dev, steps, lib=None, capi=None):
     inv, factor = ops.rope_frequencies(128, base=500000.0, device=dev, scaling=ops.RopeScaling(
         "llama3", factor=8.0, original_max_position=8192))
     rows128 = torch.empty(131072, 128, device=dev)
-    row("build_cos_sin_cache", "rope_range_kernel", "131072 positions x 128, fp32",
+    row("build_cos_sin_cache", "rope_cos_sin_kernel", "131072 positions x 128, fp32",
         timed(lambda: ops.build_cos_sin_cache(inv, 131072, attention_factor=factor, out=rows128)), rows128.numel() * 4)
     # rotation of q and k of a prefill chunk in tensors of their own, in place
     q, k = qkv[:, :nq * D].view(T, nq, D), qkv[:, nq * D:(nq + nk) * D].view(T, nk, D)

@@ -95,6 +95,26 @@ def test_rows_into_a_given_tensor_and_far_positions():
     assert ops.build_cos_sin_cache(inv, position_ids=pos[:0]).shape == (0, 64)
 
 
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("dim,n", [(2, 300), (6, 3001), (32, 9001), (40, 7003), (96, 3001), (128, 33001), (256, 9001), (1024, 1500),
+                                   (2048, 1101)])
+@pytest.mark.parametrize("first", [0, 12345, 2 ** 22 - 5, 2 ** 40 + 3])
+def test_a_position_has_one_row(dtype, dim, n, first):
+    """The same bits for a position whichever way its row is asked for: in a long range, in ranges of a few rows that begin
+    anywhere, in a list, and into memory off the 16-byte boundary."""
+    inv, factor = ops.rope_frequencies(dim, scaling=ops.RopeScaling("yarn", factor=4.0, original_max_position=2048), device=DEV)
+    kw = dict(attention_factor=factor, dtype=dtype)
+    whole = ops.build_cos_sin_cache(inv, n, first_position=first, **kw)
+    order = torch.randperm(n, generator=torch.Generator().manual_seed(n)).to(DEV)
+    assert torch.equal(ops.build_cos_sin_cache(inv, position_ids=first + order, **kw), whole[order])
+    few = order[:50].contiguous()
+    assert torch.equal(ops.build_cos_sin_cache(inv, position_ids=first + few, **kw), whole[few])
+    for at, m in ((0, 1), (0, 9), (1, 8), (7, 2), (n // 2 + 3, 13), (n - 1, 1), (3, n - 5)):
+        assert torch.equal(ops.build_cos_sin_cache(inv, m, first_position=first + at, **kw), whole[at:at + m]), (at, m)
+    odd = torch.empty(n * dim + 1, dtype=dtype, device=DEV)[1:].view(n, dim)
+    assert torch.equal(ops.build_cos_sin_cache(inv, n, first_position=first, attention_factor=factor, out=odd), whole)
+
+
 # ------------------------------------------------------------------------------------------
 # rotation
 

@@ -81,38 +81,63 @@ struct Pack {
 
 // ---- cos | sin rows ------------------------------------------------------------------------------------------------
 
-// factor * cos and factor * sin of `angle`, in 64 bits up to the one rounding to fp32: the multiple of pi / 2 is taken off
-// in two parts (its product with the leading part is exact inside the fused multiply-add, so what is left of angles up to
-// 2^50 is good to 2^-52 of the angle), then the Taylor polynomials on [-pi/4, pi/4], whose first omitted terms are below
-// 8e-12 and 2e-10, a two-hundredth of half an fp32 step.  Quadrant and signs are settled on the rounded results:
-// comparisons in 64 bits were a fifth of the operations.
-__device__ __forceinline__ void cos_sin_64(double angle, double factor, float& c, float& s) {
-  const double q = __builtin_rint(angle * 0.63661977236758134308);
+// cos and sin of `angle` in 64 bits: the multiple q of pi / 2 is taken off in two parts (its product with the leading part is
+// exact inside the fused multiply-add, so what is left of angles up to 2^50 is good to 2^-52 of the angle), then polynomials
+// in r^2 on [-pi/4, pi/4], fitted for the smallest largest error of sin r (2.4e-12) and cos r (5.4e-11, a thousandth of an
+// fp32 step) with their leading terms r and 1 kept, so that position 0 gives 1 and 0.  Adding 1.5 2^52 rounds to an integer
+// and leaves it in the low bits of the sum: conversions and roundings in 64 bits run at a fraction of the rate of products.
+struct Quarter {   // sin and cos of what is left, and q mod 4
+  double s, c;
+  u32 k;
+};
+__device__ __forceinline__ Quarter sin_cos_64(double angle) {
+  constexpr double kShift = 6755399441055744.0;
+  const double shifted = __builtin_fma(angle, 0.63661977236758134308, kShift);
+  const double q = shifted - kShift;
   double r = __builtin_fma(-q, 1.5707963267948965580, angle);
   r = __builtin_fma(-q, 6.1232339957367660359e-17, r);
   const double z = r * r;
-  double ps = -1.0 / 39916800.0;
-  ps = __builtin_fma(ps, z, 1.0 / 362880.0);
-  ps = __builtin_fma(ps, z, -1.0 / 5040.0);
-  ps = __builtin_fma(ps, z, 1.0 / 120.0);
-  ps = __builtin_fma(ps, z, -1.0 / 6.0);
-  const float sr = static_cast<float>(__builtin_fma(r * z, ps, r) * factor);
-  double pc = -1.0 / 3628800.0;
-  pc = __builtin_fma(pc, z, 1.0 / 40320.0);
-  pc = __builtin_fma(pc, z, -1.0 / 720.0);
-  pc = __builtin_fma(pc, z, 1.0 / 24.0);
-  pc = __builtin_fma(pc, z, -0.5);
-  const float cr = static_cast<float>(__builtin_fma(pc, z, 1.0) * factor);
-  // the quadrant, q mod 4 (taken before it becomes an integer, which q may not fit)
-  const u32 k = static_cast<u32>(static_cast<int>(__builtin_fma(-4.0, __builtin_floor(q * 0.25), q)));
-  const bool swap = (k & 1u) != 0;
-  c = as_f32(as_u32(swap ? sr : cr) ^ ((k + 1u) & 2u) << 30);
-  s = as_f32(as_u32(swap ? cr : sr) ^ (k & 2u) << 30);
+  double ps = 2.716013937443816e-06, pc = 2.4390449888022627e-05;
+  ps = __builtin_fma(ps, z, -0.0001983904376152292);
+  ps = __builtin_fma(ps, z, 0.00833332823868483);
+  ps = __builtin_fma(ps, z, -0.16666666627998758);
+  pc = __builtin_fma(pc, z, -0.0013886763785924106);
+  pc = __builtin_fma(pc, z, 0.041666623324085626);
+  pc = __builtin_fma(pc, z, -0.4999999972510603);
+  return {__builtin_fma(r * z, ps, r), __builtin_fma(pc, z, 1.0), static_cast<u32>(__builtin_bit_cast(uint64_t, shifted))};
 }
 
-// Short ranges and listed positions: bound by the operations in 64 bits on top of the stores (131072 rows of 128 fp32 values:
-// 15.7 us, the stores alone 11.9 us, a plain fill of as many bytes 11.4 us).
-// One lane makes V consecutive pairs of a row: V cosines and V sines, 16 bytes of each where the row allows it.
+// V pairs of the row of a position, times `factor`, rounded to fp32 (and from there to the 16-bit types).  Quadrant and signs
+// are settled on the rounded results: comparisons in 64 bits were a fifth of the operations.
+template <int V>
+__device__ __forceinline__ void row_pairs(double pos, const double (&freq)[V], double factor, float (&c)[V], float (&s)[V]) {
+  Quarter t[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) t[i] = sin_cos_64(pos * freq[i]);
+  if (factor != 1.0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      t[i].s *= factor;
+      t[i].c *= factor;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float sr = static_cast<float>(t[i].s), cr = static_cast<float>(t[i].c);
+    const bool swap = (t[i].k & 1u) != 0;
+    c[i] = as_f32(as_u32(swap ? sr : cr) ^ ((t[i].k + 1u) & 2u) << 30);
+    s[i] = as_f32(as_u32(swap ? cr : sr) ^ (t[i].k & 2u) << 30);
+  }
+}
+
+// Every row is made by the formula above from its own position, so that a position has the same bits in a table made at load,
+// in a range of any length and in a step's listed rows.  (Turning a row into the next ones by its frequencies, one evaluation
+// for eight, took 12.8 us for 131072 rows of 128 fp32 values and 9.4 us of bf16; but a turned angle is not the rounded product
+// that a listed position has, and some values fell on the other side of their rounding.)
+// One lane makes V consecutive pairs of a row: V cosines and V sines, 16 bytes of each where the row allows it.  Bound by the
+// launch (64 rows of 128 values: 2.1 us), beyond that by 17 operations in 64 bits a pair, at half the rate of those in 32, on
+// top of the stores: 131072 rows of 128 values 14.5 us in fp32, where the stores alone take 11.9 us and a plain fill of as many
+// bytes 11.4 us, and 13.3 us in bf16.  (Several rows a lane: the same.)
 template <int DT, int V>
 __global__ __launch_bounds__(kRotThreads) void rope_cos_sin_kernel(const double* inv_freq, const int64_t* positions,
                                                                    int64_t first, int64_t n_units, int half, double factor,
@@ -124,10 +149,12 @@ __global__ __launch_bounds__(kRotThreads) void rope_cos_sin_kernel(const double*
   const int64_t row = n_units <= 0x7fffffffLL ? static_cast<u32>(unit) / static_cast<u32>(per) : unit / per;
   const int i0 = static_cast<int>(unit - row * per) * V;
   const double pos = static_cast<double>(positions != nullptr ? positions[row] : first + row);
+  double freq[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) freq[i] = inv_freq[i0 + i];
   typename Elem<DT>::T* p = out + row * (2 * static_cast<int64_t>(half)) + i0;
   float c[V], s[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) cos_sin_64(pos * inv_freq[i0 + i], factor, c[i], s[i]);
+  row_pairs<V>(pos, freq, factor, c, s);
   if constexpr (V == 1) {
     p[0] = Elem<DT>::put(c[0]);
     p[half] = Elem<DT>::put(s[0]);
@@ -143,111 +170,12 @@ __global__ __launch_bounds__(kRotThreads) void rope_cos_sin_kernel(const double*
   }
 }
 
-// cos and sin of `angle` in 64 bits (the same reduction, polynomials to the last place).
-__device__ __forceinline__ void cos_sin_exact(double angle, double& c, double& s) {
-  const double q = __builtin_rint(angle * 0.63661977236758134308);
-  double r = __builtin_fma(-q, 1.5707963267948965580, angle);
-  r = __builtin_fma(-q, 6.1232339957367660359e-17, r);
-  const double z = r * r;
-  double ps = 1.0 / 355687428096000.0, pc = 1.0 / 20922789888000.0;   // 1 / 17!, 1 / 16!
-  ps = __builtin_fma(ps, z, -1.0 / 1307674368000.0);
-  ps = __builtin_fma(ps, z, 1.0 / 6227020800.0);
-  ps = __builtin_fma(ps, z, -1.0 / 39916800.0);
-  ps = __builtin_fma(ps, z, 1.0 / 362880.0);
-  ps = __builtin_fma(ps, z, -1.0 / 5040.0);
-  ps = __builtin_fma(ps, z, 1.0 / 120.0);
-  ps = __builtin_fma(ps, z, -1.0 / 6.0);
-  pc = __builtin_fma(pc, z, -1.0 / 87178291200.0);
-  pc = __builtin_fma(pc, z, 1.0 / 479001600.0);
-  pc = __builtin_fma(pc, z, -1.0 / 3628800.0);
-  pc = __builtin_fma(pc, z, 1.0 / 40320.0);
-  pc = __builtin_fma(pc, z, -1.0 / 720.0);
-  pc = __builtin_fma(pc, z, 1.0 / 24.0);
-  pc = __builtin_fma(pc, z, -0.5);
-  const double sr = __builtin_fma(r * z, ps, r), cr = __builtin_fma(pc, z, 1.0);
-  const u32 k = static_cast<u32>(static_cast<int>(__builtin_fma(-4.0, __builtin_floor(q * 0.25), q)));
-  const bool swap = (k & 1u) != 0;
-  c = swap ? sr : cr;
-  s = swap ? cr : sr;
-  if (((k + 1u) & 2u) != 0) c = -c;
-  if ((k & 2u) != 0) s = -s;
-}
-
-// (Left to itself the compiler rounds from 64 to 16 bits in one step, by a dozen operations on integers: 10 us instead of 5
-// for 4096 rows of 128 bf16 values.)
-__device__ __forceinline__ float as_single(double x) {
-  float f = static_cast<float>(x);
-  asm("" : "+v"(f));
-  return f;
-}
-
-// The rows of consecutive positions.  A workgroup takes `stride` rows at a time, kRangeSteps times; a lane keeps its V pairs
-// and turns them by stride * inv_freq from one of its rows to the next, in 64 bits: 4 operations a pair instead of 30, and
-// the turns add 1e-15.
-constexpr int kRangeSteps = 8;
-// Lanes of rope_cos_sin_kernel beyond which this one is faster; its own are an eighth as many.  262144 lanes: 65536 rows of 32
-// fp32 values 4.2 and 4.4 us here, 16384 of 256 bf16 values 5.2 and 6.0; 393216 (65536 rows of 96 bf16 values) 7.2 and 6.0;
-// 131072 rows of 128 fp32 values 15.7 and 12.7, of bf16 values 14.9 and 9.5.
-constexpr int64_t kRangeUnits = 262144;
-template <int DT, int V>
-__global__ __launch_bounds__(kRotThreads) void rope_range_kernel(const double* inv_freq, int64_t first, int64_t n_rows, int half,
-                                                                 int per, int stride, double factor, typename Elem<DT>::T* out) {
-  extern __shared__ double turn[];   // [half] cosines, [half] sines of the turn
-  for (int i = threadIdx.x; i < half; i += kRotThreads) cos_sin_exact(stride * inv_freq[i], turn[i], turn[half + i]);
-  const int line = static_cast<int>(static_cast<u32>(threadIdx.x) / static_cast<u32>(per));
-  const int i0 = (static_cast<int>(threadIdx.x) - line * per) * V;
-  int64_t row = static_cast<int64_t>(blockIdx.x) * (stride * kRangeSteps) + line;
-  double c[V], s[V], dc[V], ds[V];
-  const double pos = static_cast<double>(first + row);
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    cos_sin_exact(pos * inv_freq[i0 + i], c[i], s[i]);
-    c[i] *= factor;
-    s[i] *= factor;
-  }
-  __syncthreads();
-  if (line >= stride) return;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    dc[i] = turn[i0 + i];
-    ds[i] = turn[half + i0 + i];
-  }
-#pragma unroll
-  for (int k = 0; k < kRangeSteps; ++k, row += stride) {
-    if (row >= n_rows) return;
-    Pack<DT, V> a, b;
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      a.put2(i, as_single(c[2 * i]), as_single(c[2 * i + 1]));
-      b.put2(i, as_single(s[2 * i]), as_single(s[2 * i + 1]));
-    }
-    typename Elem<DT>::T* p = out + row * (2 * static_cast<int64_t>(half)) + i0;
-    a.store(p);
-    b.store(p + half);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const double t = c[i];
-      c[i] = __builtin_fma(t, dc[i], -(s[i] * ds[i]));
-      s[i] = __builtin_fma(s[i], dc[i], t * ds[i]);
-    }
-  }
-}
-
 template <int DT>
 int launch_cos_sin(const double* inv_freq, const int64_t* positions, int64_t first, int64_t rows, int64_t half,
                    double factor, void* out, hipStream_t stream) {
   constexpr int V = DT == XLLM_MI355_FP32 ? 4 : 8;
   using T = typename Elem<DT>::T;
   const bool wide = half % V == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  const int64_t per = half / V, stride = wide && per <= kRotThreads ? kRotThreads / per : 0;
-  if (positions == nullptr && stride > 0 && rows * per > kRangeUnits) {
-    const int64_t groups = (rows + stride * kRangeSteps - 1) / (stride * kRangeSteps);
-    if (groups > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
-    rope_range_kernel<DT, V><<<dim3(static_cast<unsigned>(groups)), kRotThreads, static_cast<size_t>(half) * 16, stream>>>(
-        inv_freq, first, rows, static_cast<int>(half), static_cast<int>(per), static_cast<int>(stride), factor,
-        static_cast<T*>(out));
-    return static_cast<int>(hipGetLastError());
-  }
   const int64_t units = rows * (wide ? half / V : half);
   const int64_t groups = (units + kRotThreads - 1) / kRotThreads;
   if (groups > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
