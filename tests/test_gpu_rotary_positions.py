@@ -265,6 +265,34 @@ def test_gradient_and_inverse():
         assert (back - x).abs().max() <= 2.0 ** -21 * x.abs().max()
 
 
+def test_gradient_through_an_autograd_function():
+    """What a training step does: the rotation in the forward, its transpose in the backward.  Outside of one, an operand that
+    requires grad is refused instead of losing its gradient."""
+    T, H, D = 5, 3, 64
+    table, pos = table_of(50, 32, FP32), torch.randint(0, 50, (T,), device=DEV)
+
+    class Rotate(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return ops.rotary_embedding(pos, x, None, table, rotary_offset=8, out_query=torch.empty_like(x))[0]
+
+        @staticmethod
+        def backward(ctx, g):
+            return ops.rotary_embedding(pos, g.contiguous(), None, table, rotary_offset=8, inverse=True, out_query=torch.empty_like(g))[0]
+
+    x, y = torch.randn(T, H, D, device=DEV, requires_grad=True), torch.randn(T, H, D, device=DEV)
+    (Rotate.apply(x) * y).sum().backward()
+    want, bound = rotate64(y, table, pos, 8, False, True)   # the formula's gradient: the transposed map of y
+    assert ((x.grad.double() - want).abs() <= bound + half_step(FP32) * (want.abs() + bound)).all()
+    for call in (ops.rotary_embedding, lambda *a: torch.ops.xllm_ops.rotary_embedding(*a)):
+        with pytest.raises((ValueError, RuntimeError)):
+            call(pos, x, None, table)
+    before = x.detach().clone()
+    with torch.no_grad():
+        ops.rotary_embedding(pos, x, None, table)
+    assert_rotated(x.detach(), before, table, pos, 0, False, False)
+
+
 def test_infinities_and_nan_stay_in_their_pair():
     T, H, D = 4, 4, 64
     x = torch.randn(T, H, D, device=DEV).to(BF16)

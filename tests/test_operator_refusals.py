@@ -195,3 +195,32 @@ def test_cpu_tensors_are_refused():
 def test_frequencies_need_no_gpu():
     inv, factor = ops.rope_frequencies(64, scaling=ops.RopeScaling("linear", factor=2.0), device="cpu")
     assert inv.dtype == torch.float64 and inv[0] == 0.5 and factor == 1.0
+
+
+def test_operands_that_require_grad_are_refused_while_a_graph_is_recorded():
+    """No operator records a graph, so a gradient would be lost without a word.  (Under no_grad the call goes on, to the
+    refusal of host tensors.)"""
+    def grad(*shape, dtype=torch.bfloat16):
+        return torch.zeros(*shape, dtype=dtype, requires_grad=True)
+
+    def plain(*shape, dtype=torch.bfloat16):
+        return torch.zeros(*shape, dtype=dtype)
+
+    pos, rows, slots = torch.zeros(1, dtype=torch.int64), torch.zeros(4, 64), torch.zeros(1, dtype=torch.int32)
+    rot = dict(position_ids=pos, query=plain(1, 2, 64), key=plain(1, 2, 64), cos_sin_cache=rows, out_query=plain(1, 2, 64),
+               out_key=plain(1, 2, 64))
+    mla = dict(q_pe=plain(1, 2, 64), kv=plain(1, 576), kv_norm_weight=plain(512), eps=1e-6, cos_sin_cache=rows, interleave=True,
+               position_ids=pos, k_cache=plain(1, 16, 1, 576), slot_mapping=slots, out_q_pe=plain(1, 2, 64), out_kv=plain(1, 576))
+    diff = dict(query=plain(1, 2, 64), k_cache=plain(1, 16, 2, 64), v_cache=plain(1, 16, 1, 128), output=plain(1, 1, 128),
+                block_table=slots.view(1, 1), seq_lens=slots, lambda_=torch.zeros(1), norm_weight=plain(128))
+    angles = dict(inv_freq=torch.ones(4, dtype=torch.float64), num_positions=3, out=torch.zeros(3, 8))
+    for fn, base in ((ops.rotary_embedding, rot), (ops.mla_norm_rope_and_cache, mla), (ops.batch_decode_diff, diff),
+                     (ops.build_cos_sin_cache, angles)):
+        for name, x in base.items():
+            if not torch.is_tensor(x) or not x.is_floating_point():
+                continue
+            args = dict(base, **{name: grad(*x.shape, dtype=x.dtype)})
+            with pytest.raises(ValueError, match="records no graph"):
+                fn(**args)
+            with torch.no_grad(), pytest.raises(ValueError, match="GPU only"):
+                fn(**args)

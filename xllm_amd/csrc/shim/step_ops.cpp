@@ -3,6 +3,7 @@
 // functions of the same names call the same code through step_ops_python.cpp.  The checks cost a microsecond here and five
 // in Python.  A violated precondition is a ValueError or a TypeError.
 #include <ATen/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
@@ -33,6 +34,15 @@ void check_rc(int rc, const char* what, const char* overlap) {
 }
 
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// These calls record no graph.  Where one would be recorded, an operand that requires grad is refused, as by the out= forms of
+// torch's own functions: its gradient would be lost without a word.
+void check_no_graph(const char* what, std::initializer_list<const Tensor*> operands) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (const Tensor* t : operands)
+    TORCH_CHECK_VALUE(!t->defined() || !t->requires_grad(), what, " records no graph, but one of its operands requires grad: call "
+                      "it under torch.no_grad(), or in the forward of a torch.autograd.Function");
+}
 
 void check_device(const Tensor& first, std::initializer_list<const Tensor*> rest) {
   TORCH_CHECK_VALUE(first.is_cuda(), "this path runs on the GPU only: every tensor must be a device tensor");
@@ -145,6 +155,8 @@ StepTables step_tables_memory(const Tensor& kv_lens, int64_t max_new_tokens) {
 
 Tensor build_cos_sin_cache(const Tensor& inv_freq, const OptTensor& position_ids, int64_t num_positions,
                            int64_t first_position, double attention_factor, torch::ScalarType dtype, const OptTensor& out_rows) {
+  const Tensor none;
+  check_no_graph("build_cos_sin_cache", {&inv_freq, given(out_rows) ? &*out_rows : &none});
   check_device(inv_freq, {});
   check_vector(inv_freq, torch::kFloat64, -1, "inv_freq");
   TORCH_CHECK_VALUE(inv_freq.numel() > 0, "inv_freq is empty");
@@ -182,6 +194,7 @@ void rotary_embedding(const Tensor& position_ids, const Tensor& query, const Opt
   const Tensor k = given(key) ? *key : Tensor();
   const Tensor ok = given(out_key) ? *out_key : k;
   TORCH_CHECK_VALUE(k.defined() || !ok.defined(), "out_key without a key");
+  check_no_graph("rotary_embedding", {&query, &k, &cos_sin_cache, &oq, &ok});
   check_device(query, {&position_ids, &cos_sin_cache, &oq, &k, &ok});
   const Heads hq = heads_of(query, oq, "query");
   check_rows(cos_sin_cache, position_ids, hq.T);
@@ -212,6 +225,7 @@ void mla_norm_rope_and_cache(const Tensor& q_pe, const Tensor& kv, const Tensor&
   const Tensor oq = given(out_q_pe) ? *out_q_pe : q_pe;
   const Tensor cache = given(k_cache) ? *k_cache : Tensor(), slots = given(slot_mapping) ? *slot_mapping : Tensor();
   const Tensor okv = given(out_kv) ? *out_kv : Tensor();
+  check_no_graph("mla_norm_rope_and_cache", {&q_pe, &kv, &kv_norm_weight, &cos_sin_cache, &cache, &oq, &okv});
   check_device(q_pe, {&kv, &kv_norm_weight, &cos_sin_cache, &position_ids, &cache, &slots, &oq, &okv});
   TORCH_CHECK_TYPE(q_pe.scalar_type() == torch::kBFloat16 || q_pe.scalar_type() == torch::kFloat16, "q_pe must be bfloat16 or float16");
   const Heads h = heads_of(q_pe, oq, "q_pe");
@@ -253,6 +267,7 @@ void batch_decode_diff(const Tensor& query, const Tensor& k_cache, const Tensor&
                        const Tensor& block_table, const Tensor& seq_lens, const Tensor& lambda, double scale,
                        const OptTensor& norm_weight, double eps, double out_scale, int64_t window_left) {
   const Tensor weight = given(norm_weight) ? *norm_weight : Tensor();
+  check_no_graph("batch_decode_diff", {&query, &k_cache, &v_cache, &output, &lambda, &weight});
   check_device(query, {&k_cache, &v_cache, &output, &block_table, &seq_lens, &lambda, &weight});
   TORCH_CHECK_TYPE(query.scalar_type() == torch::kBFloat16 || query.scalar_type() == torch::kFloat16,
                    "query must be bfloat16 or float16");

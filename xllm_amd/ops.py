@@ -25,6 +25,8 @@ Operators around the path that the reference does on the host, in its layers or 
   batch_decode_diff                               (no counterpart: the difference of two softmax maps)
 
 Errors: the reference CHECK-aborts; here every violated precondition raises.
+Gradients: no operator here records an autograd graph.  The five operators around the path refuse operands that require grad
+where one would be recorded; the others take them as plain values.
 """
 import functools
 import math
@@ -949,7 +951,8 @@ def rotary_embedding(position_ids, query, key, cos_sin_cache, interleave=False, 
     cos_sin_cache [max_position, rotary_dim] (build_cos_sin_cache); position_ids [T] int64: a position outside the cache is
     not rotated.  rotary_offset: where the rotated part of a head begins (key_rotary_offset: of a key head, if elsewhere).
     interleave: pairs (2i, 2i + 1), else (i, i + rotary_dim / 2).  inverse: the transposed map, which undoes a rotation by
-    unscaled rows and turns the gradient of the result into the gradient of the input.
+    unscaled rows and turns the gradient of the result into the gradient of the input (no graph is recorded: a training step
+    calls both from a torch.autograd.Function).
     Works in place, or into out_query / out_key.  Returns (query's result, key's result or None)."""
     _host_side().rotary_embedding(position_ids, query, key, cos_sin_cache, bool(interleave), rotary_offset,
                                   key_rotary_offset, bool(inverse), out_query, out_key)
