@@ -103,3 +103,45 @@ def test_differential_decode(xops):
                 (q, k, v, got, table, lens, lam.double(), 0.2), (q, k, v, got.float(), table, lens, lam, 0.2), (q, k, v, got, table, lens, lam, -1.0)):
         with pytest.raises((ValueError, TypeError)):
             xops.batch_decode_diff(*bad)
+
+
+def test_results_count_as_written_in_place(xops):
+    """A backward pass over values that a call has overwritten fails, as after torch's own in-place functions."""
+    T, H, D = 3, 2, 64
+    inv, _ = ops.rope_frequencies(D, device=DEV)
+    rows, pos = ops.build_cos_sin_cache(inv, 8), torch.arange(T, device=DEV)
+    for fn in (ops.rotary_embedding, xops.rotary_embedding):
+        x = torch.randn(T, H, D, device=DEV, requires_grad=True)
+        y = x.exp()   # (keeps its result for the backward pass)
+        with torch.no_grad():
+            fn(pos, y.detach(), None, rows)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+    def versions(*tensors):
+        return [t._version for t in tensors]
+
+    kv, q = torch.zeros(T, 576, dtype=BF16, device=DEV), torch.zeros(T, H, D, dtype=BF16, device=DEV)
+    cache, w = torch.zeros(1, 16, 1, 576, dtype=BF16, device=DEV), torch.ones(512, dtype=BF16, device=DEV)
+    before = versions(q, kv, cache, w, rows, pos)
+    ops.mla_norm_rope_and_cache(q, kv, w, 1e-6, rows, True, pos, k_cache=cache, slot_mapping=pos.int(), out_kv=kv)
+    assert [a - b for a, b in zip(versions(q, kv, cache, w, rows, pos), before)] == [1, 1, 1, 0, 0, 0]
+    out, key = torch.empty_like(q), torch.empty_like(q)
+    before = versions(q, kv, rows, out, key)
+    ops.rotary_embedding(pos, q, q.clone(), rows, out_query=out, out_key=key)
+    ops.build_cos_sin_cache(inv, 8, out=rows)
+    assert [a - b for a, b in zip(versions(q, kv, rows, out, key), before)] == [0, 0, 1, 1, 1]
+    t = ops.build_step_tables(i32([1, 2]), i32([1, 1]), i32([[0, 1], [2, 3]]), i32([4, 5]), 16, 4)
+    before = versions(t.block_table, t.slot_mapping, t.counters)
+    ops.build_step_tables(i32([1, 2]), i32([1, 1]), i32([[0, 1], [2, 3]]), i32([4, 5]), 16, 4, out=t)
+    assert all(a > b for a, b in zip(versions(t.block_table, t.slot_mapping, t.counters), before))
+    lens, lam = i32([5]), torch.zeros(1, device=DEV)
+    k, v, o = torch.zeros(1, 16, 2, D, dtype=BF16, device=DEV), torch.zeros(1, 16, 1, 2 * D, dtype=BF16, device=DEV), \
+        torch.zeros(1, 1, 2 * D, dtype=BF16, device=DEV)
+    before = versions(q, k, v, o)
+    ops.batch_decode_diff(q[:1], k, v, o, i32([[0]]), lens, lam)
+    assert [a - b for a, b in zip(versions(q, k, v, o), before)] == [0, 0, 0, 1]
+    with torch.inference_mode():
+        made = ops.build_cos_sin_cache(inv, 8)
+        ops.rotary_embedding(pos, torch.zeros(T, H, D, device=DEV), None, made)
+    ops.rotary_embedding(pos, torch.zeros(T, H, D, device=DEV), None, made)   # (a table made in inference mode, read outside)

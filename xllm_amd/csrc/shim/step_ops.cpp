@@ -44,6 +44,13 @@ void check_no_graph(const char* what, std::initializer_list<const Tensor*> opera
                       "it under torch.no_grad(), or in the forward of a torch.autograd.Function");
 }
 
+// Autograd keeps what its backward passes read by version: a tensor written here counts as written in place, so that a backward
+// pass over its former values fails instead of using the new ones.  (Tensors made in inference mode have no version.)
+void mark_written(std::initializer_list<const Tensor*> results) {
+  for (const Tensor* t : results)
+    if (t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 void check_device(const Tensor& first, std::initializer_list<const Tensor*> rest) {
   TORCH_CHECK_VALUE(first.is_cuda(), "this path runs on the GPU only: every tensor must be a device tensor");
   for (const Tensor* t : rest) {
@@ -137,6 +144,8 @@ void build_step_tables(const Tensor& kv_lens, const Tensor& new_lens, const Tens
                B, block_size, T, stream_of(kv_lens)),
            "xllm_mi355_build_step_tables",
            "an output of build_step_tables overlaps an input or another output (in place means block_table itself)");
+  mark_written({&out.block_table, &out.seq_lens, &out.q_cu_seq_lens, &out.position_ids, &out.slot_mapping, &out.new_page_indptr,
+                &out.counters});
 }
 
 StepTables step_tables_memory(const Tensor& kv_lens, int64_t max_new_tokens) {
@@ -184,6 +193,7 @@ Tensor build_cos_sin_cache(const Tensor& inv_freq, const OptTensor& position_ids
                                    first_position, rows, inv_freq.numel(), attention_factor, out.data_ptr(),
                                    code_of(out, "cos_sin rows"), stream_of(out)),
            "xllm_mi355_rope_cos_sin", "out overlaps an input");
+  mark_written({&out});
   return out;
 }
 
@@ -216,6 +226,7 @@ void rotary_embedding(const Tensor& position_ids, const Tensor& query, const Opt
                code_of(cos_sin_cache, "cos_sin_cache"), stream_of(query)),
            "xllm_mi355_rotary_embedding",
            "a result of rotary_embedding overlaps itself, the other one or an input (in place means the operand itself)");
+  mark_written({&oq, &ok});
 }
 
 void mla_norm_rope_and_cache(const Tensor& q_pe, const Tensor& kv, const Tensor& kv_norm_weight, double eps,
@@ -261,6 +272,7 @@ void mla_norm_rope_and_cache(const Tensor& q_pe, const Tensor& kv, const Tensor&
                interleave ? 1 : 0, code_of(q_pe, "q_pe"), code_of(cos_sin_cache, "cos_sin_cache"), stream_of(q_pe)),
            "xllm_mi355_mla_norm_rope_and_cache",
            "a result of mla_norm_rope_and_cache overlaps itself, another one or an input (in place means the operand itself)");
+  mark_written({&oq, &okv, &cache});
 }
 
 void batch_decode_diff(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache, Tensor& output,
@@ -314,6 +326,7 @@ void batch_decode_diff(const Tensor& query, const Tensor& k_cache, const Tensor&
                stride_or(output, 0, row), window_left, static_cast<float>(scale), ws.data_ptr(), bytes, code_of(query, "query"),
                stream_of(query)),
            "xllm_mi355_paged_decode_diff", "output overlaps an input");
+  mark_written({&output});
 }
 
 }  // namespace xllm::kernel::mi355
