@@ -569,6 +569,8 @@ int xllm_mi355_decode_metadata_update(const int32_t* src_tokens, const int32_t* 
  * A slot that would not fit 31 bits, or whose kept entry is negative, is -1 as well.  Outputs must not overlap kv_lens,
  * new_lens, free_pages or free_head.  max_new_tokens, n_free, table_width and block_size below 2^30, batch up to 2^20.
  * One launch for up to 4096 requests, two beyond; integer arithmetic only, the same result every time.
+ * batch 0: nothing is launched and NO output is written.  A caller with persistent buffers sets slots to -1 and counters to
+ * {0, free_head[0], 0} itself before anything reads them (the torch host sides of this library do).
  */
 int xllm_mi355_build_step_tables(const int32_t* kv_lens, const int32_t* new_lens,
                                  const int32_t* block_table_in, int64_t in_stride,

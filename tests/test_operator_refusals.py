@@ -37,6 +37,18 @@ def test_step_tables():
         assert call(fn, base, **change) == ESHAPE, change
 
 
+def test_an_empty_batch_leaves_the_results_alone():
+    """No requests: the C entry writes nothing, as its header says (host memory here; a write would be seen)."""
+    fn = capi.lib().xllm_mi355_build_step_tables
+    outs = [torch.full((n,), 77, dtype=dt) for n, dt in ((8, torch.int32), (1, torch.int32), (1, torch.int32), (8, torch.int64),
+                                                         (8, torch.int32), (1, torch.int32), (3, torch.int32))]
+    table, seq, cu, pos, slots, indptr, counters = (o.data_ptr() for o in outs)
+    lens, free, head = torch.zeros(1, dtype=torch.int32), torch.arange(9, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    assert fn(lens.data_ptr(), lens.data_ptr(), table, 8, table, 8, 8, free.data_ptr(), 9, head.data_ptr(), seq, cu, pos, slots,
+              indptr, counters, 0, 16, 8, None) == 0
+    assert all((o == 77).all() for o in outs)
+
+
 def test_cos_sin_rows():
     fn = capi.lib().xllm_mi355_rope_cos_sin
     base = dict(inv=FAKE, pos=None, first=0, rows=4, half=32, factor=1.0, out=FAKE, dtype=FP32, stream=None)
