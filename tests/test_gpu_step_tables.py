@@ -206,6 +206,22 @@ def test_no_requests():
     assert got.counters.tolist() == [0, 2, 0] and got.slot_mapping.tolist() == [-1] * 3 and got.position_ids.tolist() == [0] * 3
 
 
+@pytest.mark.parametrize("B", [0, 3])
+def test_a_free_head_inside_the_results_is_refused(B):
+    """The next step's head is counters[1]; handed over as a view of the very counters that the call writes it would be lost."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    kv, new, table, free = torch.zeros(B, **i32), torch.ones(B, **i32), torch.zeros(B, 4, **i32), torch.arange(9, **i32)
+    out = ops.build_step_tables(kv, new, table, free, 16, 6, torch.tensor([2], **i32))
+    head = int(out.counters[1])
+    assert head == 2 + B
+    for view in (out.counters[1:2], out.q_cu_seq_lens[:1], out.new_page_indptr[:1], out.slot_mapping[5:6]):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.build_step_tables(kv, new, table, free, 16, 6, view, out=out)
+    assert int(out.counters[1]) == head
+    ops.build_step_tables(kv, new, table, free, 16, 6, out.counters[1:2].clone(), out=out)
+    assert int(out.counters[1]) == head + B
+
+
 def test_refusals():
     i32 = dict(dtype=torch.int32, device="cuda")
     kv, new, table, free = torch.zeros(4, **i32), torch.ones(4, **i32), torch.zeros(4, 3, **i32), torch.arange(9, **i32)

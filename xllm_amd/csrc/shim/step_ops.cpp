@@ -128,7 +128,14 @@ void build_step_tables(const Tensor& kv_lens, const Tensor& new_lens, const Tens
   make(out.slot_mapping, T, torch::kInt32, "out.slot_mapping");
   make(out.new_page_indptr, B + 1, torch::kInt32, "out.new_page_indptr");
   make(out.counters, 3, torch::kInt32, "out.counters");
+  constexpr const char* kOverlap = "an output of build_step_tables overlaps an input or another output (in place means "
+                                   "block_table itself)";
   if (B == 0) {   // no requests: offsets and counters of an empty step
+    if (given(free_head))
+      for (const Tensor* t : {&out.q_cu_seq_lens, &out.new_page_indptr, &out.counters, &out.position_ids, &out.slot_mapping}) {
+        const char *lo = static_cast<const char*>(t->data_ptr()), *head = static_cast<const char*>(free_head->data_ptr());
+        TORCH_CHECK_VALUE(head < lo || head >= lo + t->nbytes(), kOverlap);
+      }
     for (const Tensor* t : {&out.q_cu_seq_lens, &out.new_page_indptr, &out.counters, &out.position_ids}) t->zero_();
     out.slot_mapping.fill_(-1);
     if (given(free_head)) out.counters.slice(0, 1, 2).copy_(free_head->view({1}).clamp(0, free_pages.numel()));
@@ -142,8 +149,7 @@ void build_step_tables(const Tensor& kv_lens, const Tensor& new_lens, const Tens
                out.seq_lens.data_ptr<int32_t>(), out.q_cu_seq_lens.data_ptr<int32_t>(), out.position_ids.data_ptr<int64_t>(),
                out.slot_mapping.data_ptr<int32_t>(), out.new_page_indptr.data_ptr<int32_t>(), out.counters.data_ptr<int32_t>(),
                B, block_size, T, stream_of(kv_lens)),
-           "xllm_mi355_build_step_tables",
-           "an output of build_step_tables overlaps an input or another output (in place means block_table itself)");
+           "xllm_mi355_build_step_tables", kOverlap);
   mark_written({&out.block_table, &out.seq_lens, &out.q_cu_seq_lens, &out.position_ids, &out.slot_mapping, &out.new_page_indptr,
                 &out.counters});
 }
