@@ -295,6 +295,17 @@ def test_refusals():
     assert ops.batch_decode_diff(p["q"][:0], p["k"], p["v"], none, p["table"][:0], p["lens"][:0], lam) is none
 
 
+def test_refusals_name_their_reason():
+    """What only the library knew it refused is not reported as an overlap."""
+    p = problem([20, 30], 4, 2, 64, 16, BF16)
+    out = torch.empty(2, 4, 128, dtype=BF16, device=DEV)
+    with pytest.raises(ValueError, match="scale must be positive"):
+        ops.batch_decode_diff(p["q"], p["k"], p["v"], out, p["table"], p["lens"], lam_of(4), scale=1e-60)   # (0 in 32 bits)
+    q, o = torch.zeros(1, 2 * 65536, 64, dtype=BF16, device=DEV), torch.zeros(1, 65536, 128, dtype=BF16, device=DEV)
+    with pytest.raises(ValueError, match="heads"):
+        ops.batch_decode_diff(q, p["k"], p["v"], o, p["table"][:1], p["lens"][:1], torch.zeros(1, device=DEV))
+
+
 # ------------------------------------------------------------------------------------------
 # tokens that take nearly all of the weight and bring no value: what is left are the small probabilities
 

@@ -318,7 +318,8 @@ void batch_decode_diff(const Tensor& query, const Tensor& k_cache, const Tensor&
   }
   TORCH_CHECK_VALUE(!weight.defined() || (weight.scalar_type() == query.scalar_type() && weight.numel() == 2 * D && weight.is_contiguous()),
               "norm_weight must be contiguous [2 D] of query's dtype");
-  TORCH_CHECK_VALUE(scale > 0 && eps >= 0, "scale must be positive and eps not negative");
+  TORCH_CHECK_VALUE(static_cast<float>(scale) > 0 && eps >= 0, "scale must be positive (in 32 bits) and eps not negative");
+  TORCH_CHECK_VALUE(H <= 65535, "at most 65535 differential heads");
   TORCH_CHECK_VALUE(B <= 1 || query.stride(0) >= row, "query: rows must not overlap");
   if (B == 0) return;
   const c10::DeviceGuard guard(query.device());
