@@ -586,7 +586,8 @@ int xllm_mi355_build_step_tables(const int32_t* kv_lens, const int32_t* new_lens
  * 10^5 is off by 4e-3) and one rounding to out_dtype; angles up to 2^50 in magnitude.  position(r) = positions[r], or first_position + r where positions is
  * null.  Frequencies scaled for long contexts (the reference's rotary_embedding files in
  * xllm/core/layers/common/) are the caller's inv_freq and factor; ops.rope_frequencies makes them.
- * inv_freq: [half] fp64; out: [n_rows, 2 * half] contiguous, of out_dtype (fp32, bf16, fp16).  half up to 4096.
+ * inv_freq: [half] fp64; out: [n_rows, 2 * half] contiguous, of out_dtype (fp32, bf16, fp16).  half up to 4096.  A lane makes
+ * 4 pairs of fp32 or 8 of the 16-bit types (one where half or out is no multiple of 16 bytes); one call takes up to 2^32 lanes.
  */
 int xllm_mi355_rope_cos_sin(const double* inv_freq, const int64_t* positions, int64_t first_position,
                             int64_t n_rows, int64_t half, double factor, void* out, int out_dtype, void* stream);
@@ -601,7 +602,8 @@ int xllm_mi355_rope_cos_sin(const double* inv_freq, const int64_t* positions, in
  *   cos_sin [n_positions, rotary_dim] contiguous, cos then sin.  A position outside [0, n_positions) is not rotated.
  *   interleave  nonzero: pairs (2i, 2i + 1); zero: pairs (i, i + rotary_dim / 2)
  *   inverse     nonzero: the transposed map (sin negated): undoes a rotation, and is its gradient
- * dtype: bf16, fp16 or fp32; any even rotary_dim, any alignment (16-byte aligned operands take the fast path).
+ * dtype: bf16, fp16 or fp32; any even rotary_dim, any alignment (16-byte aligned operands take the fast path).  A lane takes
+ * 16 bytes of pairs (one pair where operands are not aligned); one call takes up to 2^32 lanes.
  */
 int xllm_mi355_rotary_embedding(const int64_t* positions, const void* cos_sin, int64_t n_positions,
                                 const void* q, void* q_out, const void* k, void* k_out,
@@ -622,7 +624,7 @@ int xllm_mi355_rotary_embedding(const int64_t* positions, const void* cos_sin, i
  * what xllm_mi355_paged_decode_mla reads; it may be q_pe itself), kv, kv_out rows of 576 with a row stride (kv_out null or
  * kv itself or apart), cache [num_blocks, block_size, 1, 576] or null (one of kv_out and cache is needed).  Slots outside
  * the cache are skipped, the others are distinct; a position outside [0, n_positions) is not rotated.  Arithmetic in fp32,
- * rounded once to dtype (bf16, fp16).  Pointers and strides multiples of 16 bytes.
+ * rounded once to dtype (bf16, fp16).  Pointers and strides multiples of 16 bytes.  n_tokens * (4 n_heads + 64) below 2^32.
  */
 int xllm_mi355_mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const void* kv, void* kv_out,
                                        const void* kv_weight, float eps,

@@ -93,6 +93,19 @@ def test_mla_prologue():
         assert call(fn, base, **change) == EALIGN, change
 
 
+def test_launches_beyond_32_bits_of_threads():
+    lib = capi.lib()
+    far = [1 << 44, 1 << 45, 1 << 46, 1 << 47, 1 << 48]   # (apart from each other by more than the largest operand)
+    assert lib.xllm_mi355_rope_cos_sin(far[0], None, 0, 1 << 33, 1, 1.0, far[1], FP32, None) == ESHAPE
+    assert lib.xllm_mi355_rope_cos_sin(far[0], None, 0, 1 << 28, 64, 1.0, far[1], FP32, None) == ESHAPE
+    st = strides(64 * 64 + 1, 64)   # (not aligned: a lane per pair)
+    assert lib.xllm_mi355_rotary_embedding(far[0], far[1], 10, far[2], far[2], None, None, 1 << 22, 64, 0, 64, 0, 0, 0, 64, st, st,
+                                           None, None, 0, 0, BF16, FP32, None) == ESHAPE
+    assert lib.xllm_mi355_mla_norm_rope_and_cache(far[0], far[0], far[1], far[1], far[2], 1e-6, far[3], 10, far[4], None, None,
+                                                  1 << 23, 128, 512, 64, 8192, 64, 8192, 64, 576, 576, 16, 4, 1, BF16, FP32,
+                                                  None) == ESHAPE
+
+
 def test_differential_decode():
     lib = capi.lib()
     size = lib.xllm_mi355_paged_decode_diff_workspace_bytes

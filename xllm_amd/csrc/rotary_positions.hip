@@ -19,6 +19,7 @@ namespace xllm_mi355 {
 namespace {
 
 constexpr int kRotThreads = 256;
+constexpr int64_t kRotGroups = 0xffffffffLL / kRotThreads;   // a launch counts its threads in 32 bits
 
 // ---- element types ------------------------------------------------------------------------------------------------
 
@@ -178,7 +179,7 @@ int launch_cos_sin(const double* inv_freq, const int64_t* positions, int64_t fir
   const bool wide = half % V == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   const int64_t units = rows * (wide ? half / V : half);
   const int64_t groups = (units + kRotThreads - 1) / kRotThreads;
-  if (groups > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
+  if (groups > kRotGroups) return XLLM_MI355_ESHAPE;
   const dim3 grid(static_cast<unsigned>(groups));
   if (wide)
     rope_cos_sin_kernel<DT, V><<<grid, kRotThreads, 0, stream>>>(inv_freq, positions, first, units, static_cast<int>(half),
@@ -343,7 +344,7 @@ int launch_rotary(RotArgs a, bool copy_rest, int inverse, int64_t n_tokens, hipS
   a.units = a.rot_units + (copy_rest ? (wide - a.rot + 2 * P - 1) / (2 * P) : 0);
   a.n_units = n_tokens * (a.q.heads + a.k.heads) * a.units;
   const int64_t groups = (a.n_units + kRotThreads - 1) / kRotThreads;
-  if (groups > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
+  if (groups > kRotGroups) return XLLM_MI355_ESHAPE;
   rotary_kernel<DT, CT, INTERLEAVE, VEC><<<dim3(static_cast<unsigned>(groups)), kRotThreads, 0, stream>>>(
       a, inverse != 0 ? -1.0f : 1.0f);
   return static_cast<int>(hipGetLastError());
@@ -473,7 +474,7 @@ int launch_mla_prologue(MlaPrologueArgs a, hipStream_t stream) {
   a.q_units = a.n_tokens * a.heads * (kRopeDim / 16);
   const int64_t kv = (a.n_tokens + kRotThreads / kWave - 1) / (kRotThreads / kWave);
   const int64_t groups = kv + (a.q_units + kRotThreads - 1) / kRotThreads;
-  if (groups > 0x7fffffffLL) return XLLM_MI355_ESHAPE;
+  if (groups > kRotGroups) return XLLM_MI355_ESHAPE;
   a.kv_blocks = static_cast<int>(kv);
   mla_prologue_kernel<DT, CT, INTERLEAVE><<<dim3(static_cast<unsigned>(groups)), kRotThreads, 0, stream>>>(a);
   return static_cast<int>(hipGetLastError());
