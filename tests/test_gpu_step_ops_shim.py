@@ -1,4 +1,8 @@
 """The operators of a step through the C++ host side (torch.ops.xllm_ops.*): the same bits as xllm_amd.ops, and refusals."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -103,6 +107,45 @@ def test_differential_decode(xops):
                 (q, k, v, got, table, lens, lam.double(), 0.2), (q, k, v, got.float(), table, lens, lam, 0.2), (q, k, v, got, table, lens, lam, -1.0)):
         with pytest.raises((ValueError, TypeError)):
             xops.batch_decode_diff(*bad)
+
+
+_FIRST_CALLS = """
+import threading, torch
+from xllm_amd import ops
+N, D, pairs = 8, 128, 2
+dev = "cuda:0"
+q = torch.randn(3, 8, D, device=dev).to(torch.float16)
+k, v = torch.randn(40, 16, 2 * pairs, D, device=dev).half(), torch.randn(40, 16, pairs, 2 * D, device=dev).half()
+table = torch.arange(39, device=dev).view(3, 13).to(torch.int32)
+lens, lam = torch.tensor([200, 0, 33], dtype=torch.int32, device=dev), torch.rand(4, device=dev)
+outs = [torch.zeros(3, 4, 2 * D, dtype=torch.float16, device=dev) for _ in range(N)]
+ready, errors = threading.Barrier(N), []
+torch.cuda.synchronize()
+
+def first(out):
+    try:
+        ready.wait()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            ops.batch_decode_diff(q, k, v, out, table, lens, lam)
+    except Exception as e:
+        errors.append(e)
+
+threads = [threading.Thread(target=first, args=(o,)) for o in outs]
+[t.start() for t in threads]
+[t.join() for t in threads]
+torch.cuda.synchronize()
+assert not errors, errors
+want = ops.batch_decode_diff(q, k, v, torch.empty_like(outs[0]), table, lens, lam)
+assert all(torch.equal(o, want) for o in outs)
+print("first calls agree")
+"""
+
+
+def test_first_calls_of_several_threads():
+    """The first calls of a process come from eight threads at once: all of them find the kernel set up."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", _FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "first calls agree" in done.stdout, done.stdout + done.stderr
 
 
 def test_results_count_as_written_in_place(xops):

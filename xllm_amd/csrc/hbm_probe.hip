@@ -83,11 +83,11 @@ int xllm_mi355_stream_read(const void* src, size_t bytes, void* sink, void* stre
   if (src == nullptr || (reinterpret_cast<uintptr_t>(src) & 15) != 0 || bytes % 16 != 0) return XLLM_MI355_EALIGN;
   if (bytes == 0) return XLLM_MI355_OK;
   static std::atomic<uint64_t> configured{0};
-  if (first_use_on_current_device(configured)) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(stream_read_kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, kReadLds);
-    if (e != hipSuccess) return static_cast<int>(e);
-  }
+  const hipError_t e = once_per_device(configured, [] {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(stream_read_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                               kReadLds);
+  });
+  if (e != hipSuccess) return static_cast<int>(e);
   int dev = 0, cus = 256;
   if (hipGetDevice(&dev) == hipSuccess) (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
   launch_timed(stream_read_kernel, dim3(cus > 0 ? cus : 256), dim3(256), kReadLds, static_cast<hipStream_t>(stream),

@@ -261,15 +261,18 @@ struct Region {
   }
 };
 
-// Kernel attributes (dynamic LDS size) are set per device.  Returns true the first time it is called with
-// `seen` on the current device (devices 0..63; beyond that always true: setting them again is harmless).
-inline bool first_use_on_current_device(std::atomic<uint64_t>& seen) {
+// Kernel attributes (dynamic LDS size) are set per device: `set` is called until it has succeeded once on the current device
+// (devices 0..63; beyond that always, setting them again is harmless).  The device is marked behind the success, so that a
+// thread which finds it marked launches with the attributes set, and one that comes at the same time sets them too.
+template <typename Set>
+inline hipError_t once_per_device(std::atomic<uint64_t>& done, Set set) {
   int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev > 63) return true;
-  const uint64_t bit = 1ull << dev;
-  if ((seen.load(std::memory_order_acquire) & bit) != 0) return false;
-  seen.fetch_or(bit, std::memory_order_acq_rel);
-  return true;
+  const bool known = hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev <= 63;
+  const uint64_t bit = known ? 1ull << dev : 0;
+  if ((done.load(std::memory_order_acquire) & bit) != 0) return hipSuccess;
+  const hipError_t e = set();
+  if (e == hipSuccess) done.fetch_or(bit, std::memory_order_acq_rel);
+  return e;
 }
 
 // Compute units of the current device, looked up once per device (a process may drive several GPUs, and they need

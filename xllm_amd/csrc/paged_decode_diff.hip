@@ -796,13 +796,12 @@ __global__ __launch_bounds__(WAVES * kWave) void diff_merge_kernel(DiffArgs a) {
 template <typename QT, int D, int NB>
 int launch_diff(const DiffArgs& a, hipStream_t stream) {
   using S = DiffShape<D, NB>;
-  static std::atomic<uint64_t> seen{0};
-  const void* kern = reinterpret_cast<const void*>(diff_decode_kernel<QT, D, NB>);
-  if (first_use_on_current_device(seen)) {
-    const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(S::lds_bytes(kDiffMaxBatch)));
-    if (e != hipSuccess) return static_cast<int>(e);
-  }
+  static std::atomic<uint64_t> configured{0};
+  const hipError_t e = once_per_device(configured, [] {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(diff_decode_kernel<QT, D, NB>),
+                               hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::lds_bytes(kDiffMaxBatch)));
+  });
+  if (e != hipSuccess) return static_cast<int>(e);
   launch_timed(diff_decode_kernel<QT, D, NB>, dim3(static_cast<unsigned>(a.n_workers / S::kWaves)), dim3(S::kThreads),
                S::lds_bytes(a.batch), stream, a);
   int rc = static_cast<int>(hipGetLastError());

@@ -1968,12 +1968,11 @@ int launch_gqa_mfma(GqaArgs& a, size_t workspace_bytes, hipStream_t stream, bool
   static_assert(Lay::kPrefixOff + (kMaxBatch + 2) * 4 <= 160 * 1024, "LDS of a CU");
   auto kern = gqa_mfma_kernel<QT, FP8, NS, VL, D>;
   static std::atomic<uint64_t> configured{0};
-  if (first_use_on_current_device(configured)) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             Lay::kPrefixOff + (kMaxBatch + 2) * 4);
-    if (e != hipSuccess) return static_cast<int>(e);
-  }
+  const hipError_t e = once_per_device(configured, [&] {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                               Lay::kPrefixOff + (kMaxBatch + 2) * 4);
+  });
+  if (e != hipSuccess) return static_cast<int>(e);
   configure_mfma(a, FP8, D, VL);
   const int n_wg = a.n_workgroups / kWaves;
   const size_t part_floats = static_cast<size_t>(a.n_workgroups) * 2 * kMfmaHeads * (D + 1);

@@ -2668,7 +2668,7 @@ int paged_decode_mla(const void* q_nope, const void* q_pe, const void* k_cache, 
                                           : (n_heads + kHeadsPerWg16 - 1) / kHeadsPerWg16);
   static std::atomic<uint64_t> configured{0};
   const size_t smem = pairs ? kPrefixOff + (kMaxBatchMla + 1) * 4 : kPrefix16Off + (kMaxBatchMla + 1) * 4;
-  if (first_use_on_current_device(configured)) {
+  const hipError_t rc_attributes = once_per_device(configured, [&] {
     hipError_t e = hipSuccess;
     const int lds_pairs = static_cast<int>(kPrefixOff + (kMaxBatchMla + 1) * 4);
     const int lds_16 = static_cast<int>(kPrefix16Off + (kMaxBatchMla + 1) * 4);
@@ -2690,8 +2690,9 @@ int paged_decode_mla(const void* q_nope, const void* q_pe, const void* k_cache, 
                                 reinterpret_cast<const void*>(mla_decode_w4_kernel<FP16>)};
     for (const void* k : kernels_w4)
       if (e == hipSuccess) e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kW4LdsBytes);
-    if (e != hipSuccess) return static_cast<int>(e);
-  }
+    return e;
+  });
+  if (rc_attributes != hipSuccess) return static_cast<int>(rc_attributes);
   // The step's new rows: inside mla_decode_w4_kernel where it serves the call and the rows can be fetched 16 bytes at
   // a time; otherwise the store is a launch of its own before the decode, with the same result.
   const bool w4_call = w4_serves(n_heads, block_size);
