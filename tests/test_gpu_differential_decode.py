@@ -460,6 +460,41 @@ def test_prefill_and_decode_steps_of_differential_attention():
         kv, table, head = t.seq_lens, t.block_table, t.counters[1:2]
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_every_token_of_a_chunk_attends(dtype):
+    """Chunks and decode rows of a step, each new token a row of its own with its request's pages and its position + 1 as its
+    length (causal attention of a chunk by the single-token form), then a padded batch of them."""
+    B, H, pairs, D, bs, T = 4, 4, 2, 64, 16, 64
+    W, pool = 8, 24
+    i32 = dict(dtype=torch.int32, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    k_cache = torch.full((pool, bs, 2 * pairs, D), float("nan"), dtype=dtype, device=DEV)
+    v_cache = torch.full((pool, bs, pairs, 2 * D), float("nan"), dtype=dtype, device=DEV)
+    free, head = torch.randperm(pool, generator=torch.Generator().manual_seed(4)).to(**i32), torch.zeros(1, **i32)
+    kv, table, lam = torch.zeros(B, **i32), torch.full((B, W), -1, **i32), lam_of(H)
+    for new in ([17, 1, 0, 33], [1, 16, 5, 1], [20, 1, 1, 1]):
+        t = ops.build_step_tables(kv, torch.tensor(new, **i32), table, free, bs, T, head)
+        n = sum(new)
+        q, k = (torch.randn(T, 2 * h, D, generator=gen, device=DEV).to(dtype) for h in (H, pairs))
+        v = torch.randn(T, pairs, 2 * D, generator=gen, device=DEV).to(dtype)
+        ops.reshape_paged_cache(ops.ReshapePagedCacheParams(key=k, value=v.view(T, 2 * pairs, D), k_cache=k_cache,
+                                                            v_cache=v_cache.view(pool, bs, 2 * pairs, D),
+                                                            slot_mapping=t.slot_mapping))
+        row = torch.repeat_interleave(torch.arange(B, device=DEV), torch.tensor(new, device=DEV), output_size=n)
+        row = torch.cat([row, torch.zeros(T - n, dtype=row.dtype, device=DEV)])
+        lens = torch.where(torch.arange(T, device=DEV) < n, t.position_ids + 1, 0).to(torch.int32)   # (padding: empty rows)
+        rows = t.block_table[row].contiguous()
+        out = torch.full((T, H, 2 * D), 7.0, dtype=dtype, device=DEV)
+        ops.batch_decode_diff(q, k_cache, v_cache, out, rows, lens, lam)
+        p = dict(q=q, k=k_cache, v=v_cache, table=rows, lens=lens)
+        want, bound = reference(p, H, pairs, D, bs, lam, D ** -0.5, None, 0.0, 1.0)
+        assert ((out.double() - want).abs() <= bound).all() and (out[n:] == 0).all()
+        few = torch.full((T, H, 2 * D), 7.0, dtype=dtype, device=DEV)   # (only the rows that are there: the others stay)
+        ops.batch_decode_diff(q[:n], k_cache, v_cache, few[:n], rows[:n], lens[:n], lam)
+        assert ((few[:n].double() - want[:n]).abs() <= bound[:n]).all() and (few[n:] == 7).all()
+        kv, table, head = t.seq_lens, t.block_table, t.counters[1:2]
+
+
 def test_mla_step_from_lengths_to_attention():
     """tables -> MLA prologue -> dense_decode, against the same rows attended in 64 bits."""
     B, H, bs, pool, T = 4, 16, 64, 20, 4
