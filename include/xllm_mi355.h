@@ -583,8 +583,8 @@ int xllm_mi355_build_step_tables(const int32_t* kv_lens, const int32_t* new_lens
 /*
  * cos | sin rows for the rotary entry points of this library, out[r, i] = factor * cos(angle), out[r, half + i] = factor *
  * sin(angle), angle = position(r) * inv_freq[i], with the angle and its reduction in 64 bits (a 32-bit angle at position
- * 10^5 is off by 4e-3) and one rounding to out_dtype; angles up to 2^50 in magnitude.  position(r) = positions[r], or first_position + r where positions is
- * null.  Frequencies scaled for long contexts (the reference's rotary_embedding files in
+ * 10^5 is off by 4e-3), rounded to fp32 and from there to a 16-bit out_dtype; angles up to 2^50 in magnitude.  position(r) =
+ * positions[r], or first_position + r where positions is null; a position's row is the same bits either way.  Frequencies scaled for long contexts (the reference's rotary_embedding files in
  * xllm/core/layers/common/) are the caller's inv_freq and factor; ops.rope_frequencies makes them.
  * inv_freq: [half] fp64; out: [n_rows, 2 * half] contiguous, of out_dtype (fp32, bf16, fp16).  half up to 4096.  A lane makes
  * 4 pairs of fp32 or 8 of the 16-bit types (one where half or out is no multiple of 16 bytes); one call takes up to 2^32 lanes.
@@ -648,7 +648,8 @@ int xllm_mi355_mla_norm_rope_and_cache(const void* q_pe, void* q_pe_out, const v
  * lambda: fp32 with strides in elements (0 where a sequence or a head shares it).  norm_weight [2 head_dim] of `dtype`.
  * block_table [batch, table_stride], of which table_width entries are valid: longer contexts are cut there.  window_left
  * as in xllm_mi355_paged_decode_gqa.  A sequence with seq_lens[b] <= 0 gets out = 0.  Page ids are clamped into the cache.
- * dtype (queries, caches, output): bf16 or fp16.  head_dim 64 or 128; any block size.  The attended tokens that a table
+ * dtype (queries, caches, output): bf16 or fp16.  Probabilities are kept to 2^-16 (bf16) or 2^-22 (fp16) of themselves, in fp16
+ * not finer than 2^-39 of the largest.  head_dim 64 or 128; any block size.  The attended tokens that a table
  * row can hold (table_width * block_size, or the window) times the KV pairs stay below 2^35.
  * The workspace needs no initialisation; two calls that overlap in time need one each.
  */

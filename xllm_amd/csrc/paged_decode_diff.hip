@@ -17,8 +17,8 @@
 // nor other teams after the common prefix sum of the lengths.  A range that holds a whole context writes the output rows,
 // a part of a context goes to the workspace as (o, max, sum) in fp32 and diff_merge_kernel joins the parts.
 //
-// Data path.  Rows travel from global memory straight into a ring of the worker's own LDS (32 KB: two stages of 512-byte
-// rows, four of 256-byte rows), and the place of a stage's keys is filled again as soon as they are in registers, the
+// Data path.  Rows travel from global memory straight into a ring of the worker's own LDS (two stages: 32 KB for 512-byte
+// rows, 16 KB for 256-byte rows, of which a CU has twice the workers), and the place of a stage's keys is filled again as soon as they are in registers, the
 // place of its values likewise.  Page-table entries take the same path two ring lengths ahead, so that no load of the
 // loop waits in a register (such a wait would also wait for every younger row in flight: the counter is in order).
 //   S^T[token, column] = K[token, dims] . Q^T        v_mfma_f32_16x16x32, K read from LDS, Q^T in registers

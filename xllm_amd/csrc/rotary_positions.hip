@@ -137,7 +137,7 @@ __device__ __forceinline__ void row_pairs(double pos, const double (&freq)[V], d
 // that a listed position has, and some values fell on the other side of their rounding.)
 // One lane makes V consecutive pairs of a row: V cosines and V sines, 16 bytes of each where the row allows it.  Bound by the
 // launch (64 rows of 128 values: 2.1 us), beyond that by 17 operations in 64 bits a pair, at half the rate of those in 32, on
-// top of the stores: 131072 rows of 128 values 14.5 us in fp32, where the stores alone take 11.9 us and a plain fill of as many
+// top of the stores: 131072 rows of 128 values 14.0 us in fp32, where the stores alone take 11.9 us and a plain fill of as many
 // bytes 11.4 us, and 13.3 us in bf16.  (Several rows a lane: the same.)
 template <int DT, int V>
 __global__ __launch_bounds__(kRotThreads) void rope_cos_sin_kernel(const double* inv_freq, const int64_t* positions,
@@ -259,7 +259,7 @@ __device__ __forceinline__ void turn_words(Pack<DT, P>& x, Pack<DT, P>& y, const
 // words each, at neighbouring words in neighbouring lanes.  One head per lane: with four (one set of cosines and sines for
 // all of them, four times the bytes in flight per lane) 8192 tokens of 40 heads took the same 27 us, 4097 tokens of 20
 // heads with a copied rest 28 instead of 19 us, for want of wavefronts.  Bound by the bytes: 8192 tokens of 40 heads of 128
-// bf16 values in place (172 MB with the table's rows) 27.2 us = 6.3 TB/s, 4097 tokens of 20 heads of 256 fp16 values to
+// bf16 values (172 MB with the table's rows) 27.2 us to another place = 6.3 TB/s and 27.9 us in place, 4097 tokens of 20 heads of 256 fp16 values to
 // another place, 64 of them rotated (84 MB), 17.2 us = 4.9 TB/s; a large copy runs at 5.2 TB/s.
 // VEC = false takes one pair (or two elements to copy) per lane, for operands that are not aligned to 16 bytes.
 template <int DT, int CT, bool INTERLEAVE, bool VEC>

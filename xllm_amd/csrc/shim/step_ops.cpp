@@ -1,7 +1,8 @@
 // The operators around the decode path on the host side: torch::Tensor arguments checked, unpacked and handed to the C ABI
 // on the current HIP stream of the tensors' device.  Registered with the dispatcher as torch.ops.xllm_ops.*; the Python
 // functions of the same names call the same code through step_ops_python.cpp.  The checks cost a microsecond here and five
-// in Python.  A violated precondition is a ValueError or a TypeError.
+// in Python.  A violated precondition is a ValueError or a TypeError; what the library itself refuses -- rows off the 16-byte
+// boundary, sizes that it has no kernel for -- is a RuntimeError with its words.
 #include <ATen/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>

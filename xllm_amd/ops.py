@@ -938,7 +938,7 @@ def rope_frequencies(rotary_dim, base=10000.0, scaling=None, seq_len=0, device="
 def build_cos_sin_cache(inv_freq, num_positions=0, position_ids=None, first_position=0, attention_factor=1.0,
                         dtype=torch.float32, out=None):
     """cos | sin rows [rows, rotary_dim] for fused_qk_norm_rope, rotary_embedding and mla_norm_rope_and_cache, angles in 64
-    bits, rounded once to dtype (float32, bfloat16 or float16).  Rows of position_ids [rows] int64 -- one step's rows,
+    bits, rounded to float32 and from there to dtype (float32, bfloat16 or float16); a position's row is always the same bits.  Rows of position_ids [rows] int64 -- one step's rows,
     shared by all layers, which then index them by 0 .. rows - 1 -- or of first_position .. first_position + num_positions - 1.
     inv_freq, attention_factor: from rope_frequencies.  Returns the rows (out, if given)."""
     return _host_side().build_cos_sin_cache(inv_freq, position_ids, num_positions, first_position, attention_factor, dtype, out)
@@ -985,7 +985,8 @@ def batch_decode_diff(query, k_cache, v_cache, output, block_table, seq_lens, la
     the same bytes, so reshape_paged_cache stores both); output [B, H, 2 D]; block_table [B, W] and seq_lens [B] int32 as in
     batch_decode: an empty sequence gets zeros, a context beyond the table is cut there.  lambda_: the layer's learned
     weight as float32, one value, [H], or [B, H].  norm_weight [2 D] of query's dtype; out_scale: usually 1 - lambda_init.
-    window_left >= 0: the last window_left + 1 tokens only.  bfloat16 or float16; D 64 or 128.  Returns output."""
+    window_left >= 0: the last window_left + 1 tokens only.  bfloat16 or float16 (whose probabilities end at 2^-39 of the
+    largest); D 64 or 128.  Returns output."""
     if scale is None:
         scale = query.shape[-1] ** -0.5
     _host_side().batch_decode_diff(query, k_cache, v_cache, output, block_table, seq_lens, lambda_, scale, norm_weight, eps,
