@@ -1,4 +1,6 @@
 """Differential paged decode against its definition in 64 bits, and the operators of a step run together."""
+import math
+
 import pytest
 import torch
 
@@ -376,6 +378,37 @@ def test_small_probabilities_beside_a_sink(dtype, nats, D, H, pairs):
             want, bound = sink_reference(some, H, pairs, D, 16, lam, weight, eps, scale)
             worst = ((got.double() - want).abs() / bound).max().item()
             assert worst <= 1.0, f"{len(lens)} contexts, lambda {lam}: error is {worst:.2f} of its bound"
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("power", [10, 23, 24, 25, 26, 27, 28])
+def test_scores_beyond_the_integers_of_fp32(dtype, power):
+    """Equal scores of 2^power and a few units more (log2 units), where the running maximum and what is held against it are no
+    longer a few powers of two apart but a few steps of fp32; the second 16 tokens of a context lie 16 units higher."""
+    D, bs, n = 64, 16, 40
+    lens = [n] * 24
+    p = problem(lens, 1, 1, D, bs, dtype, seed=power)
+    p["q"].zero_(), p["k"].zero_()
+    step = max(1, 2 ** (power - 23))
+    a = power // 2
+    for b in range(len(lens)):   # score = 2^a 2^(power - a) + step b (+ 16): products and sums that fp32 holds exactly
+        t = torch.arange(n, device=DEV)
+        slot = p["table"][b, t // bs].long() * bs + t % bs
+        p["q"][b, :, 0], p["q"][b, :, 1], p["q"][b, :, 2] = 2.0 ** a, float(step), 16.0
+        k = p["k"].view(-1, 2, D)
+        k[slot, :, 0], k[slot, :, 1] = 2.0 ** (power - a), float(b)
+        k[slot[16:], :, 2] = 1.0 if b % 2 else 0.0
+    got = run(p, 1, D, torch.tensor(0.25, device=DEV), scale=math.log(2))
+    for b in range(len(lens)):
+        t = torch.arange(n, device=DEV)
+        slot = p["table"][b, t // bs].long() * bs + t % bs
+        v = p["v"].view(-1, 2 * D)[slot].double()
+        # (up to 2^23 the higher tokens have 2^16 of the others' weight; beyond, the sum may round it away or to a step more)
+        alike = (v[:16].sum(0) * 2.0 ** -16 + v[16:].sum(0)) / (16 * 2.0 ** -16 + 24)
+        wants = [v.mean(0)] if b % 2 == 0 else [alike] if power <= 23 else [alike, v[16:].mean(0), v.mean(0)]
+        half = torch.finfo(dtype).eps / 2
+        errs = [((got[b, 0].double() - 0.75 * w).abs() - 2 * half * w.abs()).max().item() for w in wants]
+        assert min(errs) <= 1e-4, (b, errs)
 
 
 @pytest.mark.parametrize("D,H,pairs", [(128, 4, 2), (64, 12, 1)])

@@ -72,7 +72,7 @@ constexpr int64_t kDiffStreamRows = 4096;
 // and moves when a score passes it by more than kLift + kSlack, so that e = exp2(s - m) stays below 2^(kLift + kSlack).
 // bf16 has fp32's range, and a wide slack keeps the moves rare.  fp16 ends at 2^16: the slack is what it can be with the
 // probabilities at the top of its range.  The moves that this adds (some two a context) are not seen in the times but for the
-// shape with the most accumulators (64 sequences, 64 heads of 128 dims, groups of sixteen: 132.3 us, 128.8 with bf16's values).
+// shape with the most accumulators (64 sequences, 64 heads of 128 dims, groups of sixteen: 133.0 us in fp16, 128.0 in bf16).
 template <typename QT>
 struct DiffProbs {
   static constexpr float kLift = QT::kIsBf16 ? 0.0f : 14.0f;
@@ -590,12 +590,13 @@ __global__ __launch_bounds__((DiffShape<D, NB>::kThreads), (DiffShape<D, NB>::kP
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         sv[r] = tok0 + r < cc.L && tok0 + r >= cc.lo ? sc[nb][r] * a.scale_log2 : -INFINITY;
-        over |= sv[r] > m[nb] + kTop;
+        over |= sv[r] - m[nb] > kTop;
       }
       if (__builtin_amdgcn_ballot_w64(over) != 0) {   // rare once the maxima have settled
         const float mx = diff_rows_max(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])));
-        if (mx > m[nb] + kTop) {
-          const float top = mx - DiffProbs<QT>::kLift;
+        if (mx - m[nb] > kTop) {
+          // (scores beyond 2^24, whose steps are wider than 1: where the lift is rounded up to 2^16 of weight, none)
+          const float lifted = mx - DiffProbs<QT>::kLift, top = mx - lifted > kTop ? mx : lifted;
           const float alpha = fast_exp2(m[nb] - top);
           m[nb] = top;
           l[nb] *= alpha;
