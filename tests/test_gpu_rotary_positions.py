@@ -351,6 +351,28 @@ def test_rotation_refusals():
             ops.rotary_embedding(*args, **kw)
 
 
+def test_lanes_beyond_31_bits():
+    """Tables and operands off the 16-byte boundary take a lane per pair: more than 2^31 of them."""
+    inv, _ = ops.rope_frequencies(66, device=DEV)
+    n = 2 ** 31 // 33 + 1000
+    rows = ops.build_cos_sin_cache(inv, n, dtype=BF16)
+    assert rows.numel() // 2 > 2 ** 31
+    few = torch.cat([torch.arange(50), torch.arange(n // 2, n // 2 + 50), torch.arange(n - 1100, n)]).to(DEV)
+    assert torch.equal(rows[few], ops.build_cos_sin_cache(inv, position_ids=few, dtype=BF16))
+    del rows
+    T, H, D = 2 ** 19 + 3, 64, 128
+    buf = torch.zeros(T * H * D + 1, dtype=BF16, device=DEV)
+    q = buf[1:].view(T, H, D)
+    table, pos = table_of(64, D, FP32), torch.arange(T, device=DEV) % 64
+    at = torch.tensor([0, 1, T // 2, T - 4, T - 1], device=DEV)
+    part = torch.randn(5, H, D, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(BF16)
+    q[at] = part
+    ops.rotary_embedding(pos, q, None, table)
+    assert torch.equal(q[at], ops.rotary_embedding(pos[at], part, None, table)[0])
+    q[at] = 0
+    assert buf[:2 ** 30].count_nonzero() == 0 and buf[-2 ** 30:].count_nonzero() == 0
+
+
 # ------------------------------------------------------------------------------------------
 # MLA prologue
 
